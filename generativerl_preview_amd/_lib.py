@@ -13,6 +13,7 @@ LIB_PATH = os.environ.get("GRLHIP_LIB") or os.path.join(_HERE, "libgrlhip.so")
 
 MAX_HIDDEN = 8
 F32, BF16 = 0, 1
+ELEM_F32, ELEM_BF16, ELEM_F16 = 0, 1, 2
 NET_RESNET, NET_CONCAT_MLP, NET_QNET = 0, 1, 2
 COEF_STRIDE = 12
 
@@ -75,6 +76,10 @@ PROTOTYPES = {
                                         ctypes.c_float, ctypes.c_float, _i64, _vp]),
     "grlhip_adam_step_counted": (ctypes.c_int, [_vp, _vp, _vp, _vp, _i64, ctypes.c_float, ctypes.c_float, ctypes.c_float,
                                                 ctypes.c_float, ctypes.c_float, _vp, ctypes.c_int, _vp]),
+    "grlhip_orthogonalize_workspace_bytes": (_sz, [_vp, _i32]),
+    "grlhip_orthogonalize": (ctypes.c_int, [_vp, _vp, _vp, _vp, _i32, ctypes.c_int, _i32, _f, _f, _f, _f, _vp, _sz, _vp]),
+    "grlhip_muon_step": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i32, ctypes.c_double, ctypes.c_int, _f, _i32, _f, _f, _f, _f,
+                                        _vp, _sz, _vp]),
     "grlhip_cep_loss_fwd_bwd": (ctypes.c_int, [_vp, _vp, ctypes.c_int, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _vp,
                                                _i64, _vp, _sz, _vp]),
 }

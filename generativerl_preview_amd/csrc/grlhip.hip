@@ -8,6 +8,7 @@
 #include <mutex>
 #include <string>
 
+#include "errors.hpp"
 #include "plan.hpp"
 using namespace grlhip;
 
@@ -63,6 +64,14 @@ int check_ready(const grlhip_plan* plan, const void* packed) {
 }
 
 }  // namespace
+
+int grlhip::set_error(int code, const std::string& message) noexcept {   // for the other translation units (errors.hpp)
+  try {
+    return fail(code, message);
+  } catch (...) {
+    return code;
+  }
+}
 
 // torch.optim.Adam's update (amsgrad / maximize off) over flat buffers, one thread per 4 elements
 typedef float f32x4 __attribute__((ext_vector_type(4)));

@@ -10,11 +10,22 @@ of the FlatGrads buffer the fused losses accumulate into.  ``step()`` is one ker
 
 ``capturable=True`` keeps the step count on the device (grlhip_adam_step_counted), as ``torch.optim.Adam(capturable=True)``
 does: a whole training step -- loss forward + backward, gradient all-reduce, ``step()`` -- can then be captured once with
-``torch.cuda.graph`` and replayed (``tests/test_optim.py``)."""
+``torch.cuda.graph`` and replayed (``tests/test_optim.py``).
+
+``orthogonalize`` / ``muon_step`` / ``FlatMuon`` are the matrix-aware step beside it (grlhip_orthogonalize,
+grlhip_muon_step): the momentum of every weight matrix is orthogonalised by a Newton-Schulz iteration before it is applied,
+all matrices of a network in the same chain of launches; biases and other vectors keep Adam."""
+import ctypes
+import math
+
 import torch
 
 from . import _lib as L
 from .distributed import attach_flat_grads
+from .engine import _ptr, _stream
+
+NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)   # a, b, c: 5 steps bring singular values from 0.002 on into [0.68, 1.21]
+_ELEM = {torch.float32: L.ELEM_F32, torch.bfloat16: L.ELEM_BF16, torch.float16: L.ELEM_F16}
 
 
 class FlatAdam:
@@ -104,3 +115,183 @@ class FlatAdam:
         self.exp_avg.copy_(sd["exp_avg"])
         self.exp_avg_sq.copy_(sd["exp_avg_sq"])
         self.param_groups[0].update(sd["param_groups"][0])
+
+
+def _matrices(tensors, name, shapes=None, written=False):
+    """Checks a list of 2-D tensors on one HIP device; returns their shapes."""
+    dev = tensors[0].device
+    seen = set()
+    for i, t in enumerate(tensors):
+        if not t.is_cuda:
+            raise L.GrlHipError("%s[%d] must live on a HIP device (got %s): there is no CPU fallback" % (name, i, t.device))
+        if t.device != dev or t.dtype != tensors[0].dtype:
+            raise ValueError("%s[%d]: all matrices must be on one device and of one type (%s %s, got %s %s)" %
+                             (name, i, dev, tensors[0].dtype, t.device, t.dtype))
+        if t.dim() != 2:
+            raise ValueError("%s[%d]: expected a matrix, got shape %s" % (name, i, tuple(t.shape)))
+        if shapes is not None and t.shape != shapes[i]:
+            raise ValueError("%s[%d]: expected shape %s, got %s" % (name, i, tuple(shapes[i]), tuple(t.shape)))
+        if written and t.numel():
+            if t.data_ptr() in seen or any(st == 0 and n > 1 for st, n in zip(t.stride(), t.shape)):
+                raise ValueError("%s[%d] is written to and must not share memory with itself or another of them" % (name, i))
+            seen.add(t.data_ptr())
+    return [t.shape for t in tensors]
+
+
+def _pointers(tensors):
+    return (ctypes.c_void_p * len(tensors))(*[t.data_ptr() for t in tensors])
+
+
+def _shape_array(shapes):
+    return (ctypes.c_int64 * (2 * len(shapes)))(*[n for s in shapes for n in s])
+
+
+def _stride_array(*lists):
+    """[count][6] element strides of up to three lists of matrices, or None when all are dense."""
+    if all(t.is_contiguous() for ts in lists for t in ts):
+        return None
+    lists = lists + (lists[0],) * (3 - len(lists))
+    return (ctypes.c_int64 * (6 * len(lists[0])))(*[v for ts in zip(*lists) for t in ts for v in t.stride()])
+
+
+def _newton_schulz_workspace(shapes, count, device):
+    need = L.lib().grlhip_orthogonalize_workspace_bytes(shapes, count)
+    if need == 0:
+        raise L.GrlHipError(L.lib().grlhip_last_error().decode())
+    # one per call: calls on different streams and captured graphs must not share it
+    return torch.empty(need, dtype=torch.uint8, device=device)
+
+
+@torch.no_grad()
+def orthogonalize(matrices, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7):
+    """Newton-Schulz orthogonalisation: ``steps`` times ``X <- a X + (b A + c A A) X`` with ``A = X X^T``, from
+    ``X = G / max(|G|_F, eps)`` (grlhip_orthogonalize).  ``matrices``: a tensor ``(..., rows, cols)`` -- every matrix of it on
+    its own -- or a list of such tensors, fp32, bf16 or fp16, any strides; all of them go through one chain of launches.
+    Returns new tensors of the same shapes and type.  Products are fp32 (two fp16 pieces per value), rounded to the type once at the end.
+    No gradient is recorded.  A matrix that holds an infinity or NaN comes back as NaN, a zero matrix as zeros."""
+    single = torch.is_tensor(matrices)
+    tensors = [matrices] if single else list(matrices)
+    if not tensors:
+        return []
+    for i, t in enumerate(tensors):
+        if t.dim() < 2:
+            raise ValueError("matrices[%d]: expected (..., rows, cols), got shape %s" % (i, tuple(t.shape)))
+        if t.dtype not in _ELEM:
+            raise TypeError("matrices[%d]: expected float32, bfloat16 or float16, got %s" % (i, t.dtype))
+    # batches as lists of matrices; a view where the strides allow one
+    flat = [t if t.dim() == 2 else t.reshape(-1, *t.shape[-2:]) if t.numel() else t.new_empty(0, *t.shape[-2:]) for t in tensors]
+    out = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in flat]
+    src = [m for t in flat for m in (t.unbind(0) if t.dim() == 3 else (t,))]
+    dst = [m for t in out for m in (t.unbind(0) if t.dim() == 3 else (t,))]
+    if src:
+        shapes = _shape_array(_matrices(src, "matrices"))
+        dev = src[0].device
+        a, b, c = (float(v) for v in coefficients)
+        ws = _newton_schulz_workspace(shapes, len(src), dev)
+        with torch.cuda.device(dev):
+            L.check(L.lib().grlhip_orthogonalize(_pointers(src), _pointers(dst), shapes, _stride_array(src, dst), len(src),
+                                                 _ELEM[src[0].dtype], int(steps), a, b, c, float(eps), _ptr(ws), ws.numel(),
+                                                 _stream(dev)))
+    out = [o.view(t.shape) for o, t in zip(out, tensors)]
+    return out[0] if single else out
+
+
+@torch.no_grad()
+def muon_step(params, grads, momentum_buffers, lr, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5,
+              coefficients=NEWTON_SCHULZ, eps=1e-7, adjust_lr="original"):
+    """One step, in place, of lists of fp32 matrices (grlhip_muon_step):
+        buf = momentum buf + (1 - momentum) grad;   u = (1 - momentum) grad + momentum buf if nesterov else buf
+        param = (1 - lr weight_decay) param - lr' orthogonalize(u)
+    with lr' = lr sqrt(max(1, rows / cols)) for ``adjust_lr="original"`` and 0.2 lr sqrt(max(rows, cols)) for
+    ``"match_rms_adamw"`` (updates of the size of Adam's).  Any strides; the three lists must not share memory.  ``lr`` and the
+    other numbers are read on the host: a captured graph keeps the ones it was captured with."""
+    params, grads, bufs = list(params), list(grads), list(momentum_buffers)
+    if not len(params) == len(grads) == len(bufs):
+        raise ValueError("muon_step: %d parameters, %d gradients, %d momentum buffers" % (len(params), len(grads), len(bufs)))
+    if lr < 0.0 or not 0.0 <= momentum < 1.0 or weight_decay < 0.0 or not eps > 0.0:
+        raise ValueError("invalid Muon hyper-parameters")
+    if adjust_lr not in ("original", "match_rms_adamw"):
+        raise ValueError("adjust_lr: expected 'original' or 'match_rms_adamw', got %r" % (adjust_lr,))
+    if not params:
+        return
+    shapes = _matrices(params, "params", written=True)
+    _matrices(grads, "grads", shapes)
+    _matrices(bufs, "momentum_buffers", shapes, written=True)
+    dev = params[0].device
+    for name, ts in (("params", params), ("grads", grads), ("momentum_buffers", bufs)):
+        if ts[0].dtype != torch.float32:
+            raise TypeError("%s: expected float32, got %s" % (name, ts[0].dtype))
+        if ts[0].device != dev:
+            raise ValueError("%s are on %s, the parameters on %s" % (name, ts[0].device, dev))
+    if {t.data_ptr() for t in bufs if t.numel()} & {t.data_ptr() for ts in (params, grads) for t in ts if t.numel()} \
+            or {t.data_ptr() for t in params if t.numel()} & {t.data_ptr() for t in grads if t.numel()}:
+        raise ValueError("muon_step: parameters, gradients and momentum buffers must not share memory")
+    rates = (ctypes.c_float * len(params))(*[
+        lr * (math.sqrt(max(1.0, r / max(c, 1))) if adjust_lr == "original" else 0.2 * math.sqrt(max(r, c))) for r, c in shapes])
+    shape_arr = _shape_array(shapes)
+    a, b, c = (float(v) for v in coefficients)
+    ws = _newton_schulz_workspace(shape_arr, len(params), dev)
+    with torch.cuda.device(dev):
+        L.check(L.lib().grlhip_muon_step(_pointers(params), _pointers(grads), _pointers(bufs), shape_arr,
+                                         _stride_array(grads, params, bufs), rates, len(params), float(momentum),
+                                         int(nesterov), float(1.0 - lr * weight_decay), int(steps), a, b, c, float(eps),
+                                         _ptr(ws), ws.numel(), _stream(dev)))
+
+
+class FlatMuon(FlatAdam):
+    """Muon over the weight matrices of ``owner`` and Adam over everything else, on FlatAdam's flat buffers (the momentum of
+    a matrix takes the place of Adam's first moment there).  ``matrices(name, parameter)`` says which parameters are stepped
+    as matrices; by default every trainable one with at least two rows and columns (input and output layers may be better
+    off with Adam: name them there).  ``param_groups[1]`` holds Muon's numbers, ``param_groups[0]`` Adam's (``adam_*``)."""
+
+    def __init__(self, owner, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, coefficients=NEWTON_SCHULZ,
+                 eps=1e-7, adjust_lr="original", matrices=None, adam_lr=1e-3, adam_betas=(0.9, 0.999), adam_eps=1e-8,
+                 adam_weight_decay=0.0, capturable=False):
+        if lr < 0.0 or not 0.0 <= momentum < 1.0 or weight_decay < 0.0 or not eps > 0.0:
+            raise ValueError("invalid Muon hyper-parameters")
+        super().__init__(owner, lr=adam_lr, betas=adam_betas, eps=adam_eps, weight_decay=adam_weight_decay, capturable=capturable)
+        names = [name for name, _ in owner.plan.params]
+        if matrices is None:
+            matrices = lambda name, p: p.dim() == 2 and min(p.shape) > 1  # noqa: E731
+        self.matrix_names, chosen = [], []
+        for name, (p, off, cnt) in zip(names, self.fg.slices):
+            if p.requires_grad and matrices(name, p):
+                if p.dim() != 2:
+                    raise ValueError("FlatMuon: %s is no matrix (shape %s)" % (name, tuple(p.shape)))
+                self.matrix_names.append(name)
+                chosen.append((p, off, cnt))
+        views = lambda flat: [flat[off:off + cnt].view(p.shape) for p, off, cnt in chosen]  # noqa: E731
+        self._matrices = views(self.flat_params), views(self.fg.flat), views(self.exp_avg)
+        taken = {off for _, off, _ in chosen}
+        self.ranges = []
+        for p, off, cnt in sorted(self.fg.slices, key=lambda s: s[1]):
+            if not p.requires_grad or off in taken:
+                continue
+            if self.ranges and self.ranges[-1][1] == off:
+                self.ranges[-1][1] = off + cnt
+            else:
+                self.ranges.append([off, off + cnt])
+        picked = {id(p) for p, _, _ in chosen}
+        self.param_groups[0]["params"] = [p for p in self.param_groups[0]["params"] if id(p) not in picked]
+        self.param_groups.append(dict(lr=lr, momentum=momentum, nesterov=bool(nesterov), weight_decay=weight_decay, steps=steps,
+                                      coefficients=tuple(coefficients), eps=eps, adjust_lr=adjust_lr,
+                                      params=[p for p, _, _ in chosen]))
+
+    @torch.no_grad()
+    def step(self):
+        self._check_views()
+        self.fg.ensure()
+        muon_step(*self._matrices, **{k: v for k, v in self.param_groups[1].items() if k != "params"})
+        super().step()
+
+    def state_dict(self):
+        sd = super().state_dict()
+        sd["param_groups"].append({k: v for k, v in self.param_groups[1].items() if k != "params"})
+        sd["matrices"] = list(self.matrix_names)
+        return sd
+
+    def load_state_dict(self, sd):
+        if sd.get("matrices") != self.matrix_names:
+            raise ValueError("the state was saved for other matrices")
+        super().load_state_dict(sd)
+        self.param_groups[1].update(sd["param_groups"][1])

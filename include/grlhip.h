@@ -345,6 +345,33 @@ int grlhip_adam_step_counted(float* params, const float* grads, float* exp_avg, 
                              float beta1, float beta2, float eps, float weight_decay, void* step_record, int advance,
                              void* stream);
 
+/* Element types of the entry points below. */
+typedef enum { GRLHIP_ELEM_F32 = 0, GRLHIP_ELEM_BF16 = 1, GRLHIP_ELEM_F16 = 2 } grlhip_elem;
+
+/* No counterpart in the reference (its optimizers are elementwise).  Newton-Schulz orthogonalisation of `count` matrices in
+ * one chain of launches: dst_i = the result of `steps` times X <- a X + (b A + c A A) X, A = X X^T, from
+ * X = src_i / max(|src_i|_F, eps) (a matrix with more rows than columns is taken transposed).  Products at fp32 rounding level
+ * whatever the element type; one rounding to it at the end.
+ * `src`, `dst`: HOST arrays of device pointers; `shapes`: HOST [count][2] rows, columns (each 0..65536; 0: nothing to do for that matrix);
+ * `strides`: HOST [count][6] element strides (row, column) of src, dst and a third pair that is ignored here, or NULL for
+ * dense rows.  Host arrays are read before the call returns.  src_i == dst_i with the same strides is allowed.
+ * Coefficients that let a singular value pass 1.9 (or b s^2 + c s^4 pass 3.8) from 1 on: GRLHIP_ERR_UNSUPPORTED.
+ * The results do not depend on the other matrices of the call.  Workspace: grlhip_orthogonalize_workspace_bytes, 256-byte aligned. */
+size_t grlhip_orthogonalize_workspace_bytes(const int64_t* shapes, int32_t count);
+int grlhip_orthogonalize(const void* const* src, void* const* dst, const int64_t* shapes, const int64_t* strides,
+                         int32_t count, int elem, int32_t steps, float a, float b, float c, float eps,
+                         void* workspace, size_t workspace_bytes, void* stream);
+
+/* No counterpart in the reference.  One optimiser step of `count` fp32 weight matrices:
+ *   buf = momentum buf + (1 - momentum) grad;   u = nesterov ? (1 - momentum) grad + momentum buf : buf;
+ *   param = keep param - rates_i orthogonalize(u)          (keep = 1 - lr * weight_decay; rates: HOST [count])
+ * with the arguments of grlhip_orthogonalize; `strides`: HOST [count][6] of grad, param, buf, or NULL for dense rows.
+ * Parameters, gradients and buffers must not overlap.  Workspace: grlhip_orthogonalize_workspace_bytes. */
+int grlhip_muon_step(float* const* params, const float* const* grads, float* const* momentum_buffers,
+                     const int64_t* shapes, const int64_t* strides, const float* rates, int32_t count, double momentum,
+                     int nesterov, float keep, int32_t steps, float a, float b, float c, float eps,
+                     void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

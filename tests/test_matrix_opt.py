@@ -1,0 +1,328 @@
+"""orthogonalize / muon_step / FlatMuon (grlhip_orthogonalize, grlhip_muon_step) against the formulas in 64 bits.
+
+Tolerances, relative 2-norm.  A product of two-piece values is off by 2^-22 of the norms multiplied (dropped low x low and
+the pieces' own 2^-23 each), the fp32 sums by less; what a step leaves in the direction of a small singular value grows by
+a = 3.4445 in each of at most 4 further steps.  5 steps: 5 a^4 2^-22 = 1.7e-4, which single fp16 pieces (2^-11 in the place of
+2^-22) pass 1000 times.  A result in a 16-bit type is rounded once more, by half a step: eps / 2."""
+import copy
+import ctypes
+import math
+
+import pytest
+import torch
+
+import util_models as um
+from generativerl_preview_amd import _lib as L
+from generativerl_preview_amd import optim
+
+DEV = "cuda:0"
+ABC = (3.4445, -4.7750, 2.0315)
+TOL = 5 * 3.4445 ** 4 * 2.0 ** -22
+
+
+def polar(g, steps=5, abc=ABC, eps=1e-7):
+    x = g.detach().double().cpu()
+    tall = x.shape[0] > x.shape[1]
+    x = x.t() if tall else x
+    x = x / max(float(torch.linalg.vector_norm(x)), eps)
+    for _ in range(steps):
+        s = x @ x.t()
+        x = abc[0] * x + abc[1] * (s @ x) + abc[2] * (s @ (s @ x))
+    return x.t() if tall else x
+
+
+def off(got, want):
+    want = want.double().cpu()
+    return float(torch.linalg.vector_norm(got.double().cpu() - want)) / max(float(torch.linalg.vector_norm(want)), 1e-300)
+
+
+def tol(dtype):
+    return TOL + (0.0 if dtype == torch.float32 else torch.finfo(dtype).eps / 2)
+
+
+def grad_like(rows, cols, seed=0, dtype=torch.float32, scale=1e-3):
+    gen = torch.Generator().manual_seed(seed)
+    rank = max(1, min(rows, cols) // 2)
+    g = torch.randn(rows, rank, generator=gen) @ torch.randn(rank, cols, generator=gen) / math.sqrt(rank)
+    return ((g + 0.1 * torch.randn(rows, cols, generator=gen)) * scale).to(dtype).to(DEV)
+
+
+SHAPES = [(1, 1), (1, 9), (7, 1), (2, 2), (17, 32), (63, 65), (64, 64), (6, 1024), (512, 6), (128, 64), (129, 300), (257, 100),
+          (520, 400)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_gpu_orthogonalize_matches_the_iteration_in_64_bits(shape, dtype):
+    g = grad_like(*shape, dtype=dtype)
+    before = g.clone()
+    got = optim.orthogonalize(g)
+    assert got.shape == g.shape and got.dtype == dtype and got.device == g.device
+    assert torch.equal(g, before)
+    assert off(got, polar(g)) <= tol(dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(1000, 777), (1024, 1024), (300, 2500), (1300, 1300)])
+def test_gpu_orthogonalize_of_larger_matrices(shape):
+    g = grad_like(*shape, seed=3)
+    assert off(optim.orthogonalize(g), polar(g)) <= TOL
+
+
+@pytest.mark.gpu
+def test_gpu_orthogonalize_moves_singular_values_towards_one():
+    gen = torch.Generator().manual_seed(5)
+    g = torch.randn(200, 300, generator=gen).to(DEV)
+    s = torch.linalg.svdvals(optim.orthogonalize(g).double().cpu())
+    assert 0.5 < float(s.min()) and float(s.max()) < 1.2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("steps,abc", [(0, ABC), (1, ABC), (2, ABC), (8, (1.5, -0.5, 0.0)), (6, (1.875, -1.25, 0.375))])
+def test_gpu_orthogonalize_with_other_steps_and_coefficients(steps, abc):
+    g = grad_like(70, 90, seed=1)
+    assert off(optim.orthogonalize(g, steps=steps, coefficients=abc), polar(g, steps, abc)) <= TOL
+
+
+@pytest.mark.gpu
+def test_gpu_orthogonalize_takes_strides_batches_and_lists():
+    big = grad_like(300, 400, seed=2)
+    for view in (big.t(), big[10:75, 3:200], big[::2, ::3], big[:, 5:6].expand(300, 4), big.view(3, 100, 400)[1].t()[7:100]):
+        got = optim.orthogonalize(view)
+        assert got.shape == view.shape and off(got, polar(view)) <= TOL
+    batch = torch.stack([grad_like(40, 30, seed=k) for k in range(6)]).view(2, 3, 40, 30)
+    for b in (batch, batch.transpose(0, 1), batch.transpose(-1, -2)):
+        got = optim.orthogonalize(b)
+        assert got.shape == b.shape
+        for i in range(b.shape[0]):
+            for k in range(b.shape[1]):
+                assert off(got[i, k], polar(b[i, k])) <= TOL
+    # more matrices than one launch describes, of all shapes; empty ones among them
+    many = [grad_like(5 + 7 * k, 90 - 3 * k, seed=k) for k in range(29)] + [torch.empty(0, 5, device=DEV), torch.empty(2, 0, 3, device=DEV),
+                                                                            torch.empty(0, 4, 4, device=DEV)]
+    got = optim.orthogonalize(many)
+    assert [g.shape for g in got] == [m.shape for m in many]
+    for g, m in zip(got[:29], many):
+        assert off(g, polar(m)) <= TOL
+    assert optim.orthogonalize([]) == []
+
+
+@pytest.mark.gpu
+def test_gpu_orthogonalize_at_the_ends_of_the_range():
+    """Tiny and huge matrices (their squares leave fp32's range), zeros, infinities and NaN -- each on its own."""
+    base = grad_like(50, 60, seed=4)
+    ms = [base * 1e-30, base * 1e30, torch.zeros(50, 60, device=DEV), base.clone(), base.clone(), base]
+    ms[3][7, 9] = math.inf
+    ms[4][0, 0] = math.nan
+    got = optim.orthogonalize(ms, eps=1e-38)
+    assert off(got[0], polar(ms[0], eps=1e-38)) <= TOL
+    assert off(got[1], polar(ms[1])) <= TOL
+    assert not got[2].any()
+    assert got[3].isnan().any() and got[4].isnan().all()
+    assert off(got[5], polar(base)) <= TOL
+    # below eps the matrix is divided by eps: it stays small
+    assert off(optim.orthogonalize(base * 1e-9), polar(base * 1e-9)) <= TOL
+    # one entry that dominates, and a rank of one
+    spike = torch.zeros(90, 90, device=DEV)
+    spike[3, 4] = 2.0
+    assert off(optim.orthogonalize(spike), polar(spike)) <= TOL
+
+
+@pytest.mark.gpu
+def test_gpu_orthogonalize_repeats_its_bits_and_follows_the_stream():
+    g = grad_like(333, 222, seed=6)
+    want = optim.orthogonalize(g)
+    assert torch.equal(optim.orthogonalize(g), want)
+    side = torch.cuda.Stream(device=DEV)
+    side.wait_stream(torch.cuda.current_stream(DEV))
+    with torch.cuda.stream(side):
+        a = optim.orthogonalize(g)
+    b = optim.orthogonalize(g)          # two calls at once: each has its own workspace
+    torch.cuda.synchronize()
+    assert torch.equal(a, want) and torch.equal(b, want)
+
+
+def reference_step(p, g, buf, lr, momentum, nesterov, decay, adjust):
+    p, g, buf = (t.detach().double().cpu() for t in (p, g, buf))
+    buf = momentum * buf + (1 - momentum) * g
+    u = (1 - momentum) * g + momentum * buf if nesterov else buf
+    r, c = p.shape
+    rate = lr * (math.sqrt(max(1.0, r / c)) if adjust == "original" else 0.2 * math.sqrt(max(r, c)))
+    return p, (1 - lr * decay) * p - rate * polar(u), buf
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nesterov,decay,adjust", [(True, 0.1, "original"), (False, 0.0, "match_rms_adamw")])
+def test_gpu_muon_step_matches_the_formula_in_64_bits(nesterov, decay, adjust):
+    shapes = [(40, 70), (200, 30), (64, 64), (1, 5), (130, 257)]
+    gen = torch.Generator().manual_seed(8)
+    ps = [torch.randn(*s, generator=gen).to(DEV) for s in shapes]
+    ps[1] = torch.randn(30, 200, generator=gen).to(DEV).t()           # stored by columns
+    gs = [grad_like(*s, seed=k) for k, s in enumerate(shapes)]
+    gs[2] = torch.randn(64, 128, generator=gen).to(DEV)[:, ::2]
+    bs = [0.1 * grad_like(*s, seed=9 + k) for k, s in enumerate(shapes)]
+    want = [reference_step(p, g, b, 0.05, 0.9, nesterov, decay, adjust) for p, g, b in zip(ps, gs, bs)]
+    kept = [g.clone() for g in gs]
+    optim.muon_step(ps, gs, bs, lr=0.05, momentum=0.9, nesterov=nesterov, weight_decay=decay, adjust_lr=adjust)
+    for p, g, b, k, (old, new, buf) in zip(ps, gs, bs, kept, want):
+        assert torch.equal(g, k)
+        # the momentum: three fp32 roundings; the change of the parameter: the iteration's error, and the rounding of p
+        assert off(b, buf) <= 3 * 2.0 ** -24
+        change = float(torch.linalg.vector_norm(new - old))
+        slip = float(torch.linalg.vector_norm(p.double().cpu() - new))
+        assert slip <= TOL * change + 2.0 ** -23 * float(torch.linalg.vector_norm(old))
+
+
+@pytest.mark.gpu
+def test_gpu_flat_muon_steps_a_network_in_training():
+    """FlatMuon on a policy network trained through its fused loss: every matrix moves by the formula, everything else as
+    torch.optim.Adam moves it, frozen parameters not at all; the state survives a round trip."""
+    name = "small_icfm"
+    kind, cfg, m = um.build(name, DEV)
+    opt = optim.FlatMuon(m.model, lr=0.02, weight_decay=0.1, adam_lr=3e-3, adam_betas=(0.8, 0.95), adam_eps=1e-7)
+    names = [n for n, _ in m.model.plan.params]
+    assert len(opt.matrix_names) > 5 and all(n.endswith(".weight") for n in opt.matrix_names)
+    frozen = m.model.model["t_encoder"].W.detach().clone()
+    slices = dict(zip(names, opt.fg.slices))
+    rest = {n: p for n, (p, _, _) in slices.items() if n not in opt.matrix_names and p.requires_grad}
+    twins = {n: p.detach().clone().requires_grad_() for n, p in rest.items()}
+    adam = torch.optim.Adam(list(twins.values()), lr=3e-3, betas=(0.8, 0.95), eps=1e-7)
+    gen = torch.Generator().manual_seed(4)
+    B = 300
+    for step in range(3):
+        x0, x1 = torch.randn(B, 6, generator=gen).to(DEV), torch.rand(B, 6, generator=gen).to(DEV)
+        cond, t, eps = torch.randn(B, 17, generator=gen).to(DEV), torch.rand(B, generator=gen).to(DEV), torch.randn(B, 6, generator=gen).to(DEV)
+        opt.zero_grad()
+        m.flow_matching_loss(x0, x1, cond, t=t, noise=eps).backward()
+        want = {}
+        for n in opt.matrix_names:
+            p, at, cnt = slices[n]
+            want[n] = reference_step(p, p.grad, opt.exp_avg[at:at + cnt].view(p.shape), 0.02, 0.95, True, 0.1, "original")
+        for n, p in rest.items():
+            twins[n].grad = p.grad.detach().clone()
+        opt.step()
+        adam.step()
+        for n, (old, new, buf) in want.items():
+            p, at, cnt = slices[n]
+            change = float(torch.linalg.vector_norm(new - old))
+            assert float(torch.linalg.vector_norm(p.detach().double().cpu() - new)) <= TOL * change + 2.0 ** -23 * float(torch.linalg.vector_norm(old)), (step, n)
+        for n, p in rest.items():
+            assert float((p - twins[n]).detach().abs().max()) <= 2e-5 * (float(p.detach().abs().max()) + 1e-12), (step, n)
+    assert torch.equal(m.model.model["t_encoder"].W.detach(), frozen)
+    sd = copy.deepcopy(opt.state_dict())
+    assert sd["step"] == 3 and len(sd["param_groups"]) == 2
+    opt.exp_avg.zero_()
+    opt.param_groups[1]["lr"] = 1.0
+    opt.load_state_dict(sd)
+    assert float(opt.exp_avg.abs().max()) > 0 and opt.param_groups[1]["lr"] == 0.02 and opt.step_count == 3
+    sd["matrices"] = []
+    with pytest.raises(ValueError):
+        opt.load_state_dict(sd)
+
+
+@pytest.mark.gpu
+def test_gpu_flat_muon_replays_from_a_captured_graph():
+    """A training step with FlatMuon(capturable=True), captured once and replayed between eager work, takes the eager steps."""
+    name = "small_icfm"
+    kind, cfg, a = um.build(name, DEV)
+    kind, cfg, b = um.build(name, DEV)
+    b.load_state_dict(copy.deepcopy(a.state_dict()))
+    oa, ob = (optim.FlatMuon(m.model, lr=0.01, capturable=True) for m in (a, b))
+    gen = torch.Generator().manual_seed(9)
+    B = 500
+    x0, x1 = torch.randn(B, 6, generator=gen).to(DEV), torch.rand(B, 6, generator=gen).to(DEV)
+    cond, t, eps = torch.randn(B, 17, generator=gen).to(DEV), torch.rand(B, generator=gen).to(DEV), torch.randn(B, 6, generator=gen).to(DEV)
+
+    def step(m, o):
+        o.zero_grad()
+        loss = m.flow_matching_loss(x0, x1, cond, t=t, noise=eps)
+        loss.backward()
+        o.step()
+        return loss.detach()
+
+    side = torch.cuda.Stream(device=DEV)
+    side.wait_stream(torch.cuda.current_stream(DEV))
+    with torch.cuda.stream(side):
+        step(b, ob)
+    torch.cuda.current_stream(DEV).wait_stream(side)
+    step(a, oa)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(b, ob)
+    for _ in range(4):
+        graph.replay()
+        torch.cuda.synchronize()
+        step(a, oa)
+        for (k, p), (_, q) in zip(a.named_parameters(), b.named_parameters()):
+            assert torch.equal(p, q), k
+    assert oa.step_count == ob.step_count == 5
+
+
+# ------------------------------------------------------------------------------------------------- refusals, on the CPU
+def test_refusals_of_the_python_calls():
+    m = torch.randn(4, 5)
+    with pytest.raises(L.GrlHipError, match="HIP device"):
+        optim.orthogonalize(m)
+    with pytest.raises(ValueError, match="rows, cols"):
+        optim.orthogonalize(torch.randn(4))
+    with pytest.raises(TypeError):
+        optim.orthogonalize(m.double())
+    with pytest.raises(L.GrlHipError, match="HIP device"):
+        optim.muon_step([m], [m.clone()], [m.clone()], lr=0.1)
+    with pytest.raises(ValueError, match="gradients"):
+        optim.muon_step([m], [], [m], lr=0.1)
+    for bad in (dict(lr=-1.0), dict(lr=0.1, momentum=1.0), dict(lr=0.1, weight_decay=-1.0), dict(lr=0.1, eps=-1.0),
+                dict(lr=0.1, adjust_lr="no")):
+        with pytest.raises(ValueError):
+            optim.muon_step([m], [m], [m], **bad)
+    assert optim.muon_step([], [], [], lr=0.1) is None
+
+
+@pytest.mark.gpu
+def test_gpu_refusals_that_need_device_tensors():
+    m, g, b = (torch.randn(4, 5, device=DEV) for _ in range(3))
+    step = lambda *a: optim.muon_step(*a, lr=0.1)  # noqa: E731
+    for bad in (([m, m], [g, g], [b, b.clone()]), ([m], [m], [b]), ([m], [g], [g]), ([m], [g], [m]), ([m], [g.t()], [b]),
+                ([m[:1].expand(4, 5)], [g], [b]), ([m.view(-1)], [g], [b])):
+        with pytest.raises(ValueError):
+            step(*bad)
+    for bad in (([m], [g.half()], [b]), ([m], [g], [b.bfloat16()])):
+        with pytest.raises(TypeError):
+            step(*bad)
+    with pytest.raises(ValueError):
+        optim.orthogonalize([m, m.half()])
+    for abc in ((30.0, 0.0, 0.0), (math.nan, 0.0, 0.0), (1.0, -9.0, 13.9)):
+        with pytest.raises(L.GrlHipError):
+            optim.orthogonalize(m, coefficients=abc)
+    # |b s^2 + c s^4| <= 2.25 and |x| <= 1 for s <= 1: in range
+    assert off(optim.orthogonalize(m, coefficients=(1.0, -9.0, 9.0)), polar(m, abc=(1.0, -9.0, 9.0))) <= TOL
+    with pytest.raises(L.GrlHipError):
+        optim.orthogonalize(m, steps=-1)
+
+
+def test_c_entry_points_check_their_arguments_without_a_gpu():
+    lib = L.lib()
+    shapes = (ctypes.c_int64 * 2)(8, 8)
+    need = lib.grlhip_orthogonalize_workspace_bytes(shapes, 1)
+    # two X and X^T of 64 x 64 four-byte values each, A and B, one partial sum, the alignment of the end
+    assert need == 6 * 64 * 64 * 4 + 8 + 256
+    buf = (ctypes.c_char * (need + 256))()
+    ws = ctypes.c_void_p((ctypes.addressof(buf) + 255) // 256 * 256)
+    one = (ctypes.c_void_p * 1)(ws.value)
+    null = (ctypes.c_void_p * 1)(None)
+    orth = lambda src=one, dst=one, sh=shapes, n=1, elem=L.ELEM_F32, steps=5, abc=ABC, eps=1e-7, w=ws, size=need: lib.grlhip_orthogonalize(  # noqa: E731
+        src, dst, sh, None, n, elem, steps, *abc, eps, w, size, None)
+    assert orth(n=0) == 0
+    assert orth(n=-1) != 0 and orth(sh=None) != 0 and orth(src=null) != 0 and orth(dst=null) != 0
+    assert orth(elem=7) != 0 and orth(steps=-1) != 0 and orth(steps=33) != 0 and orth(eps=-1.0) != 0 and orth(eps=0.0) != 0 and orth(eps=math.nan) != 0
+    assert orth(abc=(9.0, 0.0, 0.0)) == -2 and b"1.9" in lib.grlhip_last_error()
+    assert orth(size=need - 1) == -4 and orth(w=None) == -4
+    assert orth(w=ctypes.c_void_p(ws.value + 8)) == -1
+    assert orth(sh=(ctypes.c_int64 * 2)(8, 1 << 17)) == -2
+    rates = (ctypes.c_float * 1)(0.1)
+    muon = lambda p=one, g=one, b=one, r=rates, mom=0.9: lib.grlhip_muon_step(p, g, b, shapes, None, r, 1, mom, 1, 1.0, 5, *ABC, 1e-7, ws, 0, None)  # noqa: E731
+    assert muon() == -4
+    for bad in (dict(p=null), dict(g=null), dict(b=null), dict(r=None), dict(mom=1.0), dict(mom=math.nan)):
+        assert muon(**bad) == -1, bad
+    assert lib.grlhip_orthogonalize_workspace_bytes((ctypes.c_int64 * 2)(-1, 2), 1) == 0
