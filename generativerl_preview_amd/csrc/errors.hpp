@@ -30,3 +30,9 @@ size_t guarded_size(F&& f) noexcept {
   }
 }
 }  // namespace grlhip
+
+#define LAUNCH_TRY(expr)                                                                                                      \
+  do {                                                                                                                        \
+    const hipError_t e_ = (expr);                                                                                             \
+    if (e_ != hipSuccess) return grlhip::set_error(GRLHIP_ERR_HIP, std::string(#expr) + ": " + hipGetErrorString(e_)); \
+  } while (0)

@@ -236,10 +236,10 @@ __global__ __launch_bounds__(C::THREADS, 2) void k_orth_product(Group g, int k) 
       if (SYM) {
         _Float16* D = STAGE == GRAM ? p.A(a.ws) : p.B(a.ws);
         store_t_f16x2(D + at(n, (int)mb, p.mp), L.h, v);
-        if (im != in) store_n_f16x2(D + at(mb, (int)nb, p.mp), 2 * p.mp, patch, L, v);
+        if (im != in) store_n_f16x2(D + at(mb, (int)nb, p.mp), 2 * p.mp, patch, L, 32, v);
       } else if (STAGE == UPDATE) {
         store_t_f16x2(p.XT(a.ws, k ^ 1) + at(n, (int)mb, p.mp), L.h, v);
-        store_n_f16x2(p.X(a.ws, k ^ 1) + at(mb, (int)nb, p.np), 2 * p.np, patch, L, v);
+        store_n_f16x2(p.X(a.ws, k ^ 1) + at(mb, (int)nb, p.np), 2 * p.np, patch, L, 32, v);
       } else if (n < a.n) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
@@ -352,12 +352,6 @@ void set_tiles(Group& g) {
   g.nsym = sym;
   g.nupd = upd;
 }
-
-#define LAUNCH_TRY(expr)                                                                                      \
-  do {                                                                                                        \
-    const hipError_t e_ = (expr);                                                                             \
-    if (e_ != hipSuccess) return set_error(GRLHIP_ERR_HIP, std::string(#expr) + ": " + hipGetErrorString(e_)); \
-  } while (0)
 
 template <class C, class T, bool MUON>
 int iterate(Group& g, int steps, hipStream_t stream) {

@@ -1,0 +1,135 @@
+"""Softmax cross entropy of a linear head over a large vocabulary, without storing the logits: the loss of a policy over
+discretised actions (behaviour cloning, or advantage-weighted with ``row_weight``), beside the fused losses of the continuous
+models.  ``grlhip_linear_ce_forward`` / ``grlhip_linear_ce_backward``."""
+import ctypes
+
+import torch
+
+from ... import _lib as L
+from ...engine import _ptr, _stream
+
+_ELEM = {torch.float32: L.ELEM_F32, torch.bfloat16: L.ELEM_BF16, torch.float16: L.ELEM_F16}
+_REDUCE = {"none": L.REDUCE_NONE, "mean": L.REDUCE_MEAN, "sum": L.REDUCE_SUM}
+
+
+def _strides(t):
+    return None if t.is_contiguous() else (ctypes.c_int64 * 2)(*t.stride())
+
+
+class _Head:
+    """The arguments that the forward and the backward call share."""
+
+    def __init__(self, hidden, weight, bias, target, row_weight, ignore_index, reduction):
+        self.hidden, self.weight, self.target, self.row_weight = hidden, weight, target, row_weight
+        self.bias = None if bias is None else bias.float().contiguous()
+        self.rows, self.features, self.vocab = hidden.shape[0], hidden.shape[1], weight.shape[0]
+        self.elem, self.reduction, self.ignore_index = _ELEM[hidden.dtype], reduction, ignore_index
+        self.operands = (_ptr(hidden), _strides(hidden), _ptr(weight), _strides(weight))
+
+    def sizes(self):
+        return self.rows, self.features, self.vocab, self.elem
+
+    def workspace(self, backward):
+        need = L.lib().grlhip_linear_ce_workspace_bytes(*self.operands, *self.sizes(), int(backward))
+        if need == 0:
+            raise L.GrlHipError(L.lib().grlhip_last_error().decode())
+        # one per call: calls on different streams and captured graphs must not share it
+        return torch.empty(need, dtype=torch.uint8, device=self.hidden.device)
+
+    def call(self, fn, ws, *rest):
+        dev = self.hidden.device
+        with torch.cuda.device(dev):
+            L.check(fn(*self.operands, _ptr(self.bias), _ptr(self.target), self.ignore_index, _ptr(self.row_weight),
+                       *self.sizes(), self.reduction, *rest, _ptr(ws), ws.numel(), _stream(dev)))
+
+    def forward(self):
+        """(losses, logsumexp, reduced loss, number of rows that are not ignored)"""
+        dev = self.hidden.device
+        losses, lse = (torch.empty(self.rows, dtype=torch.float32, device=dev) for _ in range(2))
+        total, count = (torch.empty((), dtype=torch.float32, device=dev) for _ in range(2))
+        self.call(L.lib().grlhip_linear_ce_forward, self.workspace(False), _ptr(losses), _ptr(lse), _ptr(total), _ptr(count))
+        return losses, lse, total, count
+
+    def backward(self, lse, count, grad, need_hidden, need_weight, need_bias):
+        new = lambda need, *shape, dtype: torch.empty(*shape, dtype=dtype, device=self.hidden.device) if need else None  # noqa: E731
+        gh = new(need_hidden, self.rows, self.features, dtype=self.hidden.dtype)
+        gw = new(need_weight, self.vocab, self.features, dtype=self.hidden.dtype)
+        gb = new(need_bias, self.vocab, dtype=torch.float32)
+        self.call(L.lib().grlhip_linear_ce_backward, self.workspace(True), _ptr(lse), _ptr(count), _ptr(grad),
+                  0 if grad.dim() == 0 else grad.stride(0), _ptr(gh), _ptr(gw), _ptr(gb))
+        return gh, gw, gb
+
+
+class _LinearCrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, bias, target, row_weight, ignore_index, reduction):
+        head = _Head(hidden, weight, bias, target, row_weight, ignore_index, reduction)
+        losses, lse, total, count = head.forward()
+        ctx.save_for_backward(hidden, weight, bias, target, row_weight, lse, count)
+        ctx.numbers = ignore_index, reduction
+        return losses if reduction == L.REDUCE_NONE else total
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        hidden, weight, bias, target, row_weight, lse, count = ctx.saved_tensors
+        head = _Head(hidden, weight, bias, target, row_weight, *ctx.numbers)
+        gh, gw, gb = head.backward(lse, count, grad.float(), *ctx.needs_input_grad[:3])
+        return gh, gw, None if gb is None else gb.to(bias.dtype), None, None, None, None
+
+
+def linear_cross_entropy(hidden, weight, target, bias=None, row_weight=None, ignore_index=-100, reduction="mean"):
+    """Cross entropy of ``softmax(hidden @ weight.T + bias)`` at ``target``.
+
+    ``hidden`` (..., features) and ``weight`` (vocabulary, features): fp32, bf16 or fp16, of one type, any strides;
+    ``target`` (...): int64 (or int32); ``bias`` (vocabulary,): any floating type, -inf masks an action; ``row_weight``
+    (...): a factor of every row's loss (an advantage weight), no gradient is taken to it.  Rows whose target is ``ignore_index`` or
+    whose weight is 0 (padding) contribute nothing, whatever their hidden row holds; any other target outside the vocabulary gives NaN.
+    ``reduction``: ``"none"`` (losses of target's shape), ``"sum"``, or ``"mean"`` -- the weighted sum over the number of rows
+    that are not ignored (0 when there are none).  The loss is fp32.
+
+    Differentiable (once) with respect to hidden, weight and bias; the gradients have the operands' types.  Logits are never stored:
+    the forward pass keeps one logsumexp per row, the backward pass recomputes them in pieces of the vocabulary.  With
+    ``reduction="none"`` and no gradient this is the negative log-probability of single tokens (serving).  While a HIP graph is
+    captured, no eager autograd graph over the same leaves may be alive (drop the earlier losses first)."""
+    if reduction not in _REDUCE:
+        raise ValueError("reduction: expected 'none', 'mean' or 'sum', got %r" % (reduction,))
+    if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1]:
+        raise ValueError("expected hidden (..., features) and weight (vocabulary, features), got %s and %s" %
+                         (tuple(hidden.shape), tuple(weight.shape)))
+    if hidden.dtype not in _ELEM or weight.dtype != hidden.dtype:
+        raise TypeError("hidden and weight must both be float32, bfloat16 or float16, got %s and %s" % (hidden.dtype, weight.dtype))
+    if target.shape != hidden.shape[:-1]:
+        raise ValueError("target: expected shape %s, got %s" % (tuple(hidden.shape[:-1]), tuple(target.shape)))
+    if target.dtype not in (torch.int64, torch.int32):
+        raise TypeError("target: expected int64 or int32, got %s" % target.dtype)
+    if weight.shape[0] < 1 or weight.shape[1] < 1:
+        raise ValueError("the vocabulary and the features must not be empty, got weight %s" % (tuple(weight.shape),))
+    if bias is not None:
+        if tuple(bias.shape) != (weight.shape[0],):
+            raise ValueError("bias: expected shape %s, got %s" % ((weight.shape[0],), tuple(bias.shape)))
+        if not bias.dtype.is_floating_point:
+            raise TypeError("bias: expected a floating type, got %s" % bias.dtype)
+    if row_weight is not None:
+        if row_weight.shape != target.shape:
+            raise ValueError("row_weight: expected shape %s, got %s" % (tuple(target.shape), tuple(row_weight.shape)))
+        if row_weight.requires_grad:
+            raise ValueError("row_weight: no gradient is taken to the weights of rows; detach them")
+    for name, t in (("hidden", hidden), ("weight", weight), ("target", target), ("bias", bias), ("row_weight", row_weight)):
+        if t is not None and not t.is_cuda:
+            raise L.GrlHipError("%s must live on a HIP device (got %s): there is no CPU fallback" % (name, t.device))
+        if t is not None and t.device != hidden.device:
+            raise ValueError("%s is on %s, hidden on %s" % (name, t.device, hidden.device))
+    rows = hidden.reshape(-1, hidden.shape[-1])
+    flat = target.reshape(-1).long().contiguous()
+    if row_weight is not None:
+        row_weight = row_weight.reshape(-1).float().contiguous()
+    if rows.shape[0] == 0:   # nothing to launch; the result still has a (zero) gradient
+        empty = (rows.float().sum() + weight[:0].float().sum()) + (0.0 if bias is None else bias[:0].float().sum())
+        return empty if reduction != "none" else empty + torch.zeros(target.shape, device=hidden.device)
+    if torch.is_grad_enabled() and (rows.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
+        loss = _LinearCrossEntropy.apply(rows, weight, bias, flat, row_weight, int(ignore_index), _REDUCE[reduction])
+    else:
+        losses, _, total, _ = _Head(rows, weight, bias, flat, row_weight, int(ignore_index), _REDUCE[reduction]).forward()
+        loss = losses if reduction == "none" else total
+    return loss.view(target.shape) if reduction == "none" else loss

@@ -1,0 +1,402 @@
+"""linear_cross_entropy (grlhip_linear_ce_forward / _backward) against the formulas in 64 bits.
+
+Tolerances, entry by entry, from the arithmetic (K features, N rows, u the half step of a type: finfo.eps / 2):
+  z:  16-bit operands are multiplied exactly, fp32 ones as two fp16 pieces (2^-21 of |h| |w|); the matrix core adds blocks of
+      16 products in fp32: (K / 16 + 16) 2^-24 of sum_k |h| |w|.
+  loss: the largest error of z in the row twice (logsumexp and the target), 2^-21 of the magnitudes for exp, log and sums.
+  D = softmax - onehot: twice the error of z and exp's own |z - lse| 2^-22 relative to the softmax, then the rounding of D
+      (u of a 16-bit type, 2^-21 for pieces, 2^-38 absolute for fp16's smallest numbers).
+  dh, dW: these times |W|, |h|; the fp32 sum over V or N; the result's own rounding (u, and fp16's smallest number)."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+from generativerl_preview_amd import _lib as L
+from generativerl_preview_amd.generative_models.model_functions import linear_cross_entropy
+
+DEV = "cuda:0"
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+TYPES = [F32, BF16, F16]
+
+
+def inputs(n, k, v, dtype, seed=0, bias=True, weights=True, ignored=0.2):
+    gen = torch.Generator().manual_seed(seed)
+    h = torch.randn(n, k, generator=gen).to(dtype).to(DEV)
+    w = (torch.randn(v, k, generator=gen) * 2 / math.sqrt(k)).to(dtype).to(DEV)
+    t = torch.randint(0, v, (n,), generator=gen)
+    b = None
+    if bias:
+        b = 0.5 * torch.randn(v, generator=gen)
+        b[torch.rand(v, generator=gen) < 0.2] = -math.inf
+        b[t] = 0.25
+        b = b.to(DEV)
+    t[torch.rand(n, generator=gen) < ignored] = -100
+    rw = None
+    if weights:
+        rw = torch.rand(n, generator=gen) * 3
+        rw[torch.rand(n, generator=gen) < 0.1] = 0.0
+        rw = rw.to(DEV)
+    return h, w, t.to(DEV), b, rw
+
+
+def oracle(h, w, t, b, rw, reduction, upstream=None):
+    """Everything in 64 bits, and the entrywise tolerances: {name: (value, tolerance)}."""
+    n, k = h.shape
+    kind = h.dtype
+    H, W = h.detach().double(), w.detach().double()
+    kept = (t != -100) & (torch.ones_like(t, dtype=torch.bool) if rw is None else rw != 0)
+    H = torch.where(kept.unsqueeze(1), H, 0.0)
+    z = H @ W.t()
+    reach = H.abs() @ W.abs().t()
+    if b is not None:
+        z = z + b.detach().double()
+    lse = torch.logsumexp(z, 1)
+    at = t.clamp(min=0).unsqueeze(1)
+    picked = z.gather(1, at).squeeze(1)
+    weight = torch.where(kept, torch.ones(n, dtype=torch.float64, device=h.device) if rw is None else rw.double(), 0.0)
+    losses = torch.where(kept, (lse - picked) * weight, 0.0)
+    finite = torch.where(z.isfinite(), z, 0.0).abs()
+    ez = ((k / 16 + 16) * 2.0 ** -24 + (2.0 ** -21 if kind == F32 else 0.0)) * reach + 2.0 ** -23 * finite
+    e_row = ez.max(1).values
+    e_loss = torch.where(kept, weight * (2 * e_row + 2.0 ** -21 * (1 + lse.abs() + picked.abs())), 0.0)
+    count = max(1, int((t != -100).sum()))
+    out = {"losses": (losses, e_loss)}
+    total = losses.sum() / (count if reduction == "mean" else 1)
+    out["total"] = (total, e_loss.sum() / (count if reduction == "mean" else 1) + 2.0 ** -23 * total.abs())
+    g = weight * (torch.ones(n, dtype=torch.float64, device=h.device) if upstream is None else upstream.double())
+    if reduction == "mean":
+        g = g / count
+    p = torch.exp(z - lse.unsqueeze(1))
+    ep = p * (2 * e_row.unsqueeze(1) + (torch.where(z.isfinite(), (z - lse.unsqueeze(1)).abs(), 0.0) + 2) * 2.0 ** -22)
+    d = p.clone()
+    d.scatter_add_(1, at, torch.full_like(d[:, :1], -1.0))
+    u = {F32: 2.0 ** -21, BF16: torch.finfo(BF16).eps / 2, F16: torch.finfo(F16).eps / 2}[kind]
+    ed = ep + u * d.abs() + (0.0 if kind == BF16 else 2.0 ** -38)
+    d, ed = torch.where(kept.unsqueeze(1), d, 0.0), torch.where(kept.unsqueeze(1), ed, 0.0)
+    g = torch.where(kept, g, 0.0)
+    uo = torch.finfo(kind).eps / 2
+    least = 2.0 ** -25 if kind == F16 else 0.0
+    v = w.shape[0]
+    dh = (d @ W) * g.unsqueeze(1)
+    edh = (ed + (v / 16 + 16 + 64) * 2.0 ** -24 * d.abs()) @ W.abs() * g.abs().unsqueeze(1)
+    gd, egd = d * g.unsqueeze(1), (ed + (n / 16 + 16 + 64) * 2.0 ** -24 * d.abs()) * g.abs().max()
+    egd = torch.where(kept.unsqueeze(1), (ep + u * d.abs() + (n / 16 + 80) * 2.0 ** -24 * d.abs()) * g.abs().unsqueeze(1)
+                      + (0.0 if kind == BF16 else 2.0 ** -37 * g.abs().max()), 0.0)
+    dw = gd.t() @ H
+    edw = egd.t() @ H.abs()
+    out["dh"] = (dh, edh + uo * (dh.abs() + edh) + 2.0 ** -21 * dh.abs() + least)
+    out["dw"] = (dw, edw + uo * (dw.abs() + edw) + 2.0 ** -21 * dw.abs() + least)
+    db = gd.sum(0)
+    out["db"] = (db, ((ep + d.abs() * (n * 2.0 ** -24 + 2.0 ** -21)) * g.abs().unsqueeze(1)).sum(0))
+    return out
+
+
+def near(got, name, out):
+    want, tol = out[name]
+    gap = (got.double() - want).abs()
+    assert got.shape == want.shape and bool(got.isfinite().all()), name
+    worst = float((gap - tol).max()) if gap.numel() else 0.0
+    assert worst <= 0.0, "%s: off by up to %.3g beyond the tolerance (largest gap %.3g)" % (name, worst, float(gap.max()))
+
+
+SIZES = [(1, 1, 1), (1, 64, 100), (2, 3, 2), (3, 5, 7), (64, 64, 64), (65, 63, 129), (128, 128, 1000), (200, 100, 333), (257, 192, 1030),
+         (33, 512, 3001), (500, 40, 257), (1, 1000, 5000), (17, 256, 4099)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("size", SIZES)
+def test_gpu_loss_and_gradients_match_64_bits(size, dtype):
+    h, w, t, b, rw = inputs(*size, dtype)
+    leaves = [h.requires_grad_(), w.requires_grad_(), b.requires_grad_()]
+    for reduction in ("mean", "sum", "none"):
+        loss = linear_cross_entropy(h, w, t, bias=b, row_weight=rw, reduction=reduction)
+        up = None
+        if reduction == "none":
+            up = torch.linspace(-1, 2, size[0], device=DEV)
+        out = oracle(h, w, t, b, rw, reduction, up)
+        assert loss.dtype == F32
+        near(loss.detach(), "losses" if reduction == "none" else "total", out)
+        dh, dw, db = torch.autograd.grad(loss, leaves, grad_outputs=up)
+        assert (dh.dtype, dw.dtype, db.dtype) == (dtype, dtype, F32)
+        near(dh, "dh", out)
+        near(dw, "dw", out)
+        near(db, "db", out)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_gpu_forward_without_a_gradient_is_the_same_loss(dtype):
+    h, w, t, b, rw = inputs(77, 128, 2049, dtype, seed=3)
+    a = linear_cross_entropy(h, w, t, bias=b, row_weight=rw, reduction="none")
+    assert not a.requires_grad
+    near(a, "losses", oracle(h, w, t, b, rw, "none"))
+    plain = linear_cross_entropy(h, w, t, ignore_index=-100, reduction="none")
+    near(plain, "losses", oracle(h, w, t, None, None, "none"))
+    # a batch of any shape
+    c = linear_cross_entropy(h.view(7, 11, 128), w, t.view(7, 11), bias=b, row_weight=rw.view(7, 11), reduction="none")
+    assert c.shape == (7, 11) and torch.equal(c.view(-1), a)
+    one = linear_cross_entropy(h[0], w, t[0].clamp(min=0), bias=b, reduction="none")
+    assert one.shape == ()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_gpu_pieces_of_the_vocabulary(dtype):
+    """More rows than one piece of the vocabulary holds entries for: the gradients are added up over the pieces."""
+    n, k, v = 50000, 64, 5000
+    h, w, t, b, rw = inputs(n, k, v, dtype, seed=5)
+    leaves = [h.requires_grad_(), w.requires_grad_(), b.requires_grad_()]
+    loss = linear_cross_entropy(h, w, t, bias=b, row_weight=rw)
+    grads = torch.autograd.grad(loss, leaves)
+    out = oracle(h, w, t, b, rw, "mean")
+    near(loss.detach(), "total", out)
+    for g, name in zip(grads, ("dh", "dw", "db")):
+        near(g, name, out)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_gpu_padding_may_hold_anything(dtype):
+    """Infinities and NaN in ignored rows, and in rows of weight 0, reach nothing."""
+    h, w, t, b, rw = inputs(130, 64, 300, dtype, seed=6)
+    t[5], t[77], t[9] = -100, -100, 3
+    rw[9] = 0.0
+    clean = [x.clone() for x in (h, w)]
+    want = linear_cross_entropy(clean[0].requires_grad_(), clean[1].requires_grad_(), t, bias=b, row_weight=rw)
+    want_g = torch.autograd.grad(want, clean)
+    h[5], h[77], h[9] = math.nan, math.inf, -math.inf
+    got = linear_cross_entropy(h.requires_grad_(), w.requires_grad_(), t, bias=b, row_weight=rw)
+    got_g = torch.autograd.grad(got, [h, w])
+    assert torch.equal(got, want)
+    assert torch.equal(got_g[1], want_g[1])
+    assert torch.equal(got_g[0], want_g[0]) and not got_g[0][[5, 77, 9]].any()
+
+
+@pytest.mark.gpu
+def test_gpu_all_rows_ignored_and_no_rows():
+    h, w, t, b, rw = inputs(40, 64, 90, BF16)
+    t.fill_(-100)
+    loss = linear_cross_entropy(h.requires_grad_(), w.requires_grad_(), t, bias=b.requires_grad_())
+    grads = torch.autograd.grad(loss, [h, w, b])
+    assert float(loss.detach()) == 0.0 and not any(g.any() for g in grads)
+    e = h[:0].detach().requires_grad_()
+    for reduction in ("mean", "sum", "none"):
+        loss = linear_cross_entropy(e, w, t[:0], bias=b, reduction=reduction)
+        assert loss.shape == ((0,) if reduction == "none" else ())
+        gw, gb = torch.autograd.grad(loss.sum(), [w, b])
+        assert not gw.any() and not gb.any()
+    assert linear_cross_entropy(h[:0].detach(), w.detach(), t[:0], reduction="none").shape == (0,)
+
+
+@pytest.mark.gpu
+def test_gpu_masks_and_bad_targets():
+    h, w, t, _, _ = inputs(70, 64, 200, F32, bias=False, weights=False, ignored=0.0)
+    low = torch.zeros(200, device=DEV)
+    low[::2] = torch.finfo(F32).min          # masked by the type's lowest value: the same as -inf
+    t = (t // 2 * 2 + 1) % 200
+    inf = torch.where(low < 0, -math.inf, low)
+    a, b = (linear_cross_entropy(h, w, t, bias=x, reduction="none") for x in (low, inf))
+    assert torch.equal(a, b)
+    near(a, "losses", oracle(h, w, t, inf, None, "none"))
+    # a masked target: an infinite loss, and still a finite gradient
+    w.requires_grad_()
+    t2 = t.clone()
+    t2[3] = 0
+    loss = linear_cross_entropy(h, w, t2, bias=inf, reduction="none")
+    assert float(loss[3].detach()) == math.inf and bool(loss[torch.arange(70, device=DEV) != 3].isfinite().all())
+    (g,) = torch.autograd.grad(loss, [w], grad_outputs=torch.ones_like(loss))
+    assert bool(g.isfinite().all())
+    # everything masked: NaN, in the loss and in the gradient
+    assert bool(linear_cross_entropy(h, w.detach(), t, bias=torch.full_like(low, -math.inf), reduction="none").isnan().all())
+    # targets outside the vocabulary that are not ignore_index: NaN in their rows only; the weight's gradient says it too
+    for bad in (200, -1, 1 << 40):
+        t3 = t.clone()
+        t3[11] = bad
+        loss = linear_cross_entropy(h, w, t3, reduction="none")
+        assert bool(loss[11].isnan()) and int(loss.isnan().sum()) == 1
+        (g,) = torch.autograd.grad(loss.sum(), [w])
+        assert bool(g.isnan().any())
+        assert bool(linear_cross_entropy(h, w, t3, ignore_index=bad, reduction="none").isfinite().all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_gpu_strides_and_alignment(dtype):
+    """Transposed, sliced, misaligned and broadcast operands give what their dense copies give."""
+    h, w, t, b, rw = inputs(90, 128, 210, dtype, seed=8)
+    wide = torch.randn(90, 300, device=DEV).to(dtype)
+    cases = [(h.t().contiguous().t(), w), (h, w.t().contiguous().t()), (wide[:, 7:135], w), (wide[:, ::2][:, :128], w),
+             (h[:1].expand(90, 128), w), (h, w[:1].expand(210, 128)), (h, torch.cat([w, w], 1)[:, 128:]), (h, w.repeat(2, 1)[::2])]
+    for x, y in cases:
+        dense = x.contiguous().detach().requires_grad_(), y.contiguous().detach().requires_grad_()
+        want = linear_cross_entropy(*dense, t, bias=b, row_weight=rw)
+        wg = torch.autograd.grad(want, dense)
+        odd = x.detach().requires_grad_(), y.detach().requires_grad_()
+        got = linear_cross_entropy(*odd, t, bias=b, row_weight=rw)
+        gg = torch.autograd.grad(got, odd)
+        assert torch.equal(got, want) and all(torch.equal(p, q) for p, q in zip(gg, wg))
+    # target and weights of other types and strides
+    a = linear_cross_entropy(h, w, t, bias=b, row_weight=rw)
+    t2 = torch.stack([t, t], 1)[:, 0]
+    r2 = torch.stack([rw, rw], 1)[:, 1].double()
+    b2 = torch.stack([b, b], 1)[:, 0].double()
+    assert torch.equal(linear_cross_entropy(h, w, t2.int(), bias=b2, row_weight=r2), a)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale", [1e-20, 1e15])
+def test_gpu_fp32_operands_of_any_magnitude(scale):
+    """The two-piece products follow the operands' magnitudes: small and large factors that cancel change little."""
+    h, w, t, b, rw = inputs(64, 96, 150, F32, seed=9)
+    h, w = (h * scale).requires_grad_(), (w / scale).requires_grad_()
+    loss = linear_cross_entropy(h, w, t, bias=b, row_weight=rw)
+    out = oracle(h, w, t, b, rw, "mean")
+    near(loss.detach(), "total", out)
+    for g, name in zip(torch.autograd.grad(loss, [h, w]), ("dh", "dw")):
+        near(g, name, out)
+
+
+@pytest.mark.gpu
+def test_gpu_gradient_matches_differences():
+    """Central differences of the loss along a direction: (f(x + s d) - f(x - s d)) / 2 s is off by s^2 f''' / 6 and by the
+    loss' own rounding over s; at s = 2^-6, |f'''| <= 1 and a loss of about 7 to 2^-21 that is 4e-5 + 2e-4."""
+    h, w, t, b, rw = inputs(50, 64, 400, F32, seed=10, bias=False)
+    h.requires_grad_(), w.requires_grad_()
+    gh, gw = torch.autograd.grad(linear_cross_entropy(h, w, t, row_weight=rw), [h, w])
+    gen = torch.Generator().manual_seed(1)
+    for x, g in ((h, gh), (w, gw)):
+        d = torch.randn(x.shape, generator=gen).to(DEV)
+        d /= d.norm()
+        s = 2.0 ** -6
+        with torch.no_grad():
+            f = [float(linear_cross_entropy(*((x + k * s * d, w) if x is h else (h, x + k * s * d)), t, row_weight=rw)) for k in (1, -1)]
+        assert abs((f[0] - f[1]) / (2 * s) - float((g * d).sum())) <= 3e-4
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_gpu_results_repeat_and_follow_the_stream(dtype):
+    h, w, t, b, rw = inputs(300, 192, 1500, dtype, seed=11)
+    h.requires_grad_(), w.requires_grad_(), b.requires_grad_()
+
+    def both():
+        loss = linear_cross_entropy(h, w, t, bias=b, row_weight=rw)
+        return [loss.detach(), *torch.autograd.grad(loss, [h, w, b])]
+
+    want = both()
+    side = torch.cuda.Stream(device=DEV)
+    side.wait_stream(torch.cuda.current_stream(DEV))
+    with torch.cuda.stream(side):
+        a = both()
+    c = both()              # two calls at once: each has its own workspace
+    torch.cuda.synchronize()
+    for got in (a, c, both()):
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+@pytest.mark.gpu
+def test_gpu_captured_step_replays():
+    """Loss and gradients captured once and replayed between eager calls, on changing inputs."""
+    h, w, t, b, rw = inputs(200, 128, 900, BF16, seed=12)
+    h.requires_grad_(), w.requires_grad_(), b.requires_grad_()
+
+    def both():
+        loss = linear_cross_entropy(h, w, t, bias=b, row_weight=rw)
+        return [loss.detach(), *torch.autograd.grad(loss, [h, w, b])]
+
+    side = torch.cuda.Stream(device=DEV)
+    side.wait_stream(torch.cuda.current_stream(DEV))
+    with torch.cuda.stream(side):
+        both()
+    torch.cuda.current_stream(DEV).wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = both()
+    gen = torch.Generator().manual_seed(2)
+    for _ in range(3):
+        with torch.no_grad():
+            h.copy_(torch.randn(h.shape, generator=gen))
+            t.copy_(torch.randint(0, 900, t.shape, generator=gen))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [x.clone() for x in held]
+        assert all(torch.equal(x, y) for x, y in zip(got, both()))
+
+
+@pytest.mark.gpu
+def test_gpu_a_head_over_a_network_trains_with_flat_muon():
+    """The operators together: features of a HIP network, the head's loss over discretised actions with advantage weights,
+    gradients through both, a FlatMuon step of the network and a muon_step of the head."""
+    from generativerl_preview_amd.optim import FlatMuon, muon_step
+    from generativerl_preview_amd.generative_models.intrinsic_model import IntrinsicModel
+    torch.manual_seed(3)
+    net = IntrinsicModel(dict(t_encoder=dict(type="GaussianFourierProjectionTimeEncoder", args=dict(embed_dim=32, scale=1.0)),
+                              backbone=dict(type="TemporalSpatialResidualNet",
+                                            args=dict(hidden_sizes=[128, 64], input_dim=11, output_dim=80, t_dim=32)))).to(DEV)
+    head = torch.nn.Parameter(torch.randn(700, 80, device=DEV) / 9)
+    time, state, t = torch.rand(256, device=DEV), torch.randn(256, 11, device=DEV), torch.randint(0, 700, (256,), device=DEV)
+    weight = torch.rand(256, device=DEV) + 0.5
+    opt = FlatMuon(net, lr=0.02)
+    buf = torch.zeros_like(head)
+    for _ in range(3):
+        opt.zero_grad()
+        head.grad = None
+        features = net(time, state)
+        loss = linear_cross_entropy(features, head, t, row_weight=weight)
+        loss.backward()
+        # the network's gradients are those of the plain head, through the same network
+        plain = ((torch.nn.functional.cross_entropy(net(time, state) @ head.detach().t(), t, reduction="none")) * weight).mean()
+        names = [p for p in net.parameters() if p.requires_grad]
+        for p, g in zip(names, torch.autograd.grad(plain, names)):
+            assert float((p.grad - g).abs().max()) <= 2e-5 * float(g.abs().max()) + 1e-9
+        before = [p.detach().clone() for p in names]
+        opt.step()
+        muon_step([head.data], [head.grad], [buf], lr=0.02)
+        assert all(not torch.equal(p, q) and bool(p.isfinite().all()) for p, q in zip(names, before))
+        assert bool(head.isfinite().all())
+
+
+# ------------------------------------------------------------------------------------------------- refusals, on the CPU
+def test_refusals_of_the_python_call():
+    h, w, t = torch.randn(4, 8), torch.randn(10, 8), torch.zeros(4, dtype=torch.int64)
+    call = linear_cross_entropy
+    with pytest.raises(L.GrlHipError, match="HIP device"):
+        call(h, w, t)
+    for bad in (lambda: call(h, w, t, reduction="max"), lambda: call(h, w[:, :7], t), lambda: call(h, w[0], t), lambda: call(h, w, t[:3]),
+                lambda: call(h, w[:0], t), lambda: call(h[:, :0], w[:, :0], t), lambda: call(h, w, t, bias=torch.zeros(9)),
+                lambda: call(h, w, t, row_weight=torch.ones(3)), lambda: call(h, w, t, row_weight=torch.ones(4, requires_grad=True))):
+        with pytest.raises(ValueError):
+            bad()
+    for bad in (lambda: call(h.double(), w.double(), t), lambda: call(h.half(), w, t), lambda: call(h, w, t.float()),
+                lambda: call(h, w, t, bias=torch.zeros(10, dtype=torch.int64))):
+        with pytest.raises(TypeError):
+            bad()
+
+
+def test_c_entry_points_check_their_arguments_without_a_gpu():
+    lib = L.lib()
+    size = lambda n=4, k=8, v=10, elem=L.ELEM_F32, back=0: lib.grlhip_linear_ce_workspace_bytes(None, None, None, None, n, k, v, elem, back)  # noqa: E731
+    assert size() > 0 and size(back=1) > size()
+    assert size(n=0) == size(k=0) == size(v=0) == size(elem=3) == size(n=(1 << 20) + 1) == size(k=1 << 17) == size(v=1 << 22) == 0
+    assert b"linear_ce" in lib.grlhip_last_error()
+    # 16-bit rows that are whole K blocks are read where they are
+    assert size(v=100000, k=64, elem=L.ELEM_BF16) < size(v=100000, k=65, elem=L.ELEM_BF16)
+    buf = (ctypes.c_char * 512)()
+    p = ctypes.c_void_p((ctypes.addressof(buf) + 255) // 256 * 256)
+
+    def fwd(h=p, w=p, t=p, n=4, k=8, v=10, elem=L.ELEM_F32, red=L.REDUCE_MEAN, losses=p, lse=p, total=p, count=p, ws=p, bytes_=1):
+        return lib.grlhip_linear_ce_forward(h, None, w, None, None, t, -100, None, n, k, v, elem, red, losses, lse, total, count, ws, bytes_, None)
+
+    def bwd(h=p, w=p, t=p, n=4, red=L.REDUCE_MEAN, lse=p, count=p, grad=p, gh=p, ws=p, bytes_=1):
+        return lib.grlhip_linear_ce_backward(h, None, w, None, None, t, -100, None, n, 8, 10, L.ELEM_F32, red, lse, count, grad, 0, gh, None, None, ws, bytes_, None)
+
+    assert fwd() == -4 and bwd() == -4 and b"workspace" in lib.grlhip_last_error()
+    for bad in ("h", "w", "t", "losses", "lse", "total", "count"):
+        assert fwd(**{bad: None}) == -1, bad
+    for bad in ("h", "w", "t", "lse", "count", "grad"):
+        assert bwd(**{bad: None}) == -1, bad
+    assert fwd(n=0) == -1 and fwd(elem=9) == -1 and fwd(red=3) == -1 and fwd(n=1 << 21) == -2 and fwd(ws=ctypes.c_void_p(p.value + 8)) == -1
+    assert bwd(gh=None) == 0      # nothing is asked for
