@@ -172,7 +172,7 @@ __global__ __launch_bounds__(C::THREADS, 2) void k_ce_forward(Logits a, int tm, 
   tile_at(xcd_order(blockIdx.x, gridDim.x), tm, tn, im, in);
   const int m0 = im * C::BM, n0 = in * C::BN;
   f32x16 acc[C::TM][C::TN];
-  product<T, P, C>(a.w.p + m0 * a.w.pitch, a.w.pitch, a.cols - m0, a.h.p + n0 * a.h.pitch, a.h.pitch, a.rows - n0, a.nkb, lds, acc);
+  product<T, P, C>(a.w.p + m0 * a.w.pitch, a.w.pitch, a.cols - m0, a.h.p + n0 * a.h.pitch, a.h.pitch, a.rows - n0, a.nkb, lds, acc);   // KG == 1: every wave goes on
   const Lane L = lane_of();
   const int wm = L.wave / C::WN, wn = L.wave % C::WN;
   const float fh = P == 2 ? 1.f / scale_of(a.s->hmax) : 1.f, fw = P == 2 ? 1.f / scale_of(a.s->wmax) : 1.f;
@@ -331,7 +331,7 @@ __global__ __launch_bounds__(C::THREADS, 2) void k_ce_d(Logits a, int tm, int tn
   tile_at(xcd_order(blockIdx.x, gridDim.x), tm, tn, im, in);
   const int m0 = im * C::BM, n0 = in * C::BN;
   f32x16 acc[C::TM][C::TN];
-  product<T, P, C>(a.w.p + m0 * a.w.pitch, a.w.pitch, a.cols - m0, a.h.p + n0 * a.h.pitch, a.h.pitch, a.rows - n0, a.nkb, lds, acc);
+  product<T, P, C>(a.w.p + m0 * a.w.pitch, a.w.pitch, a.cols - m0, a.h.p + n0 * a.h.pitch, a.h.pitch, a.rows - n0, a.nkb, lds, acc);   // KG == 1: every wave goes on
   const Lane L = lane_of();
   const int wm = L.wave / C::WN, wn = L.wave % C::WN;
   const float fh = P == 2 ? 1.f / scale_of(a.s->hmax) : 1.f, fw = P == 2 ? 1.f / scale_of(a.s->wmax) : 1.f;
@@ -362,9 +362,9 @@ __global__ __launch_bounds__(C::THREADS, 2) void k_ce_d(Logits a, int tm, int tn
         if (m >= a.cols || g == 0.f) v[r] = 0.f;
         bs[r] += m >= a.cols || g == 0.f ? 0.f : p * g;
       }
-      if (in_rows && mb < a.d_cols) {
-        if constexpr (P == 2) store_t_f16x2((_Float16*)a.d + (int64_t)n * 2 * a.d_cols + mb * 2, L.h, z);
-        else store_t_16<T>((T*)a.d + (int64_t)n * a.d_cols + mb, L.h, z);
+      if (nb < a.rows && mb < a.d_cols) {
+        if constexpr (P == 2) store_t_f16x2((_Float16*)a.d + (int64_t)nb * 2 * a.d_cols + mb * 2, 2 * a.d_cols, patch, L, a.rows - nb, z);
+        else store_t_16<T>((T*)a.d + (int64_t)nb * a.d_cols + mb, a.d_cols, patch, L, a.rows - nb, z);
       }
       if (nb < a.dt_cols && mb < a.cols) {
         if constexpr (P == 2) store_n_f16x2((_Float16*)a.dt + (int64_t)mb * 2 * a.dt_cols + nb * 2, 2 * a.dt_cols, patch, L, a.cols - mb, v);
@@ -475,7 +475,7 @@ __global__ __launch_bounds__(256) void k_ce_join(Grad g) {
 struct Shape { int64_t rows, hidden, vocab; int elem; };
 int pieces(int elem) { return elem == GRLHIP_ELEM_F32 ? 2 : 1; }
 
-typedef Tile128 Main;
+typedef Tile<128, 128, 2, 2, 2> Main;
 
 // How a call goes about it: the same for its workspace and its launches.
 struct Layout {

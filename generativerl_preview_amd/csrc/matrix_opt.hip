@@ -11,10 +11,12 @@
 // is fp32's rounding level: small singular values grow by a factor of a in every step, and so does what single fp16 pieces
 // round away (measured: relative error 2e-3 to 2e-2, with two pieces 1e-6 to 1e-5, fp32 products the same).
 //
-// One launch per product for the whole group (a network's matrices), so a step of the optimiser is 3 steps + 2 launches.
+// One launch per product for all matrices of a call, whatever their number: 3 steps + 2 launches.  A call whose matrices all fit into the
+// LDS of one workgroup each (64 x 192 padded) is ONE launch, a workgroup per matrix (k_orth_small).
+#include <algorithm>
 #include <cmath>
-#include <cstdio>
 #include <string>
+#include <vector>
 
 #include "../../include/grlhip.h"
 #include "errors.hpp"
@@ -26,8 +28,10 @@ namespace {
 using namespace mx;
 
 constexpr float S = 16384.f;        // scale of X, A, B
-constexpr int GROUP = 24;           // matrices of one launch: their descriptions are kernel arguments (graphs keep them)
+constexpr int GROUP = 32;           // matrices described by the kernel arguments of one launch (graphs keep them)
 constexpr int64_t MAX_SIDE = 1 << 16;
+
+enum Stage { GRAM, POLY, UPDATE, LAST };
 
 // One matrix, oriented to m <= n.  Strides in elements: [0] along m, [1] along n.
 struct Mat {
@@ -37,26 +41,35 @@ struct Mat {
   char* ws;           // its part of the workspace, see Parts
   int64_t gs[2], os[2], bs[2];
   int m, n;
-  int blk0;           // first 64 x 64 block of the norm and split launches
-  int tsym, tupd;     // first tile of the symmetric / update launches
   float rate;         // muon: learning rate of this matrix
+  int first[4];       // its first block of the norm and split launches, and its first tile of the GRAM, POLY and UPDATE launches
 };
-struct Group {
-  Mat mat[GROUP];
-  int count, blocks, nsym, nupd;
-  double* part;       // blocks partial sums of squares
+struct Numbers {
   float ca, cb, cc, eps;
   float momentum, fresh, keep;   // muon: momentum; 1 - momentum, from 64 bits; 1 - lr * weight decay
   int nesterov;
 };
+// What the launches after the first know of the matrices lies in the workspace: `first` of all matrices, [4][count], and the
+// descriptions themselves.
+// A lone matrix comes with the kernel arguments instead: two trips to memory less in each launch.
+struct Table { const int* first; const Mat* mat; int count; double* part; Mat one; };
+struct Group {
+  Mat mat[GROUP];
+  int count, from;    // matrices here; matrices before them in the table
+  int blocks0;        // blocks before this launch
+  int* first; Mat* table; int all; double* part;
+  Numbers num;
+};
 static_assert(sizeof(Group) <= 4000, "kernel arguments");
 
+__host__ __device__ inline int64_t up32(int64_t v) { return (v + 31) / 32 * 32; }
 __host__ __device__ inline int64_t up64(int64_t v) { return (v + 63) / 64 * 64; }
 // Pieces of a matrix in the workspace: two X, two X^T (a step reads one and writes the other), A, B.
 struct Parts {
   int64_t mp, np, x, a;   // padded sides; bytes of an X, of an A
-  __host__ __device__ Parts(int m, int n) : mp(up64(m)), np(up64(n)) { x = mp * np * 4; a = mp * mp * 4; }
-  __host__ __device__ int64_t bytes() const { return 4 * x + 2 * a; }
+  __host__ __device__ Parts(int m, int n) : mp(up32(m)), np(up32(n)) { x = mp * np * 4; a = mp * mp * 4; }
+  __host__ __device__ int64_t bytes() const { return (4 * x + 2 * a + 255) / 256 * 256; }
+  __host__ __device__ int blocks() const { return (int)((mp + 63) / 64 * ((np + 63) / 64)); }
   __device__ _Float16* X(char* ws, int k) const { return (_Float16*)(ws + k * x); }
   __device__ _Float16* XT(char* ws, int k) const { return (_Float16*)(ws + (2 + k) * x); }
   __device__ _Float16* A(char* ws) const { return (_Float16*)(ws + 4 * x); }
@@ -65,15 +78,15 @@ struct Parts {
 // entry (row, col) of a piece array with `cols` columns: the high piece, the low one 32 further
 __device__ __forceinline__ int64_t at(int64_t row, int col, int64_t cols) { return row * 2 * cols + (col >> 5) * 64 + (col & 31); }
 
-template <int FIELD>   // the matrix that block / tile `id` belongs to: the last one that starts at or before it
-__device__ __forceinline__ int find(const Group& g, int id) {
-  int lo = 0, hi = g.count - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    const int first = FIELD == 0 ? g.mat[mid].blk0 : FIELD == 1 ? g.mat[mid].tsym : g.mat[mid].tupd;
-    if (first <= id) lo = mid; else hi = mid - 1;
+// The matrix that block / tile `id` of a launch belongs to: the last one that starts at or before it.  One load a lane, one
+// ballot: a search would wait for memory at every step.
+__device__ __forceinline__ int find(const int* first, int count, int id) {
+  int below = 0;
+  for (int at = 0; at < count; at += 64) {
+    const int k = at + (int)(threadIdx.x & 63);
+    below += __popcll(__ballot(k < count && first[k] <= id));
   }
-  return lo;
+  return __builtin_amdgcn_readfirstlane(below - 1);
 }
 
 template <class T> __device__ __forceinline__ float load(const T* p) { return (float)*p; }
@@ -87,7 +100,7 @@ __device__ __forceinline__ Walk walk(bool along_n) {
 
 // buf = momentum buf + (1 - momentum) g and the direction u; or u = g.  WRITE: store buf.
 template <class T, bool MUON, bool WRITE>
-__device__ __forceinline__ float direction(const Group& g, const Mat& a, int64_t i, int64_t j) {
+__device__ __forceinline__ float direction(const Numbers& g, const Mat& a, int64_t i, int64_t j) {
   const float x = load((const T*)a.g + i * a.gs[0] + j * a.gs[1]);
   if (!MUON) return x;
   float* b = a.buf + i * a.bs[0] + j * a.bs[1];
@@ -96,12 +109,37 @@ __device__ __forceinline__ float direction(const Group& g, const Mat& a, int64_t
   return g.nesterov ? g.fresh * x + g.momentum * v : v;
 }
 
-// Pass 1: momentum, and the sum of squares of each 64 x 64 block in 64 bits (a sum that every later product depends on).
+// Sum over the block, in one order; every thread gets it.
+__device__ __forceinline__ double block_sum(double v, double* sh) {
+  sh[threadIdx.x] = v;
+  __syncthreads();
+  for (int d = 128; d > 0; d >>= 1) {
+    if ((int)threadIdx.x < d) sh[threadIdx.x] += sh[threadIdx.x + d];
+    __syncthreads();
+  }
+  return sh[0];
+}
+// What u is multiplied by: in 64 bits, as the quotient can pass fp32's range where the elements are tiny.
+__device__ __forceinline__ double factor_of(double squares, float eps) {
+  const double norm = sqrt(squares);
+  return (double)S / (norm > eps || norm != norm ? norm : (double)eps);
+}
+
+// Pass 1: momentum, and the sum of squares of each 64 x 64 block in 64 bits (a sum that every later product depends on).  The
+// first block also leaves the descriptions for the launches to come.
 template <class T, bool MUON>
 __global__ __launch_bounds__(256) void k_orth_norm(Group g) {
-  const int e = find<0>(g, blockIdx.x);
+  if (blockIdx.x == 0)
+    for (int k = threadIdx.x; k < g.count; k += 256) {
+      g.table[g.from + k] = g.mat[k];
+#pragma unroll
+      for (int f = 0; f < 4; ++f) g.first[f * g.all + g.from + k] = g.mat[k].first[f];
+    }
+  const int id = blockIdx.x + g.blocks0;
+  int e = 0;
+  while (e + 1 < g.count && g.mat[e + 1].first[0] <= id) ++e;
   const Mat& a = g.mat[e];
-  const int nb = (int)(up64(a.n) / 64), b = blockIdx.x - a.blk0;
+  const int nb = (int)(up64(a.n) / 64), b = id - a.first[0];
   const int i0 = b / nb * 64, j0 = b % nb * 64;
   const Walk w = walk(a.gs[1] <= a.gs[0]);
   double s = 0.0;
@@ -109,40 +147,26 @@ __global__ __launch_bounds__(256) void k_orth_norm(Group g) {
   for (int k = 0; k < 16; ++k) {
     const int i = i0 + w.i + k * w.di, j = j0 + w.j + k * w.dj;
     if (i < a.m && j < a.n) {
-      const double u = direction<T, MUON, true>(g, a, i, j);
+      const double u = direction<T, MUON, true>(g.num, a, i, j);
       s += u * u;
     }
   }
   __shared__ double sh[256];
-  sh[threadIdx.x] = s;
-  __syncthreads();
-  for (int d = 128; d > 0; d >>= 1) {
-    if ((int)threadIdx.x < d) sh[threadIdx.x] += sh[threadIdx.x + d];
-    __syncthreads();
-  }
-  if (threadIdx.x == 0) g.part[blockIdx.x] = sh[0];
+  s = block_sum(s, sh);
+  if (threadIdx.x == 0) g.part[id] = s;
 }
 
 // Pass 2: X = S u / max(|u|, eps) as pieces, and X^T.  Every block adds its matrix' partial sums, in the same order.
 template <class T, bool MUON>
-__global__ __launch_bounds__(256) void k_orth_split(Group g) {
-  const int e = find<0>(g, blockIdx.x);
-  const Mat& a = g.mat[e];
+__global__ __launch_bounds__(256) void k_orth_split(Table t, Numbers g) {
+  const Mat& a = t.mat[find(t.first, t.count, blockIdx.x)];
   const Parts p(a.m, a.n);
-  const int nb = (int)(p.np / 64), b = blockIdx.x - a.blk0, all = (int)(p.mp / 64) * nb;
+  const int nb = (int)((p.np + 63) / 64), b = blockIdx.x - a.first[0], all = p.blocks();
   __shared__ double sh[256];
   __shared__ float tile[64][65];
   double s = 0.0;
-  for (int k = threadIdx.x; k < all; k += 256) s += g.part[a.blk0 + k];
-  sh[threadIdx.x] = s;
-  __syncthreads();
-  for (int d = 128; d > 0; d >>= 1) {
-    if ((int)threadIdx.x < d) sh[threadIdx.x] += sh[threadIdx.x + d];
-    __syncthreads();
-  }
-  const double norm = sqrt(sh[0]);
-  // in 64 bits: the quotient can pass fp32's range where the elements are tiny
-  const double inv = (double)S / (norm > g.eps || norm != norm ? norm : (double)g.eps);
+  for (int k = threadIdx.x; k < all; k += 256) s += t.part[a.first[0] + k];
+  const double inv = factor_of(block_sum(s, sh), g.eps);
   const int i0 = b / nb * 64, j0 = b % nb * 64;
   const Walk w = walk(a.gs[1] <= a.gs[0]);
 #pragma unroll 4
@@ -155,6 +179,7 @@ __global__ __launch_bounds__(256) void k_orth_split(Group g) {
   const int row = threadIdx.x >> 2, col = (threadIdx.x & 3) * 16;
   _Float16* X = p.X(a.ws, 0) + at(i0 + row, j0 + col, p.np);
   _Float16* XT = p.XT(a.ws, 0) + at(j0 + row, i0 + col, p.mp);
+  const bool x_in = i0 + row < p.mp && j0 + col < p.np, xt_in = j0 + row < p.np && i0 + col < p.mp;   // the sides are padded to 32 only
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
     f16x8 h, l, ht, lt;
@@ -168,77 +193,98 @@ __global__ __launch_bounds__(256) void k_orth_split(Group g) {
       ht[k] = x;
       lt[k] = y;
     }
-    *(f16x8*)(X + c * 8) = h;
-    *(f16x8*)(X + 32 + c * 8) = l;
-    *(f16x8*)(XT + c * 8) = ht;
-    *(f16x8*)(XT + 32 + c * 8) = lt;
+    if (x_in) {
+      *(f16x8*)(X + c * 8) = h;
+      *(f16x8*)(X + 32 + c * 8) = l;
+    }
+    if (xt_in) {
+      *(f16x8*)(XT + c * 8) = ht;
+      *(f16x8*)(XT + 32 + c * 8) = lt;
+    }
   }
 }
 
-enum Stage { GRAM, POLY, UPDATE, LAST };
-
-// One product of every matrix of the group.  k: which X is read.
+// One product of every matrix.  k: which X is read.
 template <class C, int STAGE, class T, bool MUON>
-__global__ __launch_bounds__(C::THREADS, 2) void k_orth_product(Group g, int k) {
+__global__ __launch_bounds__(C::THREADS, C::LDS > 81920 ? C::THREADS / 256 : C::THREADS / 128) void k_orth_product(Table t, Numbers g, int k) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
   constexpr bool SYM = STAGE == GRAM || STAGE == POLY;
-  const int id = xcd_order(blockIdx.x, SYM ? g.nsym : g.nupd);
-  const Mat& a = g.mat[find<SYM ? 1 : 2>(g, id)];
+  constexpr int FIRST = STAGE == LAST ? 3 : STAGE + 1;
+  Mat a;
+  if (t.count == 1) a = t.one;
+  else a = t.mat[find(t.first + FIRST * t.count, t.count, blockIdx.x)];
   const Parts p(a.m, a.n);
-  const int tm = (int)((p.mp + C::BM - 1) / C::BM);
+  const int tm = (int)((p.mp + C::BM - 1) / C::BM), tn = SYM ? tm : (int)((p.np + C::BN - 1) / C::BN);
+  // the XCDs' ranges are taken inside each matrix: matrices differ in the length of their tiles
+  const int u = xcd_order(blockIdx.x - a.first[FIRST], SYM ? tm * (tm + 1) / 2 : tm * tn);
   int im, in;
-  if (SYM) {   // tile t of the lower triangle, row by row
-    const int t = id - a.tsym;
-    im = (int)((sqrtf(8.f * t + 1.f) - 1.f) * 0.5f);
-    while (im * (im + 1) / 2 > t) --im;
-    while ((im + 1) * (im + 2) / 2 <= t) ++im;
-    in = t - im * (im + 1) / 2;
+  if (SYM) {   // tile u of the lower triangle, row by row
+    im = (int)((sqrtf(8.f * u + 1.f) - 1.f) * 0.5f);
+    while (im * (im + 1) / 2 > u) --im;
+    while ((im + 1) * (im + 2) / 2 <= u) ++im;
+    in = u - im * (im + 1) / 2;
   } else {
-    tile_at(id - a.tupd, tm, (int)((p.np + C::BN - 1) / C::BN), im, in);
+    tile_at(u, tm, tn, im, in);
   }
   const int64_t m0 = (int64_t)im * C::BM, n0 = (int64_t)in * C::BN;
   f32x16 acc[C::TM][C::TN];
   const int64_t xp = p.np * 4, ap = p.mp * 4;   // row pitches in bytes
+  const Lane L = lane_of();
+  const int wm = L.wave / C::WN % C::WM, wn = L.wave % C::WN;
+  // The operand that the epilogue adds (A of the polynomial, X of the update; read transposed: 4 consecutive entries).  Small
+  // tiles ask for it before the product: its latency, 1 us from another XCD's stores, is a good part of such a launch.
+  constexpr bool OWN = STAGE != GRAM, EARLY = OWN && C::TM * C::TN == 1;
+  f16x4 own[EARLY ? 8 : 1];
+  auto load_own = [&](int64_t mb, int64_t n, f16x4* hi, f16x4* lo) {
+    const _Float16* o = STAGE == POLY ? p.A(a.ws) + at(n, (int)mb, p.mp) : p.XT(a.ws, k) + at(n, (int)mb, p.mp);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      hi[c] = *(const f16x4*)(o + 8 * c + 4 * L.h);
+      lo[c] = *(const f16x4*)(o + 32 + 8 * c + 4 * L.h);
+    }
+  };
+  if constexpr (EARLY) {
+    const int64_t mb = m0 + wm * 32, nb = n0 + wn * 32;
+    if (mb < p.mp && nb < (SYM ? p.mp : p.np)) load_own(mb, nb + L.j, own, own + 4);
+  }
   if (STAGE == GRAM) {
     const char* x = (const char*)p.X(a.ws, k);
-    product<_Float16, 2, C>(x + m0 * xp, xp, p.mp - m0, x + n0 * xp, xp, p.mp - n0, (int)(p.np / 32), lds, acc);
+    if (!product<_Float16, 2, C>(x + m0 * xp, xp, p.mp - m0, x + n0 * xp, xp, p.mp - n0, (int)(p.np / 32), lds, acc)) return;
   } else if (STAGE == POLY) {
     const char* x = (const char*)p.A(a.ws);
-    product<_Float16, 2, C>(x + m0 * ap, ap, p.mp - m0, x + n0 * ap, ap, p.mp - n0, (int)(p.mp / 32), lds, acc);
+    if (!product<_Float16, 2, C>(x + m0 * ap, ap, p.mp - m0, x + n0 * ap, ap, p.mp - n0, (int)(p.mp / 32), lds, acc)) return;
   } else {
-    product<_Float16, 2, C>((const char*)p.B(a.ws) + m0 * ap, ap, p.mp - m0, (const char*)p.XT(a.ws, k) + n0 * ap, ap, p.np - n0,
-                            (int)(p.mp / 32), lds, acc);
+    if (!product<_Float16, 2, C>((const char*)p.B(a.ws) + m0 * ap, ap, p.mp - m0, (const char*)p.XT(a.ws, k) + n0 * ap, ap, p.np - n0,
+                                 (int)(p.mp / 32), lds, acc)) return;
   }
-  const Lane L = lane_of();
-  const int wm = L.wave / C::WN, wn = L.wave % C::WN;
   unsigned* patch = (unsigned*)(lds + L.wave * PATCH);
 #pragma unroll
   for (int y = 0; y < C::TM; ++y) {
 #pragma unroll
     for (int x = 0; x < C::TN; ++x) {
       const int64_t mb = m0 + (wm * C::TM + y) * 32, nb = n0 + (wn * C::TN + x) * 32;
-      if (mb >= p.mp || nb >= (SYM ? p.mp : p.np)) continue;   // sides are padded to 64: whole blocks only
+      if (mb >= p.mp || nb >= (SYM ? p.mp : p.np)) continue;   // sides are padded to 32: whole blocks only
       const int64_t n = nb + L.j;
       float v[16];
       if (STAGE == GRAM) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) v[r] = acc[y][x][r] * (1.f / S);
-      } else {   // add the operand itself: A of the polynomial, X (read transposed: 4 consecutive entries) of the update
-        const _Float16* own = STAGE == POLY ? p.A(a.ws) + at(n, (int)mb, p.mp) : p.XT(a.ws, k) + at(n, (int)mb, p.mp);
+      } else {
         const float f = STAGE == POLY ? g.cb : g.ca, q = (STAGE == POLY ? g.cc : 1.f) * (1.f / S);
+        f16x4 late[EARLY ? 1 : 8];
+        if constexpr (!EARLY) load_own(mb, n, late, late + 4);
+        const f16x4 *hi = EARLY ? own : late, *lo = EARLY ? own + 4 : late + 4;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const f16x4 hi = *(const f16x4*)(own + 8 * c + 4 * L.h), lo = *(const f16x4*)(own + 32 + 8 * c + 4 * L.h);
+        for (int c = 0; c < 4; ++c)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) v[4 * c + i] = f * ((float)hi[i] + (float)lo[i]) + q * acc[y][x][4 * c + i];
-        }
+          for (int i = 0; i < 4; ++i) v[4 * c + i] = f * ((float)hi[c][i] + (float)lo[c][i]) + q * acc[y][x][4 * c + i];
       }
       if (SYM) {
         _Float16* D = STAGE == GRAM ? p.A(a.ws) : p.B(a.ws);
-        store_t_f16x2(D + at(n, (int)mb, p.mp), L.h, v);
+        store_t_f16x2(D + at(nb, (int)mb, p.mp), 2 * p.mp, patch, L, 32, v);
         if (im != in) store_n_f16x2(D + at(mb, (int)nb, p.mp), 2 * p.mp, patch, L, 32, v);
       } else if (STAGE == UPDATE) {
-        store_t_f16x2(p.XT(a.ws, k ^ 1) + at(n, (int)mb, p.mp), L.h, v);
+        store_t_f16x2(p.XT(a.ws, k ^ 1) + at(nb, (int)mb, p.mp), 2 * p.mp, patch, L, 32, v);
         store_n_f16x2(p.X(a.ws, k ^ 1) + at(mb, (int)nb, p.np), 2 * p.np, patch, L, 32, v);
       } else if (n < a.n) {
 #pragma unroll
@@ -256,10 +302,10 @@ __global__ __launch_bounds__(C::THREADS, 2) void k_orth_product(Group g, int k) 
 
 // steps == 0: the normalised matrix itself
 template <class T, bool MUON>
-__global__ __launch_bounds__(256) void k_orth_join(Group g) {
-  const Mat& a = g.mat[find<0>(g, blockIdx.x)];
+__global__ __launch_bounds__(256) void k_orth_join(Table t, Numbers g) {
+  const Mat& a = t.mat[find(t.first, t.count, blockIdx.x)];
   const Parts p(a.m, a.n);
-  const int nb = (int)(p.np / 64), b = blockIdx.x - a.blk0;
+  const int nb = (int)((p.np + 63) / 64), b = blockIdx.x - a.first[0];
   const int i0 = b / nb * 64, j0 = b % nb * 64;
   const Walk w = walk(a.os[1] <= a.os[0]);
   for (int k = 0; k < 16; ++k) {
@@ -286,25 +332,20 @@ struct Call {
   int nesterov;
 };
 
-// Workspace of the matrices [from, to): their pieces, and the partial sums.
-int64_t span_bytes(const int64_t* shapes, int from, int to) {
-  int64_t bytes = 0, blocks = 0;
-  for (int i = from; i < to; ++i) {
-    const int64_t r = shapes[2 * i], c = shapes[2 * i + 1];
-    if (r <= 0 || c <= 0) continue;
-    const Parts p((int)(r < c ? r : c), (int)(r < c ? c : r));
-    bytes += p.bytes();
-    blocks += p.mp / 64 * (p.np / 64);
-  }
-  return bytes + blocks * 8 + 256;
+int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
+Parts parts_of(const int64_t* shape) {
+  const int64_t r = shape[0], c = shape[1];
+  return Parts((int)(r < c ? r : c), (int)(r < c ? c : r));
 }
 int64_t workspace_bytes(const int64_t* shapes, int count) {
-  int64_t most = 256;
-  for (int i = 0; i < count; i += GROUP) {
-    const int64_t b = span_bytes(shapes, i, i + GROUP < count ? i + GROUP : count);
-    if (b > most) most = b;
+  int64_t bytes = 0, blocks = 0;
+  for (int i = 0; i < count; ++i) {
+    if (shapes[2 * i] <= 0 || shapes[2 * i + 1] <= 0) continue;
+    const Parts p = parts_of(shapes + 2 * i);
+    bytes += p.bytes();
+    blocks += p.blocks();
   }
-  return most;
+  return bytes + up256(blocks * 8) + up256((int64_t)count * sizeof(Mat)) + up256((int64_t)count * 16) + 256;
 }
 
 int check_shapes(const char* who, const int64_t* shapes, int count) {
@@ -337,98 +378,164 @@ int check_coefficients(const char* who, float a, float b, float c, int steps) {
   return 0;
 }
 
-template <class C>
-void set_tiles(Group& g) {
-  int sym = 0, upd = 0;
-  for (int i = 0; i < g.count; ++i) {
-    Mat& a = g.mat[i];
-    const Parts p(a.m, a.n);
-    const int tm = (int)((p.mp + C::BM - 1) / C::BM), tn = (int)((p.np + C::BN - 1) / C::BN);
-    a.tsym = sym;
-    a.tupd = upd;
-    sym += tm * (tm + 1) / 2;
-    upd += tm * tn;
+// The shapes of tiles.  Measured per K block of 32 (two pieces, 3 MFMAs), operands from beyond the L2 as the launch before left them:
+// a tile alone on its CU, and the CU's time for one on a full chip (730, 720, 940, 1070, 1190, 1180 TFLOP/s of MFMAs at best).
+// 512 x 512 x 512: 4.0, 6.1, 7.5, 11.3, 12.5, 30 us; 1024 x 1024 x 1024: 17.8, 10.4, 12.8, 20, 23, 57 us; 2048 x 4096 x 2048: 225,
+// 141, 110, 90, 87, 125 us; 8192 x 8192 x 2048: 774 (128), 698 us (256).
+typedef Tile<32, 32, 1, 1, 3, 4> Orth32;
+typedef Tile<64, 64, 2, 2, 3, 2> Orth64K;      // 96 KiB: one a CU, for launches of no more tiles than CUs; three stages cover the latency
+typedef Tile<64, 64, 2, 2, 2, 2> Orth64;
+typedef Tile<128, 128, 2, 2, 2, 2> Orth128K;   // one a CU again
+typedef Tile<128, 128, 2, 2, 2> Orth128;
+typedef Tile<256, 256, 2, 4, 2> Orth256;
+constexpr int KINDS = 6, SIDE[KINDS] = {32, 64, 64, 128, 128, 256};
+constexpr double ALONE[KINDS] = {0.095, 0.27, 0.33, 0.60, 0.67, 1.9}, FULL[KINDS] = {0.11, 0.28, 0.215, 0.75, 0.68, 2.73};
+// The epilogue moves 12 bytes an entry at a CU's share of the memory and hardly overlaps with products (all tiles of a launch
+// take the same time); what a tile costs besides.
+constexpr double EPILOGUE = 12 / 15e3, FIXED[KINDS] = {1.5, 0.8, 0.8, 0.8, 0.8, 0.8};
+
+int64_t tiles_of(const Parts& p, int stage, int side) {
+  const int64_t tm = (p.mp + side - 1) / side, tn = (p.np + side - 1) / side;
+  return stage == UPDATE ? tm * tn : tm * (tm + 1) / 2;
+}
+struct Plan { int kind[3]; int64_t tiles[3]; int64_t blocks; };   // by stage
+// A launch lasts as long as its longest tile, or as its tiles together on all CUs, in whole tiles a CU.
+Plan plan_of(const int64_t* shapes, int count) {
+  Plan plan = {};
+  double longest[3][KINDS] = {}, sum[3][KINDS] = {}, best[3] = {};
+  int64_t tiles[3][KINDS] = {};
+  for (int i = 0; i < count; ++i) {
+    if (shapes[2 * i] <= 0 || shapes[2 * i + 1] <= 0) continue;
+    const Parts p = parts_of(shapes + 2 * i);
+    plan.blocks += p.blocks();
+    for (int s = 0; s < 3; ++s)
+      for (int k = 0; k < KINDS; ++k) {
+        const double kb = (double)(s == GRAM ? p.np : p.mp) / 32;
+        const int64_t t = tiles_of(p, s, SIDE[k]);
+        tiles[s][k] += t;
+        sum[s][k] += t * (kb * FULL[k] + SIDE[k] * SIDE[k] * EPILOGUE + FIXED[k]);
+        longest[s][k] = std::fmax(longest[s][k], kb * ALONE[k]);
+      }
   }
-  g.nsym = sym;
-  g.nupd = upd;
+  const double cus = device_cus();
+  for (int s = 0; s < 3; ++s) {
+    for (int k = 0; k < KINDS; ++k) {
+      const double rounds = tiles[s][k] / cus;
+      const double us = tiles[s][k] > cus ? std::fmax(longest[s][k], sum[s][k] / cus * std::ceil(rounds) / rounds)
+                                          : longest[s][k] + rounds * SIDE[k] * SIDE[k] * EPILOGUE + FIXED[k];
+      if (k == 0 || us < best[s]) {
+        best[s] = us;
+        plan.kind[s] = k;
+      }
+    }
+    plan.tiles[s] = tiles[s][plan.kind[s]];
+  }
+  return plan;
 }
 
-template <class C, class T, bool MUON>
-int iterate(Group& g, int steps, hipStream_t stream) {
-  set_tiles<C>(g);
-  // the stages before the last know nothing of the matrices' type
-  const auto gram = k_orth_product<C, GRAM, float, false>, poly = k_orth_product<C, POLY, float, false>, update = k_orth_product<C, UPDATE, float, false>,
-             last = k_orth_product<C, LAST, T, MUON>;
-  if (C::LDS > 65536)
-    for (const auto f : {gram, poly, update, last})
-      LAUNCH_TRY(hipFuncSetAttribute((const void*)f, hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS));
-  for (int s = 0; s < steps; ++s) {
-    hipLaunchKernelGGL(gram, dim3(g.nsym), dim3(C::THREADS), C::LDS, stream, g, s & 1);
-    hipLaunchKernelGGL(poly, dim3(g.nsym), dim3(C::THREADS), C::LDS, stream, g, s & 1);
-    hipLaunchKernelGGL(s + 1 < steps ? update : last, dim3(g.nupd), dim3(C::THREADS), C::LDS, stream, g, s & 1);
-  }
+template <class C, int STAGE, class T, bool MUON>
+int launch(const Table& t, const Numbers& num, int k, int64_t tiles, hipStream_t stream) {
+  const auto kernel = k_orth_product<C, STAGE, T, MUON>;
+  if (C::LDS > 65536) LAUNCH_TRY(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS));
+  hipLaunchKernelGGL(kernel, dim3((unsigned)tiles), dim3(C::THREADS), C::LDS, stream, t, num, k);
   return 0;
 }
-
-template <class T, bool MUON>
-int run_group(Group& g, int steps, hipStream_t stream) {
-  hipLaunchKernelGGL((k_orth_norm<T, MUON>), dim3(g.blocks), dim3(256), 0, stream, g);
-  hipLaunchKernelGGL((k_orth_split<T, MUON>), dim3(g.blocks), dim3(256), 0, stream, g);
-  if (steps == 0) {
-    hipLaunchKernelGGL((k_orth_join<T, MUON>), dim3(g.blocks), dim3(256), 0, stream, g);
-    LAUNCH_TRY(hipGetLastError());
-    return 0;
+template <int STAGE, class T, bool MUON>
+int product_launch(int kind, const Table& t, const Numbers& num, int k, int64_t tiles, hipStream_t stream) {
+  switch (kind) {
+    case 0: return launch<Orth32, STAGE, T, MUON>(t, num, k, tiles, stream);
+    case 1: return launch<Orth64K, STAGE, T, MUON>(t, num, k, tiles, stream);
+    case 2: return launch<Orth64, STAGE, T, MUON>(t, num, k, tiles, stream);
+    case 3: return launch<Orth128K, STAGE, T, MUON>(t, num, k, tiles, stream);
+    case 4: return launch<Orth128, STAGE, T, MUON>(t, num, k, tiles, stream);
+    default: return launch<Orth256, STAGE, T, MUON>(t, num, k, tiles, stream);
   }
-  const int rc = iterate<Tile64, T, MUON>(g, steps, stream);
-  if (rc) return rc;
-  LAUNCH_TRY(hipGetLastError());
-  return 0;
+}
+
+template <bool MUON>
+Mat describe(const Call& c, int i) {
+  Mat a = {};
+  const int64_t r = c.shapes[2 * i], q = c.shapes[2 * i + 1];
+  const int flip = r > q;   // more rows than columns: the transposed matrix
+  a.g = c.src[i];
+  a.out = c.dst[i];
+  a.buf = MUON ? c.buf[i] : nullptr;
+  for (int k = 0; k < 2; ++k) {
+    const int64_t dense = k == 0 ? q : 1;
+    a.gs[k ^ flip] = c.strides ? c.strides[6 * i + k] : dense;
+    a.os[k ^ flip] = c.strides ? c.strides[6 * i + 2 + k] : dense;
+    a.bs[k ^ flip] = c.strides ? c.strides[6 * i + 4 + k] : dense;
+  }
+  a.m = (int)(flip ? q : r);
+  a.n = (int)(flip ? r : q);
+  a.rate = c.rate ? c.rate[i] : 0.f;
+  return a;
 }
 
 template <class T, bool MUON>
 int run(const char* who, const Call& c, char* ws, size_t ws_bytes, hipStream_t stream) {
-  if (workspace_bytes(c.shapes, c.count) > (int64_t)ws_bytes || (!ws && c.count > 0))
-    return set_error(GRLHIP_ERR_WORKSPACE, std::string(who) + ": workspace too small: need " + std::to_string(workspace_bytes(c.shapes, c.count)));
+  const int64_t need = workspace_bytes(c.shapes, c.count);
+  if (need > (int64_t)ws_bytes || (!ws && c.count > 0)) return set_error(GRLHIP_ERR_WORKSPACE, std::string(who) + ": workspace too small: need " + std::to_string(need));
   if ((size_t)ws & 255) return set_error(GRLHIP_ERR_INVALID, std::string(who) + ": the workspace must be aligned to 256 bytes");
-  for (int from = 0; from < c.count; from += GROUP) {
+  // the matrices with the longest sums first, so that a launch does not end with them
+  std::vector<int> order;
+  for (int i = 0; i < c.count; ++i)
+    if (c.shapes[2 * i] > 0 && c.shapes[2 * i + 1] > 0) order.push_back(i);
+  std::stable_sort(order.begin(), order.end(), [&](int x, int y) {
+    const Parts p = parts_of(c.shapes + 2 * x), q = parts_of(c.shapes + 2 * y);
+    return p.np != q.np ? p.np > q.np : p.mp > q.mp;
+  });
+  const int present = (int)order.size();
+  if (present == 0) return 0;
+  const Numbers num{c.ca, c.cb, c.cc, c.eps, (float)c.momentum, (float)(1.0 - c.momentum), c.keep, c.nesterov};
+  const Plan plan = plan_of(c.shapes, c.count);
+  if (plan.blocks > 1 << 30 || plan.tiles[0] > 1 << 22 || plan.tiles[1] > 1 << 22 || plan.tiles[2] > 1 << 22)
+    return set_error(GRLHIP_ERR_UNSUPPORTED, std::string(who) + ": too many matrices for one call");
+  // workspace: descriptions, firsts, partial sums, then the matrices
+  char* at = ws;
+  auto take = [&](int64_t bytes) { char* p = at; at += up256(bytes); return p; };
+  Mat* table = (Mat*)take((int64_t)c.count * sizeof(Mat));
+  int* first = (int*)take((int64_t)c.count * 16);
+  double* part = (double*)take(plan.blocks * 8);
+  Mat lone = {};
+  int64_t seen[4] = {0, 0, 0, 0};
+  for (int done = 0; done < present;) {
     Group g = {};
-    char* at = ws;
-    for (int i = from; i < c.count && i < from + GROUP; ++i) {
-      const int64_t r = c.shapes[2 * i], q = c.shapes[2 * i + 1];
-      if (r == 0 || q == 0) continue;
+    g.from = done;
+    g.blocks0 = (int)seen[0];
+    for (; done < present && g.count < GROUP; ++done) {
+      const int i = order[done];
+      const Parts p = parts_of(c.shapes + 2 * i);
       Mat& a = g.mat[g.count++];
-      const int flip = r > q;   // more rows than columns: the transposed matrix
-      a.g = c.src[i];
-      a.out = c.dst[i];
-      a.buf = MUON ? c.buf[i] : nullptr;
-      for (int k = 0; k < 2; ++k) {
-        const int64_t dense = k == 0 ? q : 1;
-        a.gs[k ^ flip] = c.strides ? c.strides[6 * i + k] : dense;
-        a.os[k ^ flip] = c.strides ? c.strides[6 * i + 2 + k] : dense;
-        a.bs[k ^ flip] = c.strides ? c.strides[6 * i + 4 + k] : dense;
-      }
-      a.m = (int)(flip ? q : r);
-      a.n = (int)(flip ? r : q);
-      a.rate = c.rate ? c.rate[i] : 0.f;
-      const Parts p(a.m, a.n);
+      a = describe<MUON>(c, i);
       a.ws = at;
       at += p.bytes();
-      a.blk0 = g.blocks;
-      g.blocks += (int)(p.mp / 64 * (p.np / 64));
+      a.first[0] = (int)seen[0];
+      seen[0] += p.blocks();
+      for (int s = 0; s < 3; ++s) {
+        a.first[s + 1] = (int)seen[s + 1];
+        seen[s + 1] += tiles_of(p, s, SIDE[plan.kind[s]]);
+      }
     }
-    if (g.count == 0) continue;
-    g.part = (double*)at;
-    g.ca = c.ca;
-    g.cb = c.cb;
-    g.cc = c.cc;
-    g.eps = c.eps;
-    g.momentum = (float)c.momentum;
-    g.fresh = (float)(1.0 - c.momentum);
-    g.keep = c.keep;
-    g.nesterov = c.nesterov;
-    const int rc = run_group<T, MUON>(g, c.steps, stream);
+    g.first = first;
+    g.table = table;
+    g.all = present;
+    g.part = part;
+    g.num = num;
+    lone = g.mat[0];   // used where there is one only
+    hipLaunchKernelGGL((k_orth_norm<T, MUON>), dim3((unsigned)(seen[0] - g.blocks0)), dim3(256), 0, stream, g);
+  }
+  const Table t{first, table, present, part, lone};
+  hipLaunchKernelGGL((k_orth_split<T, MUON>), dim3((unsigned)plan.blocks), dim3(256), 0, stream, t, num);
+  if (c.steps == 0) hipLaunchKernelGGL((k_orth_join<T, MUON>), dim3((unsigned)plan.blocks), dim3(256), 0, stream, t, num);
+  for (int s = 0; s < c.steps; ++s) {   // the stages before the last know nothing of the matrices' type
+    if (const int rc = product_launch<GRAM, float, false>(plan.kind[GRAM], t, num, s & 1, plan.tiles[GRAM], stream)) return rc;
+    if (const int rc = product_launch<POLY, float, false>(plan.kind[POLY], t, num, s & 1, plan.tiles[POLY], stream)) return rc;
+    const int rc = s + 1 < c.steps ? product_launch<UPDATE, float, false>(plan.kind[UPDATE], t, num, s & 1, plan.tiles[UPDATE], stream)
+                                   : product_launch<LAST, T, MUON>(plan.kind[UPDATE], t, num, s & 1, plan.tiles[UPDATE], stream);
     if (rc) return rc;
   }
+  LAUNCH_TRY(hipGetLastError());
   return 0;
 }
 
