@@ -175,32 +175,23 @@ __global__ __launch_bounds__(256) void k_orth_split(Table t, Numbers g) {
     tile[i][j] = i0 + i < a.m && j0 + j < a.n ? (float)(direction<T, MUON, false>(g, a, i0 + i, j0 + j) * inv) : 0.f;
   }
   __syncthreads();
-  // a thread writes 16 consecutive entries of one row of X, then of X^T
-  const int row = threadIdx.x >> 2, col = (threadIdx.x & 3) * 16;
-  _Float16* X = p.X(a.ws, 0) + at(i0 + row, j0 + col, p.np);
-  _Float16* XT = p.XT(a.ws, 0) + at(j0 + row, i0 + col, p.mp);
-  const bool x_in = i0 + row < p.mp && j0 + col < p.np, xt_in = j0 + row < p.np && i0 + col < p.mp;   // the sides are padded to 32 only
+  // 8 threads write the 128 bytes of 32 entries of a row: 4 their high pieces, 4 the low ones; X, then X^T
+  const int chunk = threadIdx.x & 7, low = chunk >> 2, c8 = (chunk & 3) * 8;
 #pragma unroll
-  for (int c = 0; c < 2; ++c) {
-    f16x8 h, l, ht, lt;
+  for (int k = 0; k < 4; ++k) {
+    const int q = (threadIdx.x >> 3) + 32 * k, row = q >> 1, col = (q & 1) * 32;
+    f16x8 x, xt;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      _Float16 x, y;
-      split2(tile[row][col + c * 8 + k], x, y);
-      h[k] = x;
-      l[k] = y;
-      split2(tile[col + c * 8 + k][row], x, y);
-      ht[k] = x;
-      lt[k] = y;
+    for (int e = 0; e < 8; ++e) {
+      _Float16 hi, lo;
+      split2(tile[row][col + c8 + e], hi, lo);
+      x[e] = low ? lo : hi;
+      split2(tile[col + c8 + e][row], hi, lo);
+      xt[e] = low ? lo : hi;
     }
-    if (x_in) {
-      *(f16x8*)(X + c * 8) = h;
-      *(f16x8*)(X + 32 + c * 8) = l;
-    }
-    if (xt_in) {
-      *(f16x8*)(XT + c * 8) = ht;
-      *(f16x8*)(XT + 32 + c * 8) = lt;
-    }
+    // the sides are padded to 32 only
+    if (i0 + row < p.mp && j0 + col < p.np) *(f16x8*)(p.X(a.ws, 0) + at(i0 + row, j0 + col, p.np) + low * 32 + c8) = x;
+    if (j0 + row < p.np && i0 + col < p.mp) *(f16x8*)(p.XT(a.ws, 0) + at(j0 + row, i0 + col, p.mp) + low * 32 + c8) = xt;
   }
 }
 
@@ -286,14 +277,25 @@ __global__ __launch_bounds__(C::THREADS, C::LDS > 81920 ? C::THREADS / 256 : C::
       } else if (STAGE == UPDATE) {
         store_t_f16x2(p.XT(a.ws, k ^ 1) + at(nb, (int)mb, p.mp), 2 * p.mp, patch, L, 32, v);
         store_n_f16x2(p.X(a.ws, k ^ 1) + at(mb, (int)nb, p.np), 2 * p.np, patch, L, 32, v);
-      } else if (n < a.n) {
+      } else {   // the result, in the matrix' own type and place: the one rounding to that type
+        const bool turned = a.os[0] < a.os[1];   // dense along m: turned round in LDS, so that lanes follow memory
+        if (turned) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            *(f32x4v*)((float*)patch + L.j * 36 + 8 * c + 4 * L.h) = f32x4v{v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]};
+#pragma unroll
+          for (int i = 0; i < 16; ++i) v[i] = ((float*)patch)[(2 * i + L.h) * 36 + L.j];
+        }
+        T* const o = (T*)a.out + (turned ? (mb + L.j) * a.os[0] + (nb + L.h) * a.os[1] : (mb + 4 * L.h) * a.os[0] + n * a.os[1]);
+        auto offset = [&](int r) { return turned ? 2 * r * a.os[1] : (8 * (r >> 2) + (r & 3)) * a.os[0]; };
+        auto inside = [&](int r) { return turned ? mb + L.j < a.m && nb + 2 * r + L.h < a.n : mb + 8 * (r >> 2) + 4 * L.h + (r & 3) < a.m && n < a.n; };
+        float old[16];   // all loads before the first store: they may alias as far as the compiler knows
+#pragma unroll
+        for (int r = 0; r < 16; ++r) old[r] = MUON && inside(r) ? (float)o[offset(r)] : 0.f;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const int64_t m = mb + 8 * (r >> 2) + 4 * L.h + (r & 3);
-          if (m >= a.m) continue;
-          T* o = (T*)a.out + m * a.os[0] + n * a.os[1];
           const float d = v[r] * (1.f / S);
-          *o = MUON ? (T)(g.keep * (float)*o - a.rate * d) : (T)d;   // the one rounding to the matrix' type
+          if (inside(r)) o[offset(r)] = MUON ? (T)(g.keep * old[r] - a.rate * d) : (T)d;
         }
       }
     }
