@@ -4,14 +4,15 @@
 // Forward: a tile of z lives in accumulators only; its epilogue leaves each row's maximum and sum of exponentials, and the
 // target's logit; one pass over these partials gives logsumexp and the loss.  2 N V H flops.
 // Backward, one piece of the vocabulary at a time: z again (the same products in the same order), D = softmax - onehot written
-// in 16 bits both ways round, D as [row][v] for dH += D W and D scaled by the row's gradient as [v][row] for dW = D^T H.  6 N V H
+// in fp16 both ways round, D as [row][v] for dH += D W and D scaled by the row's gradient as [v][row] for dW = D^T H.  6 N V H
 // flops; the workspace holds D of one piece.  Recomputing z costs a third more products than keeping it would, and N V
 // floats less memory.
 //
-// fp32 operands are two fp16 pieces a value (gemm_core.hip.inc), scaled by a power of two per tensor that brings its largest
-// entry to 2^13..2^14: what is lost of a value is at most 2^-23 of it or 2^-39 of the largest.  16-bit operands are used as they
-// are.  D is rounded once, to the operands' type (bf16 2^-8, fp16 2^-11 relative; the sums over it stay in fp32): the gradients are
-// rounded to that type anyway.  All sums are taken in a fixed order: results repeat bit for bit.
+// Precision.  z: 16-bit operands are used as they are, fp32 ones as two fp16 pieces a value (gemm_core.hip.inc), scaled by a
+// power of two per tensor that brings the largest entry to 2^13..2^14: what is lost of a value is at most 2^-23 of it or 2^-39 of the
+// largest.  D lies in [-1, 1] and is held times 2^14 in fp16: one piece for 16-bit operands (off by 2^-11 at most, below the
+// gradients' own rounding; in bf16, 2^-8, it would be as large as that), two for fp32.  W^T and hidden^T beside it are fp16 for that: bf16
+// entries fit its 11 bits exactly, scaled as above.  All sums are fp32 or wider and taken in a fixed order: results repeat bit for bit.
 #include <cmath>
 #include <string>
 
@@ -26,107 +27,165 @@ using namespace mx;
 
 constexpr int64_t MAX_ROWS = 1 << 20, MAX_VOCAB = 1 << 21, MAX_HIDDEN = 1 << 16;
 constexpr int64_t PIECE = 1ll << 27;      // entries of D in one piece of the vocabulary
+constexpr int HMAX = 64, WMAX = 256, GMAX = 64;   // blocks of the maxima
 __host__ __device__ inline int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 
-// What the kernels share through the workspace.
-struct Scalars { unsigned hmax, wmax, gmax; unsigned pad; };   // largest finite magnitudes, as bits (their order is the floats')
+// What the launches share: largest finite magnitudes of hidden, weight and the rows' gradients, by block and joined.
+struct Scalars { float h, w; float hpart[HMAX], wpart[WMAX], gpart[GMAX]; };
 
 // the power of two that brings the largest magnitude to 2^13..2^14; 1 for nothing but zeros
-__device__ __forceinline__ float scale_of(unsigned bits) {
-  if (bits == 0) return 1.f;
-  int e = (int)(bits >> 23) - 127;
+__device__ __forceinline__ float scale_of(float most) {
+  if (most == 0.f) return 1.f;
+  int e = __builtin_amdgcn_frexp_expf(most) - 1;
   e = e < -100 ? -100 : e;
   return __builtin_ldexpf(1.f, 13 - e);
 }
-// the smallest power of two that no gradient factor passes
-__device__ __forceinline__ float ceil_of(unsigned bits) {
-  if (bits == 0) return 1.f;
-  const int e = (int)(bits >> 23) - 126;
+// a power of two that no gradient factor passes
+__device__ __forceinline__ float ceil_of(float most) {
+  if (most == 0.f) return 1.f;
+  const int e = __builtin_amdgcn_frexp_expf(most);
   return __builtin_ldexpf(1.f, e > 127 ? 127 : e);
 }
-
-__global__ void k_ce_clear(Scalars* s) {
-  if (threadIdx.x < 4) ((unsigned*)s)[threadIdx.x] = 0u;
+__device__ __forceinline__ float finite(float v) { return __builtin_isfinite(v) ? fabsf(v) : 0.f; }
+__device__ __forceinline__ float wave_max(float m) {
+  for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
+  return m;
 }
+// over a block of 256 threads; all of them get it
+__device__ __forceinline__ float block_max(float m, float* sh) {
+  m = wave_max(m);
+  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = m;
+  __syncthreads();
+  return fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3]));
+}
+__device__ __forceinline__ float largest_gradient(const Scalars* s) { return wave_max(s->gpart[threadIdx.x & 63]); }
 
 struct View { const void* p; int64_t s0, s1; int rows, cols; };   // element strides
 
-__device__ __forceinline__ void keep_max(unsigned* to, float v) {
-  unsigned m = __builtin_isfinite(v) ? __builtin_bit_cast(unsigned, v) & 0x7fffffffu : 0u;
-  for (int d = 32; d > 0; d >>= 1) {
-    const unsigned o = __shfl_xor(m, d);
-    m = o > m ? o : m;
-  }
-  if ((threadIdx.x & 63) == 0 && m) atomicMax(to, m);
-}
-// the largest finite magnitudes of hidden (blocks [0, hb)) and weight (the others): a maximum, whatever the order
-__global__ __launch_bounds__(256) void k_ce_absmax(View h, View w, int hb, Scalars* s) {
-  const bool is_h = (int)blockIdx.x < hb;
+// the largest finite magnitudes of hidden (blocks [0, HMAX)) and weight (the others)
+template <class T>
+__global__ __launch_bounds__(256) void k_ce_absmax(View h, View w, Scalars* s) {
+  __shared__ float sh[4];
+  const bool is_h = blockIdx.x < HMAX;
   const View& v = is_h ? h : w;
-  const int64_t first = (is_h ? (int64_t)blockIdx.x : (int64_t)blockIdx.x - hb) * 256 + threadIdx.x;
-  const int64_t step = (int64_t)(is_h ? hb : (int)gridDim.x - hb) * 256, all = (int64_t)v.rows * v.cols;
+  const int b = is_h ? blockIdx.x : blockIdx.x - HMAX, n = is_h ? HMAX : WMAX;
+  constexpr int E = 16 / sizeof(T);
+  typedef T vec __attribute__((ext_vector_type(E)));
   float m = 0.f;
-  for (int64_t k = first; k < all; k += step) {
-    const int64_t r = k / v.cols, c = k - r * v.cols;
-    const float x = fabsf(((const float*)v.p)[r * v.s0 + c * v.s1]);
-    if (__builtin_isfinite(x) && x > m) m = x;
+  if (v.s1 == 1 && v.s0 == v.cols && ((size_t)v.p & 15) == 0) {   // dense: 16 bytes a thread
+    const int64_t all = (int64_t)v.rows * v.cols, whole = all / E;
+    const vec* p = (const vec*)v.p;
+#pragma unroll 4
+    for (int64_t k = (int64_t)b * 256 + threadIdx.x; k < whole; k += (int64_t)n * 256) {
+      const vec x = p[k];
+#pragma unroll
+      for (int e = 0; e < E; ++e) m = fmaxf(m, finite((float)x[e]));
+    }
+    if (b == 0 && threadIdx.x < all - whole * E) m = fmaxf(m, finite((float)((const T*)v.p)[whole * E + threadIdx.x]));
+  } else {
+    const bool along = v.s1 <= v.s0;   // lanes along the axis that is closer in memory
+    const int outer = along ? v.rows : v.cols, inner = along ? v.cols : v.rows;
+    const int64_t so = along ? v.s0 : v.s1, si = along ? v.s1 : v.s0;
+    for (int o = b * 4 + (threadIdx.x >> 6); o < outer; o += n * 4)
+      for (int i = threadIdx.x & 63; i < inner; i += 64) m = fmaxf(m, finite((float)((const T*)v.p)[o * so + i * si]));
   }
-  keep_max(is_h ? &s->hmax : &s->wmax, m);
+  m = block_max(m, sh);
+  if (threadIdx.x == 0) (is_h ? s->hpart : s->wpart)[b] = m;
 }
 
-// A 64 x 64 block of a view -> the operand layout, as it stands (n: rows of the view) and transposed (t: its columns), either
-// may be null; columns beyond the view and up to the pitch become zeros.  P == 2: scaled fp16 pieces.  A row that does not
-// count becomes zeros: whatever it holds must not reach a sum over rows.
-template <class T> struct Piece { typedef T type; };
-template <> struct Piece<float> { typedef _Float16 type; };
-template <class T>
-__global__ __launch_bounds__(256) void k_ce_pack(View v, void* n, int64_t n_cols, void* t, int64_t t_cols, const unsigned* most,
-                                                 const int64_t* target, int64_t ignore, const float* row_weight) {
-  typedef typename Piece<T>::type E;
-  constexpr int P = sizeof(T) == 4 ? 2 : 1;
+// A view -> operands: as it stands (n: rows of the view, type E) and transposed (t: its columns, fp16), either may be null; columns
+// beyond the view and up to the pitch become zeros.  fp32: two scaled fp16 pieces both ways.  bf16 transposed: scaled.  A row that
+// does not count becomes zeros: whatever it holds must not reach a sum over rows.
+struct Job {
+  View v;
+  void* n; int64_t n_cols;
+  void* t; int64_t t_cols;
+  bool mask; int blocks;
+};
+// The gradient of each row's own loss, and the largest of them.
+struct Scale {
+  const float* grad; int64_t grad_stride;
+  const float* row_weight; const float* count;
+  const int64_t* target; int64_t ignore;
+  int rows, vocab, reduction, blocks;
+  float* scale;
+};
+template <class E, bool TWO, class F>   // 128 bytes of a row by 8 threads
+__device__ __forceinline__ void pack_rows(E* out, int64_t cols, int r0, int rows, int c0, F&& value) {
   typedef E e8 __attribute__((ext_vector_type(8)));
-  __shared__ float tile[64][65];
-  const int i0 = blockIdx.y * 64, j0 = blockIdx.x * 64, tid = threadIdx.x;
-  const float s = P == 2 ? scale_of(*most) : 1.f;
-  const bool along = v.s1 <= v.s0;
+  const int chunk = threadIdx.x & 7;
+#pragma unroll
+  for (int k = 0; k < (TWO ? 4 : 2); ++k) {
+    const int line = (threadIdx.x >> 3) + 32 * k, row = TWO ? line >> 1 : line, col = TWO ? (line & 1) * 32 + (chunk & 3) * 8 : chunk * 8;
+    e8 x;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float v = value(row, col + e);
+      if constexpr (TWO) {
+        _Float16 hi, lo;
+        split2(v, hi, lo);
+        x[e] = chunk >> 2 ? lo : hi;
+      } else {
+        x[e] = (E)v;
+      }
+    }
+    if (r0 + row < rows && c0 + col < cols)
+      *(e8*)(out + (int64_t)(r0 + row) * (TWO ? 2 : 1) * cols + (TWO ? ((c0 + col) >> 5) * 64 + (chunk >> 2) * 32 + (chunk & 3) * 8 : c0 + col)) = x;
+  }
+}
+template <class T>
+__global__ __launch_bounds__(256) void k_ce_pack(Job h, Job w, Scale g, Scalars* s) {
+  constexpr bool TWO = sizeof(T) == 4, SCALED = !__is_same(T, _Float16);
+  __shared__ float tile[64][65], sh[4];
+  if ((int)blockIdx.x >= h.blocks + w.blocks) {
+    const int b = blockIdx.x - h.blocks - w.blocks;
+    float most = 0.f;
+    for (int n = b * 256 + threadIdx.x; n < g.rows; n += g.blocks * 256) {
+      const int64_t t = g.target[n];
+      const float rw = g.row_weight ? g.row_weight[n] : 1.f;
+      float v = 0.f;
+      if (t != g.ignore && rw != 0.f) {
+        v = g.grad[n * g.grad_stride] * rw;
+        if (g.reduction == GRLHIP_REDUCE_MEAN) v /= *g.count;
+        if (t < 0 || t >= g.vocab) v = NAN;
+      }
+      g.scale[n] = v;
+      most = fmaxf(most, finite(v));
+    }
+    most = block_max(most, sh);
+    if (threadIdx.x == 0) s->gpart[b] = most;
+    if (b == 0 && (int)threadIdx.x >= g.blocks && threadIdx.x < GMAX) s->gpart[threadIdx.x] = 0.f;
+    return;
+  }
+  const bool is_h = (int)blockIdx.x < h.blocks;
+  const Job& a = is_h ? h : w;
+  const int b = is_h ? blockIdx.x : blockIdx.x - h.blocks;
+  float f = 1.f;
+  if (SCALED) {
+    const float most = is_h ? block_max(threadIdx.x < HMAX ? s->hpart[threadIdx.x] : 0.f, sh) : block_max(s->wpart[threadIdx.x], sh);
+    f = scale_of(most);
+    if (b == 0 && threadIdx.x == 0) (is_h ? s->h : s->w) = most;
+  }
+  const int across = (a.v.cols + 63) / 64, i0 = b / across * 64, j0 = b % across * 64, tid = threadIdx.x;
+  const bool along = a.v.s1 <= a.v.s0;
 #pragma unroll 4
   for (int k = 0; k < 16; ++k) {
     const int i = along ? (tid >> 6) + 4 * k : tid & 63, j = along ? tid & 63 : (tid >> 6) + 4 * k;
     float x = 0.f;
-    if (i0 + i < v.rows && j0 + j < v.cols) {
-      const bool counts = !target || (target[i0 + i] != ignore && !(row_weight && row_weight[i0 + i] == 0.f));
-      if (counts) x = (float)((const T*)v.p)[(int64_t)(i0 + i) * v.s0 + (int64_t)(j0 + j) * v.s1] * s;
+    if (i0 + i < a.v.rows && j0 + j < a.v.cols) {
+      const bool counts = !a.mask || (g.target[i0 + i] != g.ignore && !(g.row_weight && g.row_weight[i0 + i] == 0.f));
+      if (counts) x = (float)((const T*)a.v.p)[(int64_t)(i0 + i) * a.v.s0 + (int64_t)(j0 + j) * a.v.s1];
     }
-    tile[i][j] = x;
+    tile[i][j] = TWO ? x * f : x;
   }
   __syncthreads();
-  const int row = tid >> 2, col = (tid & 3) * 16;
-#pragma unroll
-  for (int way = 0; way < 2; ++way) {
-    E* out = (E*)(way ? t : n);
-    if (!out) continue;
-    const int r = (way ? j0 : i0) + row, c = (way ? i0 : j0) + col;
-    const int64_t cols = way ? t_cols : n_cols;
-    if (r >= (way ? v.cols : v.rows) || c >= cols) continue;
-    E* dst = out + (int64_t)r * P * cols + (P == 2 ? (c >> 5) * 64 + (c & 31) : c);
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      e8 hi, lo;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const float x = way ? tile[col + q * 8 + k][row] : tile[row][col + q * 8 + k];
-        if constexpr (P == 2) {
-          _Float16 a, b;
-          split2(x, a, b);
-          hi[k] = a;
-          lo[k] = b;
-        } else {
-          hi[k] = (E)x;
-        }
-      }
-      *(e8*)(dst + q * 8) = hi;
-      if (P == 2) *(e8*)(dst + 32 + q * 8) = lo;
-    }
+  if (a.n) {
+    if constexpr (TWO) pack_rows<_Float16, true>((_Float16*)a.n, a.n_cols, i0, a.v.rows, j0, [&](int r, int c) { return tile[r][c]; });
+    else pack_rows<T, false>((T*)a.n, a.n_cols, i0, a.v.rows, j0, [&](int r, int c) { return tile[r][c]; });
+  }
+  if (a.t) {
+    if constexpr (TWO) pack_rows<_Float16, true>((_Float16*)a.t, a.t_cols, j0, a.v.cols, i0, [&](int r, int c) { return tile[c][r]; });
+    else pack_rows<_Float16, false>((_Float16*)a.t, a.t_cols, j0, a.v.cols, i0, [&](int r, int c) { return tile[c][r] * f; });
   }
 }
 
@@ -166,16 +225,16 @@ __device__ __forceinline__ void logits_of(const Logits& a, const f32x16& acc, in
 }
 
 template <class T, int P, class C>
-__global__ __launch_bounds__(C::THREADS, 2) void k_ce_forward(Logits a, int tm, int tn) {
+__global__ __launch_bounds__(C::THREADS, C::LDS > 81920 ? C::THREADS / 256 : C::THREADS / 128) void k_ce_forward(Logits a, int tm, int tn) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
   int im, in;
   tile_at(xcd_order(blockIdx.x, gridDim.x), tm, tn, im, in);
   const int m0 = im * C::BM, n0 = in * C::BN;
   f32x16 acc[C::TM][C::TN];
-  product<T, P, C>(a.w.p + m0 * a.w.pitch, a.w.pitch, a.cols - m0, a.h.p + n0 * a.h.pitch, a.h.pitch, a.rows - n0, a.nkb, lds, acc);   // KG == 1: every wave goes on
+  if (!product<T, P, C>(a.w.p + m0 * a.w.pitch, a.w.pitch, a.cols - m0, a.h.p + n0 * a.h.pitch, a.h.pitch, a.rows - n0, a.nkb, lds, acc)) return;
   const Lane L = lane_of();
   const int wm = L.wave / C::WN, wn = L.wave % C::WN;
-  const float fh = P == 2 ? 1.f / scale_of(a.s->hmax) : 1.f, fw = P == 2 ? 1.f / scale_of(a.s->wmax) : 1.f;
+  const float fh = P == 2 ? 1.f / scale_of(a.s->h) : 1.f, fw = P == 2 ? 1.f / scale_of(a.s->w) : 1.f;
   float* tops = (float*)lds;                  // [WM][BN] maxima, then sums
   float* sums = tops + C::WM * C::BN;
 #pragma unroll
@@ -209,7 +268,7 @@ __global__ __launch_bounds__(C::THREADS, 2) void k_ce_forward(Logits a, int tm, 
     }
   }
   lds_barrier();
-  for (int k = threadIdx.x; k < C::BN; k += C::THREADS) {
+  for (int k = threadIdx.x; k < C::BN; k += C::ACTIVE) {
     float top = tops[k], sum = sums[k];
 #pragma unroll
     for (int w = 1; w < C::WM; ++w) {
@@ -229,33 +288,35 @@ struct Finish {
   int64_t ignore;
   int rows, tiles, vocab, blocks;
   float* losses; float* lse;
-  double* sums;       // [blocks][2]: weighted loss, rows that count
+  double* sums;       // [blocks][2]: weighted loss, rows that count; null: nobody asks for the total
   float* total; float* count;   // the reduced loss; the number of rows that are not ignored, at least 1
   int reduction;
 };
 
-// 32 rows a block, 8 threads a row: the partials of a row, then its loss.
+// Q threads a row: the partials of a row, then its loss.
+template <int Q>
 __global__ __launch_bounds__(256) void k_ce_finish(Finish a) {
-  __shared__ float tops[8][32], sums[8][32];
-  __shared__ double s[32], c[32];
-  const int r = threadIdx.x & 31, q = threadIdx.x >> 5, n = blockIdx.x * 32 + r;
+  constexpr int R = 256 / Q;
+  __shared__ float tops[Q][R], sums[Q][R];
+  __shared__ double s[R], c[R];
+  const int r = threadIdx.x % R, q = threadIdx.x / R, n = blockIdx.x * R + r;
   float top = -INFINITY, sum = 0.f;
+  auto add = [&](float t, float u) {
+    const float most = fmaxf(top, t);
+    sum = (top == -INFINITY ? sum : sum * __expf(top - most)) + (t == -INFINITY ? u : u * __expf(t - most));
+    top = most;
+  };
   if (n < a.rows)
-    for (int t = q; t < a.tiles; t += 8) {
+#pragma unroll 4
+    for (int t = q; t < a.tiles; t += Q) {
       const float2 p = a.part[(int64_t)t * a.rows + n];
-      const float most = fmaxf(top, p.x);
-      sum = (top == -INFINITY ? sum : sum * __expf(top - most)) + (p.x == -INFINITY ? p.y : p.y * __expf(p.x - most));
-      top = most;
+      add(p.x, p.y);
     }
   tops[q][r] = top;
   sums[q][r] = sum;
   __syncthreads();
   if (q == 0) {
-    for (int k = 1; k < 8; ++k) {
-      const float t = tops[k][r], u = sums[k][r], most = fmaxf(top, t);
-      sum = (top == -INFINITY ? sum : sum * __expf(top - most)) + (t == -INFINITY ? u : u * __expf(t - most));
-      top = most;
-    }
+    for (int k = 1; k < Q; ++k) add(tops[k][r], sums[k][r]);
     s[r] = c[r] = 0.0;
     if (n < a.rows) {
       const int64_t t = a.target[n];
@@ -272,9 +333,9 @@ __global__ __launch_bounds__(256) void k_ce_finish(Finish a) {
     }
   }
   __syncthreads();
-  if (threadIdx.x == 0) {
+  if (threadIdx.x == 0 && a.sums) {
     double x = 0.0, y = 0.0;
-    for (int k = 0; k < 32; ++k) { x += s[k]; y += c[k]; }
+    for (int k = 0; k < R; ++k) { x += s[k]; y += c[k]; }
     a.sums[2 * blockIdx.x] = x;
     a.sums[2 * blockIdx.x + 1] = y;
   }
@@ -297,45 +358,20 @@ __global__ __launch_bounds__(256) void k_ce_total(Finish a) {
   }
 }
 
-// The gradient of each row's own loss, and the largest of them.
-struct Scale {
-  const float* grad; int64_t grad_stride;
-  const float* row_weight; const float* count;
-  const int64_t* target; int64_t ignore;
-  int rows, vocab, reduction;
-  float* scale; Scalars* s;
-};
-__global__ __launch_bounds__(256) void k_ce_scale(Scale a) {
-  const int n = blockIdx.x * 256 + threadIdx.x;
-  float g = 0.f;
-  if (n < a.rows) {
-    const int64_t t = a.target[n];
-    const float w = a.row_weight ? a.row_weight[n] : 1.f;
-    if (t != a.ignore && w != 0.f) {
-      g = a.grad[n * a.grad_stride] * w;
-      if (a.reduction == GRLHIP_REDUCE_MEAN) g /= *a.count;
-      if (t < 0 || t >= a.vocab) g = NAN;
-    }
-    a.scale[n] = g;
-  }
-  keep_max(&a.s->gmax, g);
-}
-
-constexpr float DSCALE = 16384.f;   // fp16 D lies in [-2^14, 2^14]
-template <class T> __device__ __forceinline__ float d_scale() { return sizeof(T) == 2 && __is_same(T, __bf16) ? 1.f : DSCALE; }
+constexpr float DSCALE = 16384.f;   // D lies in [-2^14, 2^14]
 
 template <class T, int P, class C>
-__global__ __launch_bounds__(C::THREADS, 2) void k_ce_d(Logits a, int tm, int tn) {
+__global__ __launch_bounds__(C::THREADS, C::LDS > 81920 ? C::THREADS / 256 : C::THREADS / 128) void k_ce_d(Logits a, int tm, int tn) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
   int im, in;
   tile_at(xcd_order(blockIdx.x, gridDim.x), tm, tn, im, in);
   const int m0 = im * C::BM, n0 = in * C::BN;
   f32x16 acc[C::TM][C::TN];
-  product<T, P, C>(a.w.p + m0 * a.w.pitch, a.w.pitch, a.cols - m0, a.h.p + n0 * a.h.pitch, a.h.pitch, a.rows - n0, a.nkb, lds, acc);   // KG == 1: every wave goes on
+  if (!product<T, P, C>(a.w.p + m0 * a.w.pitch, a.w.pitch, a.cols - m0, a.h.p + n0 * a.h.pitch, a.h.pitch, a.rows - n0, a.nkb, lds, acc)) return;
   const Lane L = lane_of();
   const int wm = L.wave / C::WN, wn = L.wave % C::WN;
-  const float fh = P == 2 ? 1.f / scale_of(a.s->hmax) : 1.f, fw = P == 2 ? 1.f / scale_of(a.s->wmax) : 1.f;
-  const float per = 1.f / ceil_of(a.s->gmax), ds = d_scale<T>();
+  const float fh = P == 2 ? 1.f / scale_of(a.s->h) : 1.f, fw = P == 2 ? 1.f / scale_of(a.s->w) : 1.f;
+  const float per = 1.f / ceil_of(largest_gradient(a.s));
   unsigned* patch = (unsigned*)(lds + L.wave * PATCH);
   float* bsum = (float*)(lds + C::WAVES * PATCH);   // [WN][BM]
 #pragma unroll
@@ -357,18 +393,17 @@ __global__ __launch_bounds__(C::THREADS, 2) void k_ce_d(Logits a, int tm, int tn
         const int m = mb + 8 * (r >> 2) + 4 * L.h + (r & 3);
         float p = __expf(z[r] - lse) - (m == t ? 1.f : 0.f);
         if (m >= a.cols || g == 0.f) p = 0.f;
-        z[r] = p * ds;
-        v[r] = p * (g * per) * ds;
-        if (m >= a.cols || g == 0.f) v[r] = 0.f;
+        z[r] = p * DSCALE;
+        v[r] = m >= a.cols || g == 0.f ? 0.f : p * (g * per) * DSCALE;
         bs[r] += m >= a.cols || g == 0.f ? 0.f : p * g;
       }
       if (nb < a.rows && mb < a.d_cols) {
         if constexpr (P == 2) store_t_f16x2((_Float16*)a.d + (int64_t)nb * 2 * a.d_cols + mb * 2, 2 * a.d_cols, patch, L, a.rows - nb, z);
-        else store_t_16<T>((T*)a.d + (int64_t)nb * a.d_cols + mb, a.d_cols, patch, L, a.rows - nb, z);
+        else store_t_16<_Float16>((_Float16*)a.d + (int64_t)nb * a.d_cols + mb, a.d_cols, patch, L, a.rows - nb, z);
       }
       if (nb < a.dt_cols && mb < a.cols) {
         if constexpr (P == 2) store_n_f16x2((_Float16*)a.dt + (int64_t)mb * 2 * a.dt_cols + nb * 2, 2 * a.dt_cols, patch, L, a.cols - mb, v);
-        else store_n_16<T>((T*)a.dt + (int64_t)mb * a.dt_cols + nb, a.dt_cols, patch, L, a.cols - mb, v);
+        else store_n_16<_Float16>((_Float16*)a.dt + (int64_t)mb * a.dt_cols + nb, a.dt_cols, patch, L, a.cols - mb, v);
       }
     }
     if (a.bpart) {   // over the 32 columns of the lanes of a half, in one order
@@ -383,7 +418,7 @@ __global__ __launch_bounds__(C::THREADS, 2) void k_ce_d(Logits a, int tm, int tn
   }
   if (a.bpart) {
     lds_barrier();
-    for (int k = threadIdx.x; k < C::BM; k += C::THREADS) {
+    for (int k = threadIdx.x; k < C::BM; k += C::ACTIVE) {
       float s = 0.f;
 #pragma unroll
       for (int w = 0; w < C::WN; ++w) s += bsum[w * C::BM + k];
@@ -392,82 +427,121 @@ __global__ __launch_bounds__(C::THREADS, 2) void k_ce_d(Logits a, int tm, int tn
   }
 }
 
-__global__ __launch_bounds__(256) void k_ce_bias(const float* part, int tiles, int cols, float* out) {
-  const int v = blockIdx.x * 256 + threadIdx.x;
-  if (v >= cols) return;
-  float s = 0.f;
-  for (int t = 0; t < tiles; ++t) s += part[(int64_t)t * cols + v];
-  out[v] = s;
-}
-
 // out[n][m] = f(n) sum_k A[m][k] B[n][k]: dH (A = W^T, B = D; f = the row's gradient) and dW (A = hidden^T, B = D^T).
 struct Grad {
   Operand a, b;
   int m, n, nkb, split;     // split: parts of the K blocks
+  int tiles;                // of the launch; 0: not asked for
   float* slots;             // fp32 [split][n][m], or null: straight to `out`
   int add;                  // to what the slots hold
-  void* out; int64_t o0, o1;   // element strides
+  void* out;                // dense rows
   const float* scale;       // per row, or null
-  const Scalars* s; int by_w;  // the operands' factors: W's (dH) or hidden's and the gradient's (dW)
+  int by_w;                 // the operands' factors: W's (dH) or hidden's and the gradient's (dW)
 };
+struct Grads { Grad g[2]; const Scalars* s; };   // one launch: dH's tiles, then dW's
+struct Factor { float f, f2; };
 template <class T>
-__device__ __forceinline__ float grad_factor(const Grad& g) {
-  float f = 1.f / d_scale<T>();
-  if (sizeof(T) == 4) f *= 1.f / scale_of(g.by_w ? g.s->wmax : g.s->hmax);
+__device__ __forceinline__ Factor factor_of(const Grad& g, const Scalars* s) {
+  Factor f{1.f / DSCALE, 1.f};
+  if (!__is_same(T, _Float16)) f.f *= 1.f / scale_of(g.by_w ? s->w : s->h);
+  if (!g.by_w) f.f2 = ceil_of(largest_gradient(s));
   return f;
 }
 template <class T, int P, class C>
-__global__ __launch_bounds__(C::THREADS, 2) void k_ce_grad(Grad g, int tm, int tn) {
-  typedef typename Piece<T>::type E;
+__global__ __launch_bounds__(C::THREADS, C::LDS > 81920 ? C::THREADS / 256 : C::THREADS / 128) void k_ce_grad(Grads both) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
-  const int id = xcd_order(blockIdx.x, gridDim.x), part = id / (tm * tn);
+  const bool second = (int)blockIdx.x >= both.g[0].tiles;
+  const Grad& g = both.g[second];
+  const int tm = (g.m + C::BM - 1) / C::BM, tn = (g.n + C::BN - 1) / C::BN;
+  const int id = xcd_order(blockIdx.x - (second ? both.g[0].tiles : 0), g.tiles), part = id / (tm * tn);
   int im, in;
   tile_at(id - part * tm * tn, tm, tn, im, in);
   const int m0 = im * C::BM, n0 = in * C::BN;
   const int k0 = (int)((int64_t)g.nkb * part / g.split), k1 = (int)((int64_t)g.nkb * (part + 1) / g.split);
   f32x16 acc[C::TM][C::TN];
-  product<E, P, C>(g.a.p + m0 * g.a.pitch + (int64_t)k0 * KBLOCK, g.a.pitch, g.m - m0, g.b.p + n0 * g.b.pitch + (int64_t)k0 * KBLOCK, g.b.pitch,
-                   g.n - n0, k1 - k0, lds, acc);
+  if (!product<_Float16, P, C>(g.a.p + m0 * g.a.pitch + (int64_t)k0 * KBLOCK, g.a.pitch, g.m - m0, g.b.p + n0 * g.b.pitch + (int64_t)k0 * KBLOCK,
+                               g.b.pitch, g.n - n0, k1 - k0, lds, acc)) return;
   const Lane L = lane_of();
   const int wm = L.wave / C::WN, wn = L.wave % C::WN;
-  const float f = grad_factor<T>(g), f2 = g.by_w ? 1.f : ceil_of(g.s->gmax);
+  const Factor f = factor_of<T>(g, both.s);
+  float* patch = (float*)(lds + L.wave * PATCH);
+  const bool to_slots = g.slots != nullptr;
+  // whole 16-byte stores where the rows allow them
+  const bool wide = to_slots ? g.m % 4 == 0 : g.m * sizeof(T) % 16 == 0 && ((size_t)g.out & 15) == 0;
 #pragma unroll
   for (int x = 0; x < C::TN; ++x) {
-    const int n = n0 + (wn * C::TN + x) * 32 + L.j;
-    if (n >= g.n) continue;
-    const float row = g.scale && !g.slots ? g.scale[n] : 1.f;
-    const bool none = g.scale && !g.slots && row == 0.f;
 #pragma unroll
     for (int y = 0; y < C::TM; ++y) {
+      const int mb = m0 + (wm * C::TM + y) * 32, nb = n0 + (wn * C::TN + x) * 32;
+      // through LDS: two lanes hold the 32 entries of a row (see store_t_f16x2)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        *(f32x4v*)(patch + L.j * 36 + 8 * q + 4 * L.h) = f32x4v{acc[y][x][4 * q], acc[y][x][4 * q + 1], acc[y][x][4 * q + 2], acc[y][x][4 * q + 3]};
+      float v[16];
+      const int row = L.lane >> 1, half = L.lane & 1, n = nb + row, m = mb + half * 16;
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const int m = m0 + (wm * C::TM + y) * 32 + 8 * q + 4 * L.h;
-        if (m >= g.m) continue;
-        if (g.slots) {
-          float* o = g.slots + ((int64_t)part * g.n + n) * g.m + m;
+        const f32x4v t = *(const f32x4v*)(patch + row * 36 + half * 16 + 4 * q);
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (m + i < g.m) o[i] = acc[y][x][4 * q + i] + (g.add ? o[i] : 0.f);
+        for (int i = 0; i < 4; ++i) v[4 * q + i] = t[i];
+      }
+      if (n >= g.n || m >= g.m) continue;
+      if (to_slots) {
+        float* o = g.slots + ((int64_t)part * g.n + n) * g.m + m;
+        if (wide && m + 16 <= g.m) {
+          f32x4v old[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) old[q] = g.add ? *(const f32x4v*)(o + 4 * q) : f32x4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int q = 0; q < 4; ++q) *(f32x4v*)(o + 4 * q) = old[q] + f32x4v{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
         } else {
-          T* o = (T*)g.out + (int64_t)n * g.o0 + (int64_t)m * g.o1;
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (m + i < g.m) o[i * g.o1] = none ? (T)0.f : (T)(acc[y][x][4 * q + i] * f * f2 * row);
+          for (int i = 0; i < 16 && m + i < g.m; ++i) o[i] = v[i] + (g.add ? o[i] : 0.f);
         }
+        continue;
+      }
+      const float r = g.scale ? g.scale[n] : 1.f;
+      T w[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) w[i] = g.scale && r == 0.f ? (T)0.f : (T)(v[i] * f.f * f.f2 * r);
+      T* o = (T*)g.out + (int64_t)n * g.m + m;
+      if (wide && m + 16 <= g.m) {
+        constexpr int E = 16 / sizeof(T);
+        typedef T vec __attribute__((ext_vector_type(E)));
+#pragma unroll
+        for (int q = 0; q < 16 / E; ++q) {
+          vec t;
+#pragma unroll
+          for (int e = 0; e < E; ++e) t[e] = w[q * E + e];
+          *(vec*)(o + q * E) = t;
+        }
+      } else {
+        for (int i = 0; i < 16 && m + i < g.m; ++i) o[i] = w[i];
       }
     }
   }
 }
+// The parts of the sums, in order: dH's blocks, dW's, the bias' (part [tiles][cols]).
+struct Join { Grads both; int blocks[2]; const float* bpart; int btiles, cols; float* gb; };
 template <class T>
-__global__ __launch_bounds__(256) void k_ce_join(Grad g) {
-  const float f = grad_factor<T>(g), f2 = g.by_w ? 1.f : ceil_of(g.s->gmax);
-  const int64_t all = (int64_t)g.n * g.m;
-  for (int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x; k < all; k += (int64_t)gridDim.x * 256) {
-    const int64_t n = k / g.m, m = k - n * g.m;
+__global__ __launch_bounds__(256) void k_ce_join(Join a) {
+  const int b = blockIdx.x;
+  if (b >= a.blocks[0] + a.blocks[1]) {
+    const int v = (b - a.blocks[0] - a.blocks[1]) * 256 + threadIdx.x;
+    if (v >= a.cols) return;
     float s = 0.f;
-    for (int p = 0; p < g.split; ++p) s += g.slots[p * all + k];
-    const float row = g.scale ? g.scale[n] : 1.f;
-    ((T*)g.out)[n * g.o0 + m * g.o1] = g.scale && row == 0.f ? (T)0.f : (T)(s * f * f2 * row);
+    for (int t = 0; t < a.btiles; ++t) s += a.bpart[(int64_t)t * a.cols + v];
+    a.gb[v] = s;
+    return;
+  }
+  const int k = b >= a.blocks[0];
+  const Grad& g = a.both.g[k];
+  const Factor f = factor_of<T>(g, a.both.s);
+  const int64_t all = (int64_t)g.n * g.m, step = (int64_t)a.blocks[k] * 256;
+  for (int64_t i = (int64_t)(k ? b - a.blocks[0] : b) * 256 + threadIdx.x; i < all; i += step) {
+    float s = 0.f;
+    for (int p = 0; p < g.split; ++p) s += g.slots[p * all + i];
+    const float row = g.scale ? g.scale[i / g.m] : 1.f;
+    ((T*)g.out)[i] = g.scale && row == 0.f ? (T)0.f : (T)(s * f.f * f.f2 * row);
   }
 }
 
@@ -475,48 +549,92 @@ __global__ __launch_bounds__(256) void k_ce_join(Grad g) {
 struct Shape { int64_t rows, hidden, vocab; int elem; };
 int pieces(int elem) { return elem == GRLHIP_ELEM_F32 ? 2 : 1; }
 
-typedef Tile<128, 128, 2, 2, 2> Main;
+// The shapes of tiles.  Measured per K block (128 bytes a row), one or two pieces: a tile alone on its CU, and the CU's time for one on
+// a full chip.  4096 x 4096 x 8192 in bf16: 446, 282, 245 us (616, 976, 1123 TFLOP/s); 1024 x 1024 x 1024: 7.5, 12, 24 us.
+typedef Tile<64, 64, 2, 2, 2, 2> Ce64;
+typedef Tile<128, 128, 2, 2, 2> Ce128;
+typedef Tile<256, 256, 2, 4, 2> Ce256;
+constexpr int KINDS = 3, SIDE[KINDS] = {64, 128, 256};
+constexpr double ALONE[2][KINDS] = {{0.30, 0.61, 1.28}, {0.33, 0.67, 1.9}}, FULL[2][KINDS] = {{0.21, 0.55, 1.91}, {0.22, 0.72, 2.73}};
+int64_t tiles_of(int64_t m, int64_t n, int k) { return up(m, SIDE[k]) / SIDE[k] * (up(n, SIDE[k]) / SIDE[k]); }
+// Time of a launch: its longest tile, or its tiles together on all CUs, in whole tiles a CU; `entry_ns` is a CU's time for one
+// entry of the epilogue, 0.8 us what a tile costs besides.
+double launch_us(double tiles, double kb, int p, int k, double entry_ns) {
+  const double cus = device_cus(), epilogue = SIDE[k] * SIDE[k] * entry_ns * 1e-3 + 0.8;
+  return tiles <= cus ? kb * ALONE[p - 1][k] + epilogue : std::ceil(tiles / cus) * (kb * FULL[p - 1][k] + epilogue);
+}
+int kind_for(int64_t m, int64_t n, int64_t kb, int p, double entry_ns) {
+  int best = 0;
+  for (int k = 1; k < KINDS; ++k)
+    if (launch_us((double)tiles_of(m, n, k), (double)kb, p, k, entry_ns) < launch_us((double)tiles_of(m, n, best), (double)kb, p, best, entry_ns)) best = k;
+  return best;
+}
+constexpr double FORWARD_NS = 0.15;   // exponentials
+double d_ns(int p) { return 0.2 + 4.0 * p / 15; }   // exponentials, and 4 or 8 bytes written at a CU's share of the memory
 
 // How a call goes about it: the same for its workspace and its launches.
 struct Layout {
   int64_t kp, np;                   // hidden and rows, padded to whole K blocks
   int64_t piece;                    // vocabulary entries of a piece
   bool pack_h, pack_w;
+  int kind_z, kind_g;               // tiles of the logits, of the gradients
   int split_h, split_w;             // parts of the sums of dH and dW
   int64_t pieces_n;
   // offsets
   int64_t scalars, hp, wp, ht, wt, d, dt, part, picked, sums, scale, bpart, hslots, wslots, bytes;
 };
-int split_for(int64_t tiles, int64_t nkb) {   // enough workgroups for the chip, but no part under 8 K blocks
-  int64_t s = tiles >= 256 ? 1 : (512 + tiles - 1) / tiles;
-  if (s > nkb / 8) s = nkb / 8;
-  return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
+// Both gradients are one launch: the tiles and the parts of the sums that make it shortest.  A part costs writing and reading back
+// fp32 sums, 8 bytes an entry at 4 TB/s, and a second launch.
+void plan_gradients(Layout& l, const Shape& c, int64_t vp, int p) {
+  const int64_t kb = p == 2 ? 32 : 64, kh = vp / kb, kw = l.np / kb;
+  double best = 0;
+  for (int k = 0; k < KINDS; ++k) {
+    const int64_t th = tiles_of(c.hidden, c.rows, k), tw = tiles_of(c.hidden, l.piece, k);
+    for (int sh = 1; sh <= 32; sh *= 2)
+      for (int sw = 1; sw <= 32; sw *= 2) {
+        if ((sh > 1 && kh / sh < 4) || (sw > 1 && kw / sw < 4)) continue;
+        const double parts = (sh > 1 ? (double)sh * c.rows * c.hidden : 0) + (sw > 1 ? (double)sw * l.piece * c.hidden : 0);
+        const double cus = device_cus(), epilogue = SIDE[k] * SIDE[k] * 0.3e-3 + 0.8;
+        const double sum = th * sh * ((double)kh / sh * FULL[p - 1][k] + epilogue) + tw * sw * ((double)kw / sw * FULL[p - 1][k] + epilogue);
+        const double tiles = (double)(th * sh + tw * sw), longest = std::fmax((double)kh / sh, (double)kw / sw) * ALONE[p - 1][k] + epilogue;
+        const double us = (tiles <= cus ? longest : std::fmax(longest, sum / cus * std::ceil(tiles / cus) / (tiles / cus))) + (parts > 0 ? 4.0 + parts * 8 / 4e6 : 0);
+        if ((k == 0 && sh == 1 && sw == 1) || us < best) {
+          best = us;
+          l.kind_g = k;
+          l.split_h = sh;
+          l.split_w = sw;
+        }
+      }
+  }
 }
 Layout layout_of(const Shape& c, bool direct_h, bool direct_w, bool backward, bool bias) {
   Layout l = {};
-  const int64_t per = pieces(c.elem) * 2;   // bytes of an operand entry
+  const int p = pieces(c.elem);
+  const int64_t per = p * 2;   // bytes of an operand entry
   l.kp = up(c.hidden, 64);
   l.np = up(c.rows, 64);
   l.pack_h = !direct_h;
   l.pack_w = !direct_w;
   int64_t limit = backward ? PIECE / l.np : l.pack_w ? PIECE / l.kp : c.vocab;
   limit = limit < 1024 ? 1024 : limit / 256 * 256;
-  if (backward && limit > 1 << 19) limit = 1 << 19;                                       // row offsets inside a tile are 32 bits
-  const int64_t most = (1 << 22) / (up(c.rows, Main::BN) / Main::BN) * Main::BM;          // and so is a launch
-  if (limit > most) limit = most;
+  if (backward && limit > 1 << 19) limit = 1 << 19;                            // row offsets inside a tile are 32 bits
+  const int64_t most = (1 << 20) / (up(c.rows, 64) / 64) * 64;                 // and so is a launch
+  if (limit > most) limit = most < 256 ? 256 : most / 256 * 256;
   l.pieces_n = (c.vocab + limit - 1) / limit;
   l.piece = up((c.vocab + l.pieces_n - 1) / l.pieces_n, 256);
   if (l.piece > c.vocab) l.piece = c.vocab;
   l.pieces_n = (c.vocab + l.piece - 1) / l.piece;
+  l.kind_z = kind_for(l.piece, c.rows, l.kp * per / KBLOCK, p, backward ? d_ns(p) : FORWARD_NS);
+  const int side = SIDE[l.kind_z];
   int64_t at = 0;
   auto take = [&](int64_t bytes) { const int64_t o = at; at += up(bytes, 256); return o; };
   l.scalars = take(sizeof(Scalars));
   if (l.pack_h) l.hp = take(c.rows * l.kp * per);
   if (l.pack_w) l.wp = take(l.piece * l.kp * per);
   if (!backward) {
-    l.part = take(up(c.vocab, Main::BM) / Main::BM * c.rows * 8 + l.pieces_n * c.rows * 8);
+    l.part = take((up(c.vocab, side) / side + l.pieces_n) * c.rows * 8);
     l.picked = take(c.rows * 4);
-    l.sums = take(up(c.rows, 32) / 32 * 16);
+    l.sums = take(up(c.rows, 4) / 4 * 16);
   } else {
     const int64_t vp = up(l.piece, 64);
     l.ht = take(c.hidden * l.np * per);
@@ -524,11 +642,8 @@ Layout layout_of(const Shape& c, bool direct_h, bool direct_w, bool backward, bo
     l.d = take(c.rows * vp * per);
     l.dt = take(l.piece * l.np * per);
     l.scale = take(c.rows * 4);
-    if (bias) l.bpart = take(up(c.rows, Main::BN) / Main::BN * l.piece * 4);
-    auto tiles = [](int64_t m, int64_t n) { return up(m, Main::BM) / Main::BM * (up(n, Main::BN) / Main::BN); };
-    const int64_t kb = pieces(c.elem) == 2 ? 32 : 64;
-    l.split_h = split_for(tiles(c.hidden, c.rows), vp / kb);
-    l.split_w = split_for(tiles(c.hidden, l.piece), l.np / kb);
+    if (bias) l.bpart = take(up(c.rows, side) / side * l.piece * 4);
+    plan_gradients(l, c, vp, p);
     if (l.split_h > 1 || l.pieces_n > 1) l.hslots = take(l.split_h * c.rows * c.hidden * 4);
     if (l.split_w > 1) l.wslots = take(l.split_w * l.piece * c.hidden * 4);
   }
@@ -557,175 +672,184 @@ int check(const char* who, const Call& a) {
   if (c.rows < 1 || c.hidden < 1 || c.vocab < 1) return set_error(GRLHIP_ERR_INVALID, w + "rows, hidden and vocabulary must be at least 1");
   if (c.rows > MAX_ROWS || c.vocab > MAX_VOCAB || c.hidden > MAX_HIDDEN)
     return set_error(GRLHIP_ERR_UNSUPPORTED, w + "over 2^20 rows, 2^21 vocabulary entries or 2^16 features");
+  if (c.rows * c.hidden > 1ll << 34 || c.vocab * c.hidden > 1ll << 34) return set_error(GRLHIP_ERR_UNSUPPORTED, w + "over 2^34 entries of hidden or weight");
   if (c.elem != GRLHIP_ELEM_F32 && c.elem != GRLHIP_ELEM_BF16 && c.elem != GRLHIP_ELEM_F16) return set_error(GRLHIP_ERR_INVALID, w + "unknown element type");
   if (a.reduction < 0 || a.reduction > 2) return set_error(GRLHIP_ERR_INVALID, w + "unknown reduction");
-  if (!a.h || !a.w || !a.target || !a.lse || !a.count) return set_error(GRLHIP_ERR_INVALID, w + "null hidden, weight, target, lse or count");
-  return 0;
-}
-template <class K>
-int lds_for(K k, int bytes) {
-  if (bytes > 65536) LAUNCH_TRY(hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
-  return 0;
-}
-
-// hidden / weight (a piece of it) as operands, packed where they have to be
-template <class T>
-int pack(const Call& a, const View& v, void* n, int64_t n_cols, void* t, int64_t t_cols, const unsigned* most, bool mask) {
-  if (!n && !t) return 0;
-  const dim3 grid((unsigned)(up(v.cols, 64) / 64), (unsigned)(up(v.rows, 64) / 64));
-  hipLaunchKernelGGL(k_ce_pack<T>, grid, dim3(256), 0, a.stream, v, n, n_cols, t, t_cols, most, mask ? a.target : nullptr, a.ignore, mask ? a.row_weight : nullptr);
+  if (!a.h || !a.w || !a.target || !a.lse) return set_error(GRLHIP_ERR_INVALID, w + "null hidden, weight, target or lse");
   return 0;
 }
 template <class T>
 View weight_piece(const Call& a, int64_t v0, int64_t cols) {
   return {(const char*)a.w + v0 * a.w0 * (int64_t)sizeof(T), a.w0, a.w1, (int)cols, (int)a.c.hidden};
 }
+View hidden_of(const Call& a) { return {a.h, a.h0, a.h1, (int)a.c.rows, (int)a.c.hidden}; }
+
 template <class T>
-int begin(const Call& a, Scalars* s) {
-  hipLaunchKernelGGL(k_ce_clear, dim3(1), dim3(64), 0, a.stream, s);
-  if (sizeof(T) == 4) {
-    const View h{a.h, a.h0, a.h1, (int)a.c.rows, (int)a.c.hidden}, w{a.w, a.w0, a.w1, (int)a.c.vocab, (int)a.c.hidden};
-    auto blocks = [](int64_t n) { n = (n + 4095) / 4096; return (int)(n > 1024 ? 1024 : n); };
-    const int hb = blocks((int64_t)h.rows * h.cols), wb = blocks((int64_t)w.rows * w.cols);
-    hipLaunchKernelGGL(k_ce_absmax, dim3(hb + wb), dim3(256), 0, a.stream, h, w, hb, s);
-  }
+void absmax_launch(const Call& a, Scalars* s) {
+  hipLaunchKernelGGL(k_ce_absmax<T>, dim3(HMAX + WMAX), dim3(256), 0, a.stream, hidden_of(a), weight_piece<T>(a, 0, a.c.vocab), s);
+}
+// Packs hidden (h null: not in this launch) and a weight piece, and takes the rows' gradients.
+template <class T>
+void pack_launch(const Call& a, Job h, Job w, Scale g, Scalars* s) {
+  auto blocks = [](Job& j) { j.blocks = j.n || j.t ? (int)(up(j.v.cols, 64) / 64 * (up(j.v.rows, 64) / 64)) : 0; };
+  blocks(h);
+  blocks(w);
+  const int all = h.blocks + w.blocks + g.blocks;
+  if (all > 0) hipLaunchKernelGGL(k_ce_pack<T>, dim3(all), dim3(256), 0, a.stream, h, w, g, s);
+}
+
+template <class K, class... A>
+int tile_launch(K kernel, int64_t tiles, int threads, int lds, hipStream_t stream, const A&... args) {
+  if (lds > 65536) LAUNCH_TRY(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+  hipLaunchKernelGGL(kernel, dim3((unsigned)tiles), dim3(threads), lds, stream, args...);
+  return 0;
+}
+#define BY_KIND(kind, call)            \
+  ((kind) == 0 ? call(Ce64) : (kind) == 1 ? call(Ce128) : call(Ce256))
+
+template <class T>
+Logits logits_call(const Call& a, const Layout& l, const View& w, int64_t v0, Scalars* s) {
+  constexpr int P = sizeof(T) == 4 ? 2 : 1;
+  Logits g = {};
+  g.h = l.pack_h ? Operand{a.ws + l.hp, l.kp * 2 * P} : Operand{(const char*)a.h, a.h0 * 2};
+  g.w = l.pack_w ? Operand{a.ws + l.wp, l.kp * 2 * P} : Operand{(const char*)w.p, a.w0 * 2};
+  g.bias = a.bias ? a.bias + v0 : nullptr;
+  g.target = a.target;
+  g.s = s;
+  g.rows = (int)a.c.rows;
+  g.v0 = (int)v0;
+  g.cols = w.rows;
+  g.nkb = (int)(l.kp * 2 * P / KBLOCK);
+  return g;
+}
+
+template <class T> struct Operands { typedef T type; };
+template <> struct Operands<float> { typedef _Float16 type; };
+
+int join_blocks(const Grad& g) {
+  const int64_t blocks = ((int64_t)g.n * g.m + 1023) / 1024;
+  return (int)(blocks > 4096 ? 4096 : blocks);
+}
+
+// From the partials to losses, logsumexps and the total.
+template <class T>
+int finish(const Call& a, const Layout& l, int tiles) {
+  const int64_t q = a.c.rows >= 2048 ? 8 : 64, blocks = (a.c.rows + 256 / q - 1) / (256 / q);   // few rows: more threads for each
+  const Finish f{(float2*)(a.ws + l.part), (float*)(a.ws + l.picked), a.target, a.row_weight, a.ignore, (int)a.c.rows, tiles, (int)a.c.vocab, (int)blocks,
+                 a.losses, a.lse, a.total ? (double*)(a.ws + l.sums) : nullptr, a.total, a.count, a.reduction};
+  if (q == 8) hipLaunchKernelGGL(k_ce_finish<8>, dim3((unsigned)blocks), dim3(256), 0, a.stream, f);
+  else hipLaunchKernelGGL(k_ce_finish<64>, dim3((unsigned)blocks), dim3(256), 0, a.stream, f);
+  if (a.total) hipLaunchKernelGGL(k_ce_total, dim3(1), dim3(256), 0, a.stream, f);
+  LAUNCH_TRY(hipGetLastError());
   return 0;
 }
 
 template <class T>
 int forward(const Call& a) {
-  typedef typename Piece<T>::type E;
   constexpr int P = sizeof(T) == 4 ? 2 : 1;
-  typedef Main C;
   const Layout l = layout_of(a.c, direct(a.h, a.h0, a.h1, a.c), direct(a.w, a.w0, a.w1, a.c), false, false);
   if (!a.ws || (int64_t)a.ws_bytes < l.bytes) return set_error(GRLHIP_ERR_WORKSPACE, "linear_ce_forward: workspace too small: need " + std::to_string(l.bytes));
   Scalars* s = (Scalars*)(a.ws + l.scalars);
-  begin<T>(a, s);
-  const View h{a.h, a.h0, a.h1, (int)a.c.rows, (int)a.c.hidden};
-  if (l.pack_h) pack<T>(a, h, a.ws + l.hp, l.kp, nullptr, 0, &s->hmax, false);
-  const auto kernel = k_ce_forward<E, P, C>;
-  if (const int rc = lds_for(kernel, C::LDS)) return rc;
+  if (P == 2) absmax_launch<T>(a, s);
+  const int side = SIDE[l.kind_z];
+  const int64_t tn = up(a.c.rows, side) / side;
   int tiles = 0;
   for (int64_t v0 = 0; v0 < a.c.vocab; v0 += l.piece) {
-    const int64_t cols = a.c.vocab - v0 < l.piece ? a.c.vocab - v0 : l.piece;
-    const View w = weight_piece<T>(a, v0, cols);
-    if (l.pack_w) pack<T>(a, w, a.ws + l.wp, l.kp, nullptr, 0, &s->wmax, false);
-    Logits g = {};
-    g.h = l.pack_h ? Operand{a.ws + l.hp, l.kp * 2 * P} : Operand{(const char*)a.h, a.h0 * 2};
-    g.w = l.pack_w ? Operand{a.ws + l.wp, l.kp * 2 * P} : Operand{(const char*)w.p, a.w0 * 2};
-    g.bias = a.bias ? a.bias + v0 : nullptr;
-    g.target = a.target;
-    g.s = s;
-    g.rows = (int)a.c.rows;
-    g.v0 = (int)v0;
-    g.cols = (int)cols;
-    g.nkb = (int)(l.kp * 2 * P / KBLOCK);
+    const View w = weight_piece<T>(a, v0, a.c.vocab - v0 < l.piece ? a.c.vocab - v0 : l.piece);
+    Job jh{hidden_of(a), v0 == 0 && l.pack_h ? a.ws + l.hp : nullptr, l.kp, nullptr, 0, false, 0};
+    Job jw{w, l.pack_w ? a.ws + l.wp : nullptr, l.kp, nullptr, 0, false, 0};
+    pack_launch<T>(a, jh, jw, Scale{}, s);
+    Logits g = logits_call<T>(a, l, w, v0, s);
     g.part = (float2*)(a.ws + l.part) + (int64_t)tiles * a.c.rows;
     g.picked = (float*)(a.ws + l.picked);
-    const int tm = (int)(up(cols, C::BM) / C::BM), tn = (int)(up(a.c.rows, C::BN) / C::BN);
-    hipLaunchKernelGGL(kernel, dim3(tm * tn), dim3(C::THREADS), C::LDS, a.stream, g, tm, tn);
+    const int tm = (int)(up(w.rows, side) / side);
+#define CALL(C) tile_launch(k_ce_forward<typename Operands<T>::type, P, C>, tm * tn, C::THREADS, C::LDS, a.stream, g, tm, (int)tn)
+    if (const int rc = BY_KIND(l.kind_z, CALL)) return rc;
+#undef CALL
     tiles += tm;
   }
-  Finish f{(float2*)(a.ws + l.part), (float*)(a.ws + l.picked), a.target, a.row_weight, a.ignore, (int)a.c.rows, tiles, (int)a.c.vocab,
-           (int)(up(a.c.rows, 32) / 32), a.losses, a.lse, (double*)(a.ws + l.sums), a.total, a.count, a.reduction};
-  hipLaunchKernelGGL(k_ce_finish, dim3(f.blocks), dim3(256), 0, a.stream, f);
-  hipLaunchKernelGGL(k_ce_total, dim3(1), dim3(256), 0, a.stream, f);
-  LAUNCH_TRY(hipGetLastError());
-  return 0;
-}
-
-template <class T, class C>
-int grad_launch(const Call& a, const Grad& g) {
-  constexpr int P = sizeof(T) == 4 ? 2 : 1;
-  const auto kernel = k_ce_grad<T, P, C>;
-  if (const int rc = lds_for(kernel, C::LDS)) return rc;
-  const int tm = (int)(up(g.m, C::BM) / C::BM), tn = (int)(up(g.n, C::BN) / C::BN);
-  hipLaunchKernelGGL(kernel, dim3(tm * tn * g.split), dim3(C::THREADS), C::LDS, a.stream, g, tm, tn);
-  return 0;
-}
-template <class T>
-void join_launch(const Call& a, const Grad& g) {
-  const int64_t blocks = ((int64_t)g.n * g.m + 1023) / 1024;
-  hipLaunchKernelGGL(k_ce_join<T>, dim3((unsigned)(blocks > 4096 ? 4096 : blocks)), dim3(256), 0, a.stream, g);
+  return finish<T>(a, l, tiles);
 }
 
 template <class T>
 int backward(const Call& a) {
-  typedef typename Piece<T>::type E;
   constexpr int P = sizeof(T) == 4 ? 2 : 1;
-  typedef Main C;
   const Layout l = layout_of(a.c, direct(a.h, a.h0, a.h1, a.c), direct(a.w, a.w0, a.w1, a.c), true, a.gb != nullptr);
   if (!a.ws || (int64_t)a.ws_bytes < l.bytes) return set_error(GRLHIP_ERR_WORKSPACE, "linear_ce_backward: workspace too small: need " + std::to_string(l.bytes));
   Scalars* s = (Scalars*)(a.ws + l.scalars);
-  begin<T>(a, s);
+  if (!__is_same(T, _Float16)) absmax_launch<T>(a, s);
   float* scale = (float*)(a.ws + l.scale);
-  const Scale sc{a.grad, a.grad_stride, a.row_weight, a.count, a.target, a.ignore, (int)a.c.rows, (int)a.c.vocab, a.reduction, scale, s};
-  hipLaunchKernelGGL(k_ce_scale, dim3((unsigned)((a.c.rows + 255) / 256)), dim3(256), 0, a.stream, sc);
-  const View h{a.h, a.h0, a.h1, (int)a.c.rows, (int)a.c.hidden};
-  pack<T>(a, h, l.pack_h ? a.ws + l.hp : nullptr, l.kp, a.gw ? a.ws + l.ht : nullptr, l.np, &s->hmax, true);
-  const auto kernel = k_ce_d<E, P, C>;
-  if (const int rc = lds_for(kernel, C::LDS)) return rc;
-  Grad gh = {};
+  const int side = SIDE[l.kind_z];
+  const int64_t tn = up(a.c.rows, side) / side;
   for (int64_t v0 = 0; v0 < a.c.vocab; v0 += l.piece) {
-    const int64_t cols = a.c.vocab - v0 < l.piece ? a.c.vocab - v0 : l.piece, vp = up(cols, 64);
+    const bool first = v0 == 0, last = v0 + l.piece >= a.c.vocab;
+    const int64_t cols = last ? a.c.vocab - v0 : l.piece, vp = up(cols, 64);
     const View w = weight_piece<T>(a, v0, cols);
-    pack<T>(a, w, l.pack_w ? a.ws + l.wp : nullptr, l.kp, a.gh ? a.ws + l.wt : nullptr, vp, &s->wmax, false);
-    Logits g = {};
-    g.h = l.pack_h ? Operand{a.ws + l.hp, l.kp * 2 * P} : Operand{(const char*)a.h, a.h0 * 2};
-    g.w = l.pack_w ? Operand{a.ws + l.wp, l.kp * 2 * P} : Operand{(const char*)w.p, a.w0 * 2};
-    g.bias = a.bias ? a.bias + v0 : nullptr;
-    g.target = a.target;
+    const Job jh{hidden_of(a), first && l.pack_h ? a.ws + l.hp : nullptr, l.kp, first && a.gw ? a.ws + l.ht : nullptr, l.np, true, 0};
+    const Job jw{w, l.pack_w ? a.ws + l.wp : nullptr, l.kp, a.gh ? a.ws + l.wt : nullptr, vp, false, 0};
+    int64_t gblocks = (a.c.rows + 255) / 256;
+    if (gblocks > GMAX) gblocks = GMAX;
+    const Scale sc{a.grad, a.grad_stride, a.row_weight, a.count, a.target, a.ignore, (int)a.c.rows, (int)a.c.vocab, a.reduction, first ? (int)gblocks : 0, scale};
+    pack_launch<T>(a, jh, jw, sc, s);
+
+    Logits g = logits_call<T>(a, l, w, v0, s);
     g.lse = a.lse;
     g.scale = scale;
-    g.s = s;
-    g.rows = (int)a.c.rows;
-    g.v0 = (int)v0;
-    g.cols = (int)cols;
-    g.nkb = (int)(l.kp * 2 * P / KBLOCK);
     g.d = a.ws + l.d;
     g.d_cols = vp;
     g.dt = a.ws + l.dt;
     g.dt_cols = l.np;
     g.bpart = a.gb ? (float*)(a.ws + l.bpart) : nullptr;
-    const int tm = (int)(up(cols, C::BM) / C::BM), tn = (int)(up(a.c.rows, C::BN) / C::BN);
-    hipLaunchKernelGGL(kernel, dim3(tm * tn), dim3(C::THREADS), C::LDS, a.stream, g, tm, tn);
-    if (a.gb) hipLaunchKernelGGL(k_ce_bias, dim3((unsigned)((cols + 255) / 256)), dim3(256), 0, a.stream, g.bpart, tn, (int)cols, a.gb + v0);
+    const int tm = (int)(up(cols, side) / side);
+#define CALL(C) tile_launch(k_ce_d<typename Operands<T>::type, P, C>, tm * tn, C::THREADS, C::LDS, a.stream, g, tm, (int)tn)
+    if (const int rc = BY_KIND(l.kind_z, CALL)) return rc;
+#undef CALL
+
+    Join j = {};
+    Grad &gh = j.both.g[0], &gw = j.both.g[1];
+    j.both.s = s;
     if (a.gh) {
-      gh = Grad{};
       gh.a = {a.ws + l.wt, vp * 2 * P};
       gh.b = {a.ws + l.d, vp * 2 * P};
       gh.m = (int)a.c.hidden;
       gh.n = (int)a.c.rows;
       gh.nkb = (int)(vp * 2 * P / KBLOCK);
       gh.split = l.split_h;
+      gh.tiles = (int)tiles_of(gh.m, gh.n, l.kind_g) * gh.split;
       gh.slots = l.hslots ? (float*)(a.ws + l.hslots) : nullptr;
-      gh.add = v0 > 0;
+      gh.add = !first;
       gh.out = a.gh;
-      gh.o0 = a.c.hidden;
-      gh.o1 = 1;
       gh.scale = scale;
-      gh.s = s;
       gh.by_w = 1;
-      if (const int rc = grad_launch<T, C>(a, gh)) return rc;
+      if (gh.slots && last) j.blocks[0] = join_blocks(gh);
     }
     if (a.gw) {
-      Grad gw = {};
       gw.a = {a.ws + l.ht, l.np * 2 * P};
       gw.b = {a.ws + l.dt, l.np * 2 * P};
       gw.m = (int)a.c.hidden;
       gw.n = (int)cols;
       gw.nkb = (int)(l.np * 2 * P / KBLOCK);
       gw.split = l.split_w;
+      gw.tiles = (int)tiles_of(gw.m, gw.n, l.kind_g) * gw.split;
       gw.slots = l.wslots ? (float*)(a.ws + l.wslots) : nullptr;
       gw.out = (T*)a.gw + v0 * a.c.hidden;
-      gw.o0 = a.c.hidden;
-      gw.o1 = 1;
-      gw.s = s;
-      if (const int rc = grad_launch<T, C>(a, gw)) return rc;
-      if (gw.slots) join_launch<T>(a, gw);
+      if (gw.slots) j.blocks[1] = join_blocks(gw);
     }
+    if (gh.tiles + gw.tiles > 0) {
+#define CALL(C) tile_launch(k_ce_grad<T, P, C>, gh.tiles + gw.tiles, C::THREADS, C::LDS, a.stream, j.both)
+      if (const int rc = BY_KIND(l.kind_g, CALL)) return rc;
+#undef CALL
+    }
+    int blocks = j.blocks[0] + j.blocks[1];
+    if (a.gb) {
+      j.bpart = g.bpart;
+      j.btiles = (int)tn;
+      j.cols = (int)cols;
+      j.gb = a.gb + v0;
+      blocks += (int)((cols + 255) / 256);
+    }
+    if (blocks > 0) hipLaunchKernelGGL(k_ce_join<T>, dim3(blocks), dim3(256), 0, a.stream, j);
   }
-  if (a.gh && gh.slots) join_launch<T>(a, gh);
   LAUNCH_TRY(hipGetLastError());
   return 0;
 }
@@ -778,7 +902,8 @@ int grlhip_linear_ce_forward(const void* hidden, const int64_t* hidden_strides, 
     a.ws_bytes = workspace_bytes;
     a.stream = (hipStream_t)stream;
     if (const int rc = check("linear_ce_forward", a)) return rc;
-    if (!losses || !total) return set_error(GRLHIP_ERR_INVALID, "linear_ce_forward: null losses or total");
+    if (!losses) return set_error(GRLHIP_ERR_INVALID, "linear_ce_forward: null losses");
+    if (!total != !count || (!total && reduction != GRLHIP_REDUCE_NONE)) return set_error(GRLHIP_ERR_INVALID, "linear_ce_forward: total and count go together, and may be NULL for GRLHIP_REDUCE_NONE only");
     if ((size_t)workspace & 255) return set_error(GRLHIP_ERR_INVALID, "linear_ce_forward: the workspace must be aligned to 256 bytes");
     return elem == GRLHIP_ELEM_F32 ? forward<float>(a) : elem == GRLHIP_ELEM_BF16 ? forward<__bf16>(a) : forward<_Float16>(a);
   });
@@ -813,7 +938,7 @@ int grlhip_linear_ce_backward(const void* hidden, const int64_t* hidden_strides,
     a.ws_bytes = workspace_bytes;
     a.stream = (hipStream_t)stream;
     if (const int rc = check("linear_ce_backward", a)) return rc;
-    if (!grad) return set_error(GRLHIP_ERR_INVALID, "linear_ce_backward: null gradient");
+    if (!grad || (!count && reduction == GRLHIP_REDUCE_MEAN)) return set_error(GRLHIP_ERR_INVALID, "linear_ce_backward: null gradient or count");
     if ((size_t)workspace & 255) return set_error(GRLHIP_ERR_INVALID, "linear_ce_backward: the workspace must be aligned to 256 bytes");
     if (!grad_hidden && !grad_weight && !grad_bias) return 0;
     return elem == GRLHIP_ELEM_F32 ? backward<float>(a) : elem == GRLHIP_ELEM_BF16 ? backward<__bf16>(a) : backward<_Float16>(a);

@@ -46,7 +46,9 @@ class _Head:
         """(losses, logsumexp, reduced loss, number of rows that are not ignored)"""
         dev = self.hidden.device
         losses, lse = (torch.empty(self.rows, dtype=torch.float32, device=dev) for _ in range(2))
-        total, count = (torch.empty((), dtype=torch.float32, device=dev) for _ in range(2))
+        total = count = None
+        if self.reduction != L.REDUCE_NONE:
+            total, count = (torch.empty((), dtype=torch.float32, device=dev) for _ in range(2))
         self.call(L.lib().grlhip_linear_ce_forward, self.workspace(False), _ptr(losses), _ptr(lse), _ptr(total), _ptr(count))
         return losses, lse, total, count
 

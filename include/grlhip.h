@@ -378,12 +378,12 @@ typedef enum { GRLHIP_REDUCE_NONE = 0, GRLHIP_REDUCE_MEAN = 1, GRLHIP_REDUCE_SUM
  * vocabulary (discretised actions), without storing the logits z = hidden weight^T + bias:
  *   losses[i] = row_weight[i] (logsumexp_v z[i][v] - z[i][target[i]]);   lse[i] = logsumexp_v z[i][v]
  *   *total = sum of the losses (GRLHIP_REDUCE_SUM, _NONE) or that over *count (_MEAN); *count = number of rows whose target is
- *   not ignore_index, at least 1.
+ *   not ignore_index, at least 1.  Both may be NULL for GRLHIP_REDUCE_NONE.
  * hidden [rows][features], weight [vocab][features]: element type `elem`, element strides {row, column} in HOST arrays (NULL:
  * dense).  bias [vocab] fp32 or NULL; -inf masks an entry.  target [rows] int64; row_weight [rows] fp32 or NULL (1).
  * A row whose target is ignore_index or whose weight is 0 has loss 0 and contributes nothing, whatever its hidden row holds.  Any other
  * target outside [0, vocab): loss and gradients NaN.  A row with every entry masked: NaN.
- * rows, features, vocab: 1 to 2^20, 2^16, 2^21.  Results repeat bit for bit.  Workspace: grlhip_linear_ce_workspace_bytes for the
+ * rows, features, vocab: 1 to 2^20, 2^16, 2^21, and at most 2^34 entries of hidden and of weight.  Results repeat bit for bit.  Workspace: grlhip_linear_ce_workspace_bytes for the
  * same operands (backward = 0), 256-byte aligned. */
 size_t grlhip_linear_ce_workspace_bytes(const void* hidden, const int64_t* hidden_strides, const void* weight,
                                         const int64_t* weight_strides, int64_t rows, int64_t features, int64_t vocab, int elem,

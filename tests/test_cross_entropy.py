@@ -5,7 +5,7 @@ Tolerances, entry by entry, from the arithmetic (K features, N rows, u the half 
       16 products in fp32: (K / 16 + 16) 2^-24 of sum_k |h| |w|.
   loss: the largest error of z in the row twice (logsumexp and the target), 2^-21 of the magnitudes for exp, log and sums.
   D = softmax - onehot: twice the error of z and exp's own |z - lse| 2^-22 relative to the softmax, then the rounding of D
-      (u of a 16-bit type, 2^-21 for pieces, 2^-38 absolute for fp16's smallest numbers).
+      (u of fp16, 2^-21 for two pieces, 2^-38 absolute for fp16's smallest numbers).
   dh, dW: these times |W|, |h|; the fp32 sum over V or N; the result's own rounding (u, and fp16's smallest number)."""
 import ctypes
 import math
@@ -72,8 +72,8 @@ def oracle(h, w, t, b, rw, reduction, upstream=None):
     ep = p * (2 * e_row.unsqueeze(1) + (torch.where(z.isfinite(), (z - lse.unsqueeze(1)).abs(), 0.0) + 2) * 2.0 ** -22)
     d = p.clone()
     d.scatter_add_(1, at, torch.full_like(d[:, :1], -1.0))
-    u = {F32: 2.0 ** -21, BF16: torch.finfo(BF16).eps / 2, F16: torch.finfo(F16).eps / 2}[kind]
-    ed = ep + u * d.abs() + (0.0 if kind == BF16 else 2.0 ** -38)
+    u = 2.0 ** -21 if kind == F32 else torch.finfo(F16).eps / 2
+    ed = ep + u * d.abs() + 2.0 ** -38
     d, ed = torch.where(kept.unsqueeze(1), d, 0.0), torch.where(kept.unsqueeze(1), ed, 0.0)
     g = torch.where(kept, g, 0.0)
     uo = torch.finfo(kind).eps / 2
@@ -83,7 +83,7 @@ def oracle(h, w, t, b, rw, reduction, upstream=None):
     edh = (ed + (v / 16 + 16 + 64) * 2.0 ** -24 * d.abs()) @ W.abs() * g.abs().unsqueeze(1)
     gd, egd = d * g.unsqueeze(1), (ed + (n / 16 + 16 + 64) * 2.0 ** -24 * d.abs()) * g.abs().max()
     egd = torch.where(kept.unsqueeze(1), (ep + u * d.abs() + (n / 16 + 80) * 2.0 ** -24 * d.abs()) * g.abs().unsqueeze(1)
-                      + (0.0 if kind == BF16 else 2.0 ** -37 * g.abs().max()), 0.0)
+                      + 2.0 ** -37 * g.abs().max(), 0.0)
     dw = gd.t() @ H
     edw = egd.t() @ H.abs()
     out["dh"] = (dh, edh + uo * (dh.abs() + edh) + 2.0 ** -21 * dh.abs() + least)
@@ -394,6 +394,7 @@ def test_c_entry_points_check_their_arguments_without_a_gpu():
         return lib.grlhip_linear_ce_backward(h, None, w, None, None, t, -100, None, n, 8, 10, L.ELEM_F32, red, lse, count, grad, 0, gh, None, None, ws, bytes_, None)
 
     assert fwd() == -4 and bwd() == -4 and b"workspace" in lib.grlhip_last_error()
+    assert fwd(total=None, count=None) == -1 and fwd(total=None, count=None, red=L.REDUCE_NONE) == -4
     for bad in ("h", "w", "t", "losses", "lse", "total", "count"):
         assert fwd(**{bad: None}) == -1, bad
     for bad in ("h", "w", "t", "lse", "count", "grad"):
