@@ -211,19 +211,24 @@ struct Logits {
   float* bpart;             // [row tiles][cols] partial sums of the bias' gradient, or null
 };
 
-// z of one 32 x 32 block
-template <int P>
-__device__ __forceinline__ void logits_of(const Logits& a, const f32x16& acc, int mb, int h, float fh, float fw, float (&z)[16]) {
+// The accumulators of 32 rows of the tile (vocabulary entries from mb on) become z, in place.
+template <int P, int TN>
+__device__ __forceinline__ void logits_of(const Logits& a, f32x16 (&acc)[TN], int mb, int h, float fh, float fw) {
+  if (P == 2)
 #pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    const int m = mb + 8 * (r >> 2) + 4 * h + (r & 3);
-    float v = acc[r];
-    if (P == 2) v = v * fh * fw;
-    if (a.bias && m < a.cols) v += a.bias[m];
-    z[r] = v;
-  }
+    for (int x = 0; x < TN; ++x) acc[x] = acc[x] * fh * fw;   // one at a time: their product may leave fp32's range
+  if (a.bias)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int m = mb + 8 * (r >> 2) + 4 * h + (r & 3);
+      const float b = a.bias[m < a.cols ? m : a.cols - 1];
+#pragma unroll
+      for (int x = 0; x < TN; ++x) acc[x][r] += b;
+    }
 }
 
+// The epilogue is most of a tile's time where the features are few (8 K blocks of 512 features: 15 us of products): ~9 operations an
+// entry -- exp counts for 4 -- and what concerns few entries (the end of the vocabulary, the targets) under branches of the whole wave.
 template <class T, int P, class C>
 __global__ __launch_bounds__(C::THREADS, C::LDS > 81920 ? C::THREADS / 256 : C::THREADS / 128) void k_ce_forward(Logits a, int tm, int tn) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
@@ -238,29 +243,41 @@ __global__ __launch_bounds__(C::THREADS, C::LDS > 81920 ? C::THREADS / 256 : C::
   float* tops = (float*)lds;                  // [WM][BN] maxima, then sums
   float* sums = tops + C::WM * C::BN;
 #pragma unroll
+  for (int y = 0; y < C::TM; ++y) {
+    const int mb = m0 + (wm * C::TM + y) * 32;
+    logits_of<P>(a, acc[y], mb, L.h, fh, fw);
+    if (mb + 32 > a.cols)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (mb + 8 * (r >> 2) + 4 * L.h + (r & 3) >= a.cols)
+#pragma unroll
+          for (int x = 0; x < C::TN; ++x) acc[y][x][r] = -INFINITY;
+  }
+#pragma unroll
   for (int x = 0; x < C::TN; ++x) {
     const int nl = (wn * C::TN + x) * 32 + L.j, n = n0 + nl;
-    const int64_t t = n < a.rows ? a.target[n] - a.v0 : -1;
-    float top = -INFINITY, z[C::TM][16];
+    const int64_t t = (n < a.rows ? a.target[n] : -1) - a.v0 - m0 - wm * C::TM * 32;
+    const int rel = t >= 0 && t < C::TM * 32 && t + m0 + wm * C::TM * 32 < a.cols ? (int)t : -1;   // the target's row of this wave's part
+    if (__any(rel >= 0)) {
 #pragma unroll
-    for (int y = 0; y < C::TM; ++y) {
-      const int mb = m0 + (wm * C::TM + y) * 32;
-      logits_of<P>(a, acc[y][x], mb, L.h, fh, fw, z[y]);
+      for (int y = 0; y < C::TM; ++y)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int m = mb + 8 * (r >> 2) + 4 * L.h + (r & 3);
-        if (m == t && m < a.cols) a.picked[n] = z[y][r];
-        if (m >= a.cols) z[y][r] = -INFINITY;
-        top = fmaxf(top, z[y][r]);
-      }
+        for (int r = 0; r < 16; ++r)
+          if (rel == y * 32 + 8 * (r >> 2) + 4 * L.h + (r & 3)) a.picked[n] = acc[y][x][r];
     }
-    top = fmaxf(top, __shfl_xor(top, 32));
-    float sum = 0.f;
-    // nothing but -inf: no sum, whatever -inf - -inf is.  A NaN logit passes fmaxf, and is caught by the sum
+    float top = -INFINITY;
 #pragma unroll
     for (int y = 0; y < C::TM; ++y)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) sum += z[y][r] == -INFINITY ? 0.f : __expf(z[y][r] - top);
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, acc[y][x][r]);
+    top = fmaxf(top, __shfl_xor(top, 32));
+    // nothing but -inf: a sum of zeros, not of -inf - -inf.  A NaN passes fmaxf, and is caught by the sum
+    const float ref = top == -INFINITY ? 0.f : top;
+    float sum = 0.f;
+#pragma unroll
+    for (int y = 0; y < C::TM; ++y)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sum += __expf(acc[y][x][r] - ref);
     sum += __shfl_xor(sum, 32);
     if (L.h == 0) {
       tops[wm * C::BN + nl] = top;
@@ -371,31 +388,52 @@ __global__ __launch_bounds__(C::THREADS, C::LDS > 81920 ? C::THREADS / 256 : C::
   const Lane L = lane_of();
   const int wm = L.wave / C::WN, wn = L.wave % C::WN;
   const float fh = P == 2 ? 1.f / scale_of(a.s->h) : 1.f, fw = P == 2 ? 1.f / scale_of(a.s->w) : 1.f;
-  const float per = 1.f / ceil_of(largest_gradient(a.s));
+  const float per = DSCALE / ceil_of(largest_gradient(a.s));
   unsigned* patch = (unsigned*)(lds + L.wave * PATCH);
   float* bsum = (float*)(lds + C::WAVES * PATCH);   // [WN][BM]
+  float lse[C::TN], g[C::TN];
+  int64_t t[C::TN];
+#pragma unroll
+  for (int x = 0; x < C::TN; ++x) {
+    const int n = n0 + (wn * C::TN + x) * 32 + L.j;
+    lse[x] = n < a.rows ? a.lse[n] : 0.f;
+    g[x] = n < a.rows ? a.scale[n] : 0.f;
+    t[x] = (n < a.rows ? a.target[n] : -1) - a.v0;
+  }
 #pragma unroll
   for (int y = 0; y < C::TM; ++y) {
     const int mb = m0 + (wm * C::TM + y) * 32;
+    logits_of<P>(a, acc[y], mb, L.h, fh, fw);
     float bs[16];
 #pragma unroll
     for (int r = 0; r < 16; ++r) bs[r] = 0.f;
 #pragma unroll
     for (int x = 0; x < C::TN; ++x) {
-      const int nb = n0 + (wn * C::TN + x) * 32, n = nb + L.j;
-      const bool in_rows = n < a.rows;
-      const float lse = in_rows ? a.lse[n] : 0.f, g = in_rows ? a.scale[n] : 0.f;
-      const int64_t t = in_rows ? a.target[n] - a.v0 : -1;
+      const int nb = n0 + (wn * C::TN + x) * 32;
+      const bool dead = g[x] == 0.f;   // a row that does not count, whatever its logits are
       float z[16], v[16];
-      logits_of<P>(a, acc[y][x], mb, L.h, fh, fw, z);
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const int m = mb + 8 * (r >> 2) + 4 * L.h + (r & 3);
-        float p = __expf(z[r] - lse) - (m == t ? 1.f : 0.f);
-        if (m >= a.cols || g == 0.f) p = 0.f;
-        z[r] = p * DSCALE;
-        v[r] = m >= a.cols || g == 0.f ? 0.f : p * (g * per) * DSCALE;
-        bs[r] += m >= a.cols || g == 0.f ? 0.f : p * g;
+        const float p = __expf(acc[y][x][r] - lse[x]);
+        z[r] = dead ? 0.f : p;
+      }
+      const int rel = t[x] >= mb && t[x] < mb + 32 && !dead ? (int)(t[x] - mb) : -1;
+      if (__any(rel >= 0)) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) z[r] -= rel == 8 * (r >> 2) + 4 * L.h + (r & 3) ? 1.f : 0.f;
+      }
+      if (mb + 32 > a.cols)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (mb + 8 * (r >> 2) + 4 * L.h + (r & 3) >= a.cols) z[r] = 0.f;
+      if (a.bpart)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) bs[r] += z[r] * g[x];
+      const float gd = g[x] * per;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        v[r] = z[r] * gd;
+        z[r] *= DSCALE;
       }
       if (nb < a.rows && mb < a.d_cols) {
         if constexpr (P == 2) store_t_f16x2((_Float16*)a.d + (int64_t)nb * 2 * a.d_cols + mb * 2, 2 * a.d_cols, patch, L, a.rows - nb, z);
@@ -569,8 +607,8 @@ int kind_for(int64_t m, int64_t n, int64_t kb, int p, double entry_ns) {
     if (launch_us((double)tiles_of(m, n, k), (double)kb, p, k, entry_ns) < launch_us((double)tiles_of(m, n, best), (double)kb, p, best, entry_ns)) best = k;
   return best;
 }
-constexpr double FORWARD_NS = 0.15;   // exponentials
-double d_ns(int p) { return 0.2 + 4.0 * p / 15; }   // exponentials, and 4 or 8 bytes written at a CU's share of the memory
+constexpr double FORWARD_NS = 0.1;   // exponentials
+double d_ns(int p) { return 0.1 + 4.0 * p / 15; }   // exponentials, and 4 or 8 bytes written at a CU's share of the memory
 
 // How a call goes about it: the same for its workspace and its launches.
 struct Layout {
@@ -615,7 +653,7 @@ Layout layout_of(const Shape& c, bool direct_h, bool direct_w, bool backward, bo
   l.np = up(c.rows, 64);
   l.pack_h = !direct_h;
   l.pack_w = !direct_w;
-  int64_t limit = backward ? PIECE / l.np : l.pack_w ? PIECE / l.kp : c.vocab;
+  int64_t limit = backward ? PIECE / l.np : l.pack_w ? PIECE / l.kp : up(c.vocab, 256);
   limit = limit < 1024 ? 1024 : limit / 256 * 256;
   if (backward && limit > 1 << 19) limit = 1 << 19;                            // row offsets inside a tile are 32 bits
   const int64_t most = (1 << 20) / (up(c.rows, 64) / 64) * 64;                 // and so is a launch
