@@ -302,6 +302,171 @@ __global__ __launch_bounds__(C::THREADS, C::LDS > 81920 ? C::THREADS / 256 : C::
   }
 }
 
+// ------------------------------------------------------------------------------------------------- small matrices
+// A matrix whose sides are at most 64 and 192 stays in one workgroup's LDS from the first load to the last store: X, X^T, A and B as
+// pieces, a barrier between products.  One launch for the group where the chain has 17, each of which lasts 4 us however little
+// it does: 128 x 64 in 28 us (chain: 75), 16 x 16 in 12.  What bounds it is latency -- 9 500 cycles a step of 128 x 64 --, hence 16 waves with a 16 x 16 block each (16x16x32 instructions, a third of the 32 x 32 block's
+// dependent time), one accumulator for each of the three products of pieces.
+constexpr int SMALL_M = 64, SMALL_N = 192, SMALL_THREADS = 1024, SMALL_WAVES = SMALL_THREADS / 64;
+constexpr int SMALL_X = SMALL_M * (SMALL_N * 4 + 16), SMALL_XT = SMALL_N * (SMALL_M * 4 + 16), SMALL_A = SMALL_M * (SMALL_M * 4 + 16);
+constexpr int SMALL_LDS = SMALL_X + SMALL_XT + 2 * SMALL_A;
+
+// Rows of K blocks (32 high pieces, 32 low ones), 16 bytes apart from a multiple of 128: 16 rows of one chunk then lie in different banks
+struct Plane {
+  unsigned char* p; int pitch;   // bytes
+  __device__ Plane(unsigned char* at_, int cols) : p(at_), pitch(cols * 4 + 16) {}
+  __device__ unsigned char* at(int row, int col) const { return p + row * pitch + (col >> 5) * 128 + (col & 31) * 2; }   // the high piece; the low one is 64 further
+  __device__ void put(int row, int col, _Float16 hi, _Float16 lo) const {
+    unsigned char* q = at(row, col);
+    *(_Float16*)q = hi;
+    *(_Float16*)(q + 64) = lo;
+  }
+};
+typedef float f32x4a __attribute__((ext_vector_type(4)));
+// Sum over kb of rows ra.. of a and rows rb.. of b: a lane's entries are rows 4 (lane / 16) + i of a, row lane % 16 of b.
+__device__ __forceinline__ f32x4a small_product(Plane a, int ra, Plane b, int rb, int nkb, int lane) {
+  f32x4a hh = {0.f, 0.f, 0.f, 0.f}, hl = hh, lh = hh;
+  const unsigned char *pa = a.p + (ra + (lane & 15)) * a.pitch + (lane >> 4) * 16, *pb = b.p + (rb + (lane & 15)) * b.pitch + (lane >> 4) * 16;
+#pragma unroll 2
+  for (int kb = 0; kb < nkb; ++kb) {
+    const f16x8 ah = *(const f16x8*)(pa + kb * 128), al = *(const f16x8*)(pa + kb * 128 + 64);
+    const f16x8 bh = *(const f16x8*)(pb + kb * 128), bl = *(const f16x8*)(pb + kb * 128 + 64);
+    hl = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, bl, hl, 0, 0, 0);
+    lh = __builtin_amdgcn_mfma_f32_16x16x32_f16(al, bh, lh, 0, 0, 0);
+    hh = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, bh, hh, 0, 0, 0);
+  }
+  return hh + (hl + lh);
+}
+// Values of a block -> row n, 4 entries from m of `t`, and (both) rows m.., entry n of `d`.
+__device__ __forceinline__ void small_store(Plane t, Plane d, bool both, int m, int n, f32x4a v) {
+  f16x4 hi, lo;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    _Float16 x, y;
+    split2(v[i], x, y);
+    hi[i] = x;
+    lo[i] = y;
+    if (both) d.put(m + i, n, x, y);
+  }
+  unsigned char* q = t.at(n, m);
+  *(f16x4*)q = hi;
+  *(f16x4*)(q + 64) = lo;
+}
+__device__ __forceinline__ f32x4a small_load(Plane t, int m, int n) {
+  const unsigned char* q = t.at(n, m);
+  const f16x4 hi = *(const f16x4*)q, lo = *(const f16x4*)(q + 64);
+  f32x4a v;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = (float)hi[i] + (float)lo[i];
+  return v;
+}
+
+// entry k of a matrix, counted along the axis that is dense in memory.  The quotient of k < 2^14 by a side < 2^8 in fp32: off by less
+// than the 1 / 2^9 that (k + 1/2) / side keeps from the next integer.
+struct Spread {
+  bool along; int inner; float inverse;
+  __device__ Spread(bool along_n, const Mat& a) : along(along_n), inner(along_n ? a.n : a.m) { inverse = 1.f / inner; }
+  __device__ void at(int k, int& r, int& c) const {
+    const int o = (int)((k + 0.5f) * inverse), i = k - o * inner;
+    r = along ? o : i;
+    c = along ? i : o;
+  }
+};
+
+template <class T, bool MUON>
+__global__ __launch_bounds__(SMALL_THREADS, 4) void k_orth_small(Group g, int steps) {
+  extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
+  __shared__ double sh[SMALL_WAVES];
+  const Mat& a = g.mat[blockIdx.x];
+  const int mp = (int)up32(a.m), np = (int)up32(a.n);
+  const Lane L = lane_of();
+  const Plane X(lds, np), XT(lds + SMALL_X, mp), A(lds + SMALL_X + SMALL_XT, mp), B(lds + SMALL_X + SMALL_XT + SMALL_A, mp);
+  // momentum and norm; threads along the axis that is dense in memory, all of a thread's loads in flight at once
+  constexpr int PER = SMALL_M * SMALL_N / SMALL_THREADS;
+  const int all = a.m * a.n;
+  const Spread in{a.gs[1] <= a.gs[0], a}, to{a.os[1] <= a.os[0], a};
+  float u[PER];
+  double s = 0.0;
+#pragma unroll
+  for (int e = 0; e < PER; ++e) {
+    const int k = threadIdx.x + e * SMALL_THREADS;
+    int r, c;
+    in.at(k, r, c);
+    u[e] = k < all ? direction<T, MUON, true>(g.num, a, r, c) : 0.f;
+  }
+#pragma unroll
+  for (int e = 0; e < PER; ++e) s += (double)u[e] * u[e];
+  for (int k = threadIdx.x; k < (SMALL_X + SMALL_XT) / 16; k += SMALL_THREADS) ((u32x4*)lds)[k] = u32x4{0, 0, 0, 0};   // the padding stays zero
+  for (int d = 32; d > 0; d >>= 1) s += __shfl_xor(s, d);
+  if (L.lane == 0) sh[L.wave] = s;
+  __syncthreads();
+  s = 0.0;
+#pragma unroll
+  for (int k = 0; k < SMALL_WAVES; ++k) s += sh[k];
+  const double inv = factor_of(s, g.num.eps);
+#pragma unroll
+  for (int e = 0; e < PER; ++e) {
+    const int k = threadIdx.x + e * SMALL_THREADS;
+    if (k >= all) continue;
+    int r, c;
+    in.at(k, r, c);
+    _Float16 hi, lo;
+    split2((float)(u[e] * inv), hi, lo);
+    X.put(r, c, hi, lo);
+    XT.put(c, r, hi, lo);
+  }
+  __syncthreads();
+
+  constexpr int EACH = SMALL_M / 16 * (SMALL_N / 16) / SMALL_WAVES;
+  const int lane = L.lane, m4 = 4 * (lane >> 4), n1 = lane & 15, tm = mp / 16, tn = np / 16;
+  // the symmetric products: block w of the lower triangle by wave w
+  int bm = 0;
+  while ((bm + 1) * (bm + 2) / 2 <= L.wave) ++bm;
+  const int bn = L.wave - bm * (bm + 1) / 2;
+  const bool sym = bm < tm;
+  for (int step = 0; step < steps; ++step) {
+    if (sym) small_store(A, A, bm != bn, bm * 16 + m4, bn * 16 + n1, small_product(X, bm * 16, X, bn * 16, np / 32, lane) * (1.f / S));
+    __syncthreads();
+    if (sym) {
+      const f32x4a own = small_load(A, bm * 16 + m4, bn * 16 + n1);
+      small_store(B, B, bm != bn, bm * 16 + m4, bn * 16 + n1,
+                  g.num.cb * own + (g.num.cc * (1.f / S)) * small_product(A, bm * 16, A, bn * 16, mp / 32, lane));
+    }
+    __syncthreads();
+    f32x4a v[EACH];
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+      const int b = L.wave + e * SMALL_WAVES, im = b % tm * 16, in = b / tm * 16;
+      if (b < tm * tn) v[e] = g.num.ca * small_load(XT, im + m4, in + n1) + (1.f / S) * small_product(B, im, XT, in, mp / 32, lane);
+    }
+    __syncthreads();   // everybody has read X before it is written
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+      const int b = L.wave + e * SMALL_WAVES, im = b % tm * 16, in = b / tm * 16;
+      if (b < tm * tn) small_store(XT, X, true, im + m4, in + n1, v[e]);
+    }
+    __syncthreads();
+  }
+  // the result, threads along memory again: the one rounding to the matrix' type (pieces hold 22 bits)
+  float old[PER];
+#pragma unroll
+  for (int e = 0; e < PER; ++e) {
+    const int k = threadIdx.x + e * SMALL_THREADS;
+    int r, c;
+    to.at(k, r, c);
+    old[e] = MUON && k < all ? (float)((T*)a.out)[r * a.os[0] + c * a.os[1]] : 0.f;
+  }
+#pragma unroll
+  for (int e = 0; e < PER; ++e) {
+    const int k = threadIdx.x + e * SMALL_THREADS;
+    if (k >= all) continue;
+    int r, c;
+    to.at(k, r, c);
+    const float d = ((float)*(_Float16*)X.at(r, c) + (float)*(_Float16*)(X.at(r, c) + 64)) * (1.f / S);
+    ((T*)a.out)[r * a.os[0] + c * a.os[1]] = MUON ? (T)(g.num.keep * old[e] - a.rate * d) : (T)d;
+  }
+}
+
 // steps == 0: the normalised matrix itself
 template <class T, bool MUON>
 __global__ __launch_bounds__(256) void k_orth_join(Table t, Numbers g) {
@@ -490,6 +655,23 @@ int run(const char* who, const Call& c, char* ws, size_t ws_bytes, hipStream_t s
   const int present = (int)order.size();
   if (present == 0) return 0;
   const Numbers num{c.ca, c.cb, c.cc, c.eps, (float)c.momentum, (float)(1.0 - c.momentum), c.keep, c.nesterov};
+  bool small = true;
+  for (const int i : order) {
+    const Parts p = parts_of(c.shapes + 2 * i);
+    small = small && p.mp <= SMALL_M && p.np <= SMALL_N;
+  }
+  if (small) {
+    const auto kernel = k_orth_small<T, MUON>;
+    LAUNCH_TRY(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, SMALL_LDS));
+    for (int done = 0; done < present;) {
+      Group g = {};
+      for (; done < present && g.count < GROUP; ++done) g.mat[g.count++] = describe<MUON>(c, order[done]);
+      g.num = num;
+      hipLaunchKernelGGL(kernel, dim3((unsigned)g.count), dim3(SMALL_THREADS), SMALL_LDS, stream, g, c.steps);
+    }
+    LAUNCH_TRY(hipGetLastError());
+    return 0;
+  }
   const Plan plan = plan_of(c.shapes, c.count);
   if (plan.blocks > 1 << 30 || plan.tiles[0] > 1 << 22 || plan.tiles[1] > 1 << 22 || plan.tiles[2] > 1 << 22)
     return set_error(GRLHIP_ERR_UNSUPPORTED, std::string(who) + ": too many matrices for one call");

@@ -98,6 +98,10 @@ def test_gpu_orthogonalize_takes_strides_batches_and_lists():
         for i in range(b.shape[0]):
             for k in range(b.shape[1]):
                 assert off(got[i, k], polar(b[i, k])) <= TOL
+    # more small matrices than one launch describes (a workgroup each), with every side of the padding
+    few = [grad_like(1 + 3 * k % 64, 190 - 5 * k, seed=k) for k in range(37)] + [grad_like(64, 192), grad_like(192, 33), grad_like(65, 4)[:64]]
+    for g, m in zip(optim.orthogonalize(few), few):
+        assert off(g, polar(m)) <= TOL
     # more matrices than one launch describes, of all shapes; empty ones among them
     many = [grad_like(5 + 7 * k, 90 - 3 * k, seed=k) for k in range(29)] + [torch.empty(0, 5, device=DEV), torch.empty(2, 0, 3, device=DEV),
                                                                             torch.empty(0, 4, 4, device=DEV)]
