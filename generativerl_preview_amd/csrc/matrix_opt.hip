@@ -546,20 +546,21 @@ int check_coefficients(const char* who, float a, float b, float c, int steps) {
 }
 
 // The shapes of tiles.  Measured per K block of 32 (two pieces, 3 MFMAs), operands from beyond the L2 as the launch before left them:
-// a tile alone on its CU, and the CU's time for one on a full chip (730, 720, 940, 1070, 1190, 1180 TFLOP/s of MFMAs at best).
-// 512 x 512 x 512: 4.0, 6.1, 7.5, 11.3, 12.5, 30 us; 1024 x 1024 x 1024: 17.8, 10.4, 12.8, 20, 23, 57 us; 2048 x 4096 x 2048: 225,
-// 141, 110, 90, 87, 125 us; 8192 x 8192 x 2048: 774 (128), 698 us (256).
+// a tile alone on its CU, and the CU's time for one on a full chip (730, 720, 940, 760, 1070, 1190, 1180 TFLOP/s of MFMAs at best).
+// 512 x 512 x 512: 4.0, 6.1, 7.5, -, 11.3, 12.5, 30 us; 1024 x 1024 x 1024: 17.8, 10.4, 12.8, -, 20, 23, 57 us; 2048 x 4096 x 2048: 225,
+// 141, 110, -, 90, 87, 125 us; 1536 x 1536 x 4096: -, 98, -, 63, 77 us; 8192 x 8192 x 2048: 774 (128), 698 us (256).
 typedef Tile<32, 32, 1, 1, 3, 4> Orth32;
 typedef Tile<64, 64, 2, 2, 3, 2> Orth64K;      // 96 KiB: one a CU, for launches of no more tiles than CUs; three stages cover the latency
 typedef Tile<64, 64, 2, 2, 2, 2> Orth64;
+typedef Tile<96, 96, 1, 3, 2, 3> Orth96K;      // one a CU again: the triangle of 2048 is 253 of these, and 136 of 128
 typedef Tile<128, 128, 2, 2, 2, 2> Orth128K;   // one a CU again
 typedef Tile<128, 128, 2, 2, 2> Orth128;
 typedef Tile<256, 256, 2, 4, 2> Orth256;
-constexpr int KINDS = 6, SIDE[KINDS] = {32, 64, 64, 128, 128, 256};
-constexpr double ALONE[KINDS] = {0.095, 0.27, 0.33, 0.60, 0.67, 1.9}, FULL[KINDS] = {0.11, 0.28, 0.215, 0.75, 0.68, 2.73};
+constexpr int KINDS = 7, SIDE[KINDS] = {32, 64, 64, 96, 128, 128, 256};
+constexpr double ALONE[KINDS] = {0.095, 0.27, 0.33, 0.47, 0.60, 0.67, 1.9}, FULL[KINDS] = {0.11, 0.28, 0.215, 0.60, 0.75, 0.68, 2.73};
 // The epilogue moves 12 bytes an entry at a CU's share of the memory and hardly overlaps with products (all tiles of a launch
 // take the same time); what a tile costs besides.
-constexpr double EPILOGUE = 12 / 15e3, FIXED[KINDS] = {1.5, 0.8, 0.8, 0.8, 0.8, 0.8};
+constexpr double EPILOGUE = 12 / 15e3, FIXED[KINDS] = {1.5, 0.8, 0.8, 0.8, 0.8, 0.8, 0.8};
 
 int64_t tiles_of(const Parts& p, int stage, int side) {
   const int64_t tm = (p.mp + side - 1) / side, tn = (p.np + side - 1) / side;
@@ -580,16 +581,15 @@ Plan plan_of(const int64_t* shapes, int count) {
         const double kb = (double)(s == GRAM ? p.np : p.mp) / 32;
         const int64_t t = tiles_of(p, s, SIDE[k]);
         tiles[s][k] += t;
-        sum[s][k] += t * (kb * FULL[k] + SIDE[k] * SIDE[k] * EPILOGUE + FIXED[k]);
+        sum[s][k] += t * (kb * FULL[k] + FIXED[k]);
         longest[s][k] = std::fmax(longest[s][k], kb * ALONE[k]);
       }
   }
   const double cus = device_cus();
   for (int s = 0; s < 3; ++s) {
     for (int k = 0; k < KINDS; ++k) {
-      const double rounds = tiles[s][k] / cus;
-      const double us = tiles[s][k] > cus ? std::fmax(longest[s][k], sum[s][k] / cus * std::ceil(rounds) / rounds)
-                                          : longest[s][k] + rounds * SIDE[k] * SIDE[k] * EPILOGUE + FIXED[k];
+      const double rounds = tiles[s][k] / cus, all = rounds > 1 ? sum[s][k] / cus * std::ceil(rounds) / rounds : 0.0;
+      const double us = std::fmax(longest[s][k] + FIXED[k], all) + rounds * SIDE[k] * SIDE[k] * EPILOGUE;
       if (k == 0 || us < best[s]) {
         best[s] = us;
         plan.kind[s] = k;
@@ -613,8 +613,9 @@ int product_launch(int kind, const Table& t, const Numbers& num, int k, int64_t 
     case 0: return launch<Orth32, STAGE, T, MUON>(t, num, k, tiles, stream);
     case 1: return launch<Orth64K, STAGE, T, MUON>(t, num, k, tiles, stream);
     case 2: return launch<Orth64, STAGE, T, MUON>(t, num, k, tiles, stream);
-    case 3: return launch<Orth128K, STAGE, T, MUON>(t, num, k, tiles, stream);
-    case 4: return launch<Orth128, STAGE, T, MUON>(t, num, k, tiles, stream);
+    case 3: return launch<Orth96K, STAGE, T, MUON>(t, num, k, tiles, stream);
+    case 4: return launch<Orth128K, STAGE, T, MUON>(t, num, k, tiles, stream);
+    case 5: return launch<Orth128, STAGE, T, MUON>(t, num, k, tiles, stream);
     default: return launch<Orth256, STAGE, T, MUON>(t, num, k, tiles, stream);
   }
 }
