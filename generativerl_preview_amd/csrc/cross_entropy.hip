@@ -310,13 +310,14 @@ struct Finish {
   int reduction;
 };
 
-// Q threads a row: the partials of a row, then its loss.
+// The partials of a row, then its loss: Q threads a row.  8: rows along the lanes, as they lie in memory; 64: a wave a row, where rows
+// are few and partials many.
 template <int Q>
 __global__ __launch_bounds__(256) void k_ce_finish(Finish a) {
   constexpr int R = 256 / Q;
-  __shared__ float tops[Q][R], sums[Q][R];
+  __shared__ float tops[8][32], sums[8][32];
   __shared__ double s[R], c[R];
-  const int r = threadIdx.x % R, q = threadIdx.x / R, n = blockIdx.x * R + r;
+  const int r = Q == 64 ? threadIdx.x / 64 : threadIdx.x % R, q = Q == 64 ? threadIdx.x % 64 : threadIdx.x / R, n = blockIdx.x * R + r;
   float top = -INFINITY, sum = 0.f;
   auto add = [&](float t, float u) {
     const float most = fmaxf(top, t);
@@ -329,11 +330,20 @@ __global__ __launch_bounds__(256) void k_ce_finish(Finish a) {
       const float2 p = a.part[(int64_t)t * a.rows + n];
       add(p.x, p.y);
     }
-  tops[q][r] = top;
-  sums[q][r] = sum;
-  __syncthreads();
+  if (Q == 64) {
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) {
+      const float t = __shfl_xor(top, d), u = __shfl_xor(sum, d);
+      add(t, u);
+    }
+  } else {
+    tops[q][r] = top;
+    sums[q][r] = sum;
+    __syncthreads();
+    if (q == 0)
+      for (int k = 1; k < Q; ++k) add(tops[k][r], sums[k][r]);
+  }
   if (q == 0) {
-    for (int k = 1; k < Q; ++k) add(tops[k][r], sums[k][r]);
     s[r] = c[r] = 0.0;
     if (n < a.rows) {
       const int64_t t = a.target[n];
@@ -349,8 +359,9 @@ __global__ __launch_bounds__(256) void k_ce_finish(Finish a) {
       c[r] = kept ? 1.0 : 0.0;
     }
   }
+  if (!a.sums) return;
   __syncthreads();
-  if (threadIdx.x == 0 && a.sums) {
+  if (threadIdx.x == 0) {
     double x = 0.0, y = 0.0;
     for (int k = 0; k < R; ++k) { x += s[k]; y += c[k]; }
     a.sums[2 * blockIdx.x] = x;

@@ -98,15 +98,31 @@ __device__ __forceinline__ Walk walk(bool along_n) {
   return along_n ? Walk{t >> 6, t & 63, 4, 0} : Walk{t & 63, t >> 6, 0, 4};
 }
 
-// buf = momentum buf + (1 - momentum) g and the direction u; or u = g.  WRITE: store buf.
-template <class T, bool MUON, bool WRITE>
-__device__ __forceinline__ float direction(const Numbers& g, const Mat& a, int64_t i, int64_t j) {
-  const float x = load((const T*)a.g + i * a.gs[0] + j * a.gs[1]);
-  if (!MUON) return x;
-  float* b = a.buf + i * a.bs[0] + j * a.bs[1];
-  float v = *b;
-  if (WRITE) { v = g.momentum * v + g.fresh * x; *b = v; }
-  return g.nesterov ? g.fresh * x + g.momentum * v : v;
+// buf = momentum buf + (1 - momentum) g and the direction u, or u = g, of N entries of a thread (entry e at (r[e], c[e]); outside the matrix:
+// 0).  FIRST: the pass that updates buf; later ones find it updated.  All loads come before the first store, which may
+// alias them as far as the compiler knows: one trip to memory, not N.
+template <class T, bool MUON, bool FIRST, int N, class F>
+__device__ __forceinline__ void directions(const Numbers& g, const Mat& a, F&& place, float (&u)[N]) {
+  float v[MUON ? N : 1];
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    int r, c;
+    const bool in = place(e, r, c);
+    u[e] = in ? load((const T*)a.g + r * a.gs[0] + c * a.gs[1]) : 0.f;
+    if (MUON) v[MUON ? e : 0] = in ? a.buf[r * a.bs[0] + c * a.bs[1]] : 0.f;
+  }
+  if (!MUON) return;
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    int r, c;
+    const bool in = place(e, r, c);
+    float& b = v[MUON ? e : 0];
+    if (FIRST) {
+      b = g.momentum * b + g.fresh * u[e];
+      if (in) a.buf[r * a.bs[0] + c * a.bs[1]] = b;
+    }
+    u[e] = g.nesterov ? g.fresh * u[e] + g.momentum * b : b;
+  }
 }
 
 // Sum over the block, in one order; every thread gets it.
@@ -136,21 +152,18 @@ __global__ __launch_bounds__(256) void k_orth_norm(Group g) {
       for (int f = 0; f < 4; ++f) g.first[f * g.all + g.from + k] = g.mat[k].first[f];
     }
   const int id = blockIdx.x + g.blocks0;
-  int e = 0;
-  while (e + 1 < g.count && g.mat[e + 1].first[0] <= id) ++e;
+  // the last matrix that starts at or before this block: a lane looks at each
+  const int lane = threadIdx.x & 63;
+  const int e = __builtin_amdgcn_readfirstlane(__popcll(__ballot(lane < g.count && g.mat[lane < GROUP ? lane : 0].first[0] <= id)) - 1);
   const Mat& a = g.mat[e];
   const int nb = (int)(up64(a.n) / 64), b = id - a.first[0];
   const int i0 = b / nb * 64, j0 = b % nb * 64;
   const Walk w = walk(a.gs[1] <= a.gs[0]);
+  float u[16];
+  directions<T, MUON, true>(g.num, a, [&](int k, int& i, int& j) { i = i0 + w.i + k * w.di; j = j0 + w.j + k * w.dj; return i < a.m && j < a.n; }, u);
   double s = 0.0;
-#pragma unroll 4
-  for (int k = 0; k < 16; ++k) {
-    const int i = i0 + w.i + k * w.di, j = j0 + w.j + k * w.dj;
-    if (i < a.m && j < a.n) {
-      const double u = direction<T, MUON, true>(g.num, a, i, j);
-      s += u * u;
-    }
-  }
+#pragma unroll
+  for (int k = 0; k < 16; ++k) s += (double)u[k] * u[k];
   __shared__ double sh[256];
   s = block_sum(s, sh);
   if (threadIdx.x == 0) g.part[id] = s;
@@ -164,16 +177,15 @@ __global__ __launch_bounds__(256) void k_orth_split(Table t, Numbers g) {
   const int nb = (int)((p.np + 63) / 64), b = blockIdx.x - a.first[0], all = p.blocks();
   __shared__ double sh[256];
   __shared__ float tile[64][65];
+  const int i0 = b / nb * 64, j0 = b % nb * 64;
+  const Walk w = walk(a.gs[1] <= a.gs[0]);
+  float u[16];
+  directions<T, MUON, false>(g, a, [&](int k, int& i, int& j) { i = i0 + w.i + k * w.di; j = j0 + w.j + k * w.dj; return i < a.m && j < a.n; }, u);
   double s = 0.0;
   for (int k = threadIdx.x; k < all; k += 256) s += t.part[a.first[0] + k];
   const double inv = factor_of(block_sum(s, sh), g.eps);
-  const int i0 = b / nb * 64, j0 = b % nb * 64;
-  const Walk w = walk(a.gs[1] <= a.gs[0]);
-#pragma unroll 4
-  for (int k = 0; k < 16; ++k) {
-    const int i = w.i + k * w.di, j = w.j + k * w.dj;
-    tile[i][j] = i0 + i < a.m && j0 + j < a.n ? (float)(direction<T, MUON, false>(g, a, i0 + i, j0 + j) * inv) : 0.f;
-  }
+#pragma unroll
+  for (int k = 0; k < 16; ++k) tile[w.i + k * w.di][w.j + k * w.dj] = (float)(u[k] * inv);
   __syncthreads();
   // 8 threads write the 128 bytes of 32 entries of a row: 4 their high pieces, 4 the low ones; X, then X^T
   const int chunk = threadIdx.x & 7, low = chunk >> 2, c8 = (chunk & 3) * 8;
@@ -386,14 +398,8 @@ __global__ __launch_bounds__(SMALL_THREADS, 4) void k_orth_small(Group g, int st
   const int all = a.m * a.n;
   const Spread in{a.gs[1] <= a.gs[0], a}, to{a.os[1] <= a.os[0], a};
   float u[PER];
+  directions<T, MUON, true>(g.num, a, [&](int e, int& r, int& c) { const int k = threadIdx.x + e * SMALL_THREADS; in.at(k, r, c); return k < all; }, u);
   double s = 0.0;
-#pragma unroll
-  for (int e = 0; e < PER; ++e) {
-    const int k = threadIdx.x + e * SMALL_THREADS;
-    int r, c;
-    in.at(k, r, c);
-    u[e] = k < all ? direction<T, MUON, true>(g.num, a, r, c) : 0.f;
-  }
 #pragma unroll
   for (int e = 0; e < PER; ++e) s += (double)u[e] * u[e];
   for (int k = threadIdx.x; k < (SMALL_X + SMALL_XT) / 16; k += SMALL_THREADS) ((u32x4*)lds)[k] = u32x4{0, 0, 0, 0};   // the padding stays zero
@@ -560,7 +566,7 @@ constexpr int KINDS = 7, SIDE[KINDS] = {32, 64, 64, 96, 128, 128, 256};
 constexpr double ALONE[KINDS] = {0.095, 0.27, 0.33, 0.47, 0.60, 0.67, 1.9}, FULL[KINDS] = {0.11, 0.28, 0.215, 0.60, 0.75, 0.68, 2.73};
 // The epilogue moves 12 bytes an entry at a CU's share of the memory and hardly overlaps with products (all tiles of a launch
 // take the same time); what a tile costs besides.
-constexpr double EPILOGUE = 12 / 15e3, FIXED[KINDS] = {1.5, 0.8, 0.8, 0.8, 0.8, 0.8, 0.8};
+constexpr double EPILOGUE = 12 / 15e3, FIXED[KINDS] = {2.5, 0.8, 0.8, 0.8, 0.8, 0.8, 0.8};
 
 int64_t tiles_of(const Parts& p, int stage, int side) {
   const int64_t tm = (p.mp + side - 1) / side, tn = (p.np + side - 1) / side;

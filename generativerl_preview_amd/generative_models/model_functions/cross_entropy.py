@@ -6,10 +6,13 @@ import ctypes
 import torch
 
 from ... import _lib as L
-from ...engine import _ptr, _stream
 
 _ELEM = {torch.float32: L.ELEM_F32, torch.bfloat16: L.ELEM_BF16, torch.float16: L.ELEM_F16}
 _REDUCE = {"none": L.REDUCE_NONE, "mean": L.REDUCE_MEAN, "sum": L.REDUCE_SUM}
+
+
+def _address(t):
+    return None if t is None else t.data_ptr()
 
 
 def _strides(t):
@@ -20,45 +23,44 @@ class _Head:
     """The arguments that the forward and the backward call share."""
 
     def __init__(self, hidden, weight, bias, target, row_weight, ignore_index, reduction):
-        self.hidden, self.weight, self.target, self.row_weight = hidden, weight, target, row_weight
-        self.bias = None if bias is None else bias.float().contiguous()
-        self.rows, self.features, self.vocab = hidden.shape[0], hidden.shape[1], weight.shape[0]
-        self.elem, self.reduction, self.ignore_index = _ELEM[hidden.dtype], reduction, ignore_index
-        self.operands = (_ptr(hidden), _strides(hidden), _ptr(weight), _strides(weight))
+        self.device, self.dtype, self.reduction = hidden.device, hidden.dtype, reduction
+        bias = None if bias is None else bias.float().contiguous()
+        self.kept = hidden, weight, bias, target, row_weight     # alive until the launches are queued
+        (rows, features), vocab = hidden.shape, weight.shape[0]
+        self.shape = rows, features, vocab
+        self.operands = hidden.data_ptr(), _strides(hidden), weight.data_ptr(), _strides(weight)
+        self.sizes = rows, features, vocab, _ELEM[hidden.dtype]
+        self.arguments = (*self.operands, _address(bias), target.data_ptr(), ignore_index, _address(row_weight), *self.sizes, reduction)
 
-    def sizes(self):
-        return self.rows, self.features, self.vocab, self.elem
-
-    def workspace(self, backward):
-        need = L.lib().grlhip_linear_ce_workspace_bytes(*self.operands, *self.sizes(), int(backward))
+    def call(self, name, backward, *rest):
+        lib = L.lib()
+        need = lib.grlhip_linear_ce_workspace_bytes(*self.operands, *self.sizes, backward)
         if need == 0:
-            raise L.GrlHipError(L.lib().grlhip_last_error().decode())
-        # one per call: calls on different streams and captured graphs must not share it
-        return torch.empty(need, dtype=torch.uint8, device=self.hidden.device)
-
-    def call(self, fn, ws, *rest):
-        dev = self.hidden.device
-        with torch.cuda.device(dev):
-            L.check(fn(*self.operands, _ptr(self.bias), _ptr(self.target), self.ignore_index, _ptr(self.row_weight),
-                       *self.sizes(), self.reduction, *rest, _ptr(ws), ws.numel(), _stream(dev)))
+            raise L.GrlHipError(lib.grlhip_last_error().decode())
+        # one workspace per call: calls on different streams and captured graphs must not share it
+        with torch.cuda.device(self.device):
+            ws = torch.empty(need, dtype=torch.uint8, device=self.device)
+            stream = torch.cuda.current_stream(self.device).cuda_stream
+            L.check(getattr(lib, name)(*self.arguments, *rest, ws.data_ptr(), need, stream))
 
     def forward(self):
         """(losses, logsumexp, reduced loss, number of rows that are not ignored)"""
-        dev = self.hidden.device
-        losses, lse = (torch.empty(self.rows, dtype=torch.float32, device=dev) for _ in range(2))
+        rows, dev = self.shape[0], self.device
+        losses, lse = torch.empty(rows, dtype=torch.float32, device=dev), torch.empty(rows, dtype=torch.float32, device=dev)
         total = count = None
         if self.reduction != L.REDUCE_NONE:
-            total, count = (torch.empty((), dtype=torch.float32, device=dev) for _ in range(2))
-        self.call(L.lib().grlhip_linear_ce_forward, self.workspace(False), _ptr(losses), _ptr(lse), _ptr(total), _ptr(count))
+            total, count = torch.empty((), dtype=torch.float32, device=dev), torch.empty((), dtype=torch.float32, device=dev)
+        self.call("grlhip_linear_ce_forward", 0, losses.data_ptr(), lse.data_ptr(), _address(total), _address(count))
         return losses, lse, total, count
 
     def backward(self, lse, count, grad, need_hidden, need_weight, need_bias):
-        new = lambda need, *shape, dtype: torch.empty(*shape, dtype=dtype, device=self.hidden.device) if need else None  # noqa: E731
-        gh = new(need_hidden, self.rows, self.features, dtype=self.hidden.dtype)
-        gw = new(need_weight, self.vocab, self.features, dtype=self.hidden.dtype)
-        gb = new(need_bias, self.vocab, dtype=torch.float32)
-        self.call(L.lib().grlhip_linear_ce_backward, self.workspace(True), _ptr(lse), _ptr(count), _ptr(grad),
-                  0 if grad.dim() == 0 else grad.stride(0), _ptr(gh), _ptr(gw), _ptr(gb))
+        rows, features, vocab = self.shape
+        dev = self.device
+        gh = torch.empty(rows, features, dtype=self.dtype, device=dev) if need_hidden else None
+        gw = torch.empty(vocab, features, dtype=self.dtype, device=dev) if need_weight else None
+        gb = torch.empty(vocab, dtype=torch.float32, device=dev) if need_bias else None
+        self.call("grlhip_linear_ce_backward", 1, lse.data_ptr(), _address(count), grad.data_ptr(),
+                  0 if grad.dim() == 0 else grad.stride(0), _address(gh), _address(gw), _address(gb))
         return gh, gw, gb
 
 
@@ -117,12 +119,13 @@ def linear_cross_entropy(hidden, weight, target, bias=None, row_weight=None, ign
             raise ValueError("row_weight: expected shape %s, got %s" % (tuple(target.shape), tuple(row_weight.shape)))
         if row_weight.requires_grad:
             raise ValueError("row_weight: no gradient is taken to the weights of rows; detach them")
-    for name, t in (("hidden", hidden), ("weight", weight), ("target", target), ("bias", bias), ("row_weight", row_weight)):
-        if t is not None and not t.is_cuda:
-            raise L.GrlHipError("%s must live on a HIP device (got %s): there is no CPU fallback" % (name, t.device))
-        if t is not None and t.device != hidden.device:
-            raise ValueError("%s is on %s, hidden on %s" % (name, t.device, hidden.device))
-    rows = hidden.reshape(-1, hidden.shape[-1])
+    dev = hidden.device
+    if dev.type != "cuda":
+        raise L.GrlHipError("hidden must live on a HIP device (got %s): there is no CPU fallback" % dev)
+    for name, t in (("weight", weight), ("target", target), ("bias", bias), ("row_weight", row_weight)):
+        if t is not None and t.device != dev:
+            raise ValueError("%s is on %s, hidden on %s" % (name, t.device, dev))
+    rows = hidden if hidden.dim() == 2 else hidden.reshape(-1, hidden.shape[-1])
     flat = target.reshape(-1).long().contiguous()
     if row_weight is not None:
         row_weight = row_weight.reshape(-1).float().contiguous()

@@ -117,39 +117,44 @@ class FlatAdam:
         self.param_groups[0].update(sd["param_groups"][0])
 
 
-def _matrices(tensors, name, shapes=None, written=False):
-    """Checks a list of 2-D tensors on one HIP device; returns their shapes."""
-    dev = tensors[0].device
-    seen = set()
+def _matrices(tensors, name, like=None):
+    """Checks a list of matrices on one HIP device (that of `like`, with its shapes); returns their addresses and whether all
+    are dense."""
+    first = tensors[0] if like is None else like[0]
+    dev, dtype, dense = first.device, tensors[0].dtype, True
+    if dev.type != "cuda":
+        raise L.GrlHipError("%s must live on a HIP device (got %s): there is no CPU fallback" % (name, dev))
     for i, t in enumerate(tensors):
-        if not t.is_cuda:
-            raise L.GrlHipError("%s[%d] must live on a HIP device (got %s): there is no CPU fallback" % (name, i, t.device))
-        if t.device != dev or t.dtype != tensors[0].dtype:
+        if t.device != dev or t.dtype != dtype:
             raise ValueError("%s[%d]: all matrices must be on one device and of one type (%s %s, got %s %s)" %
-                             (name, i, dev, tensors[0].dtype, t.device, t.dtype))
-        if t.dim() != 2:
-            raise ValueError("%s[%d]: expected a matrix, got shape %s" % (name, i, tuple(t.shape)))
-        if shapes is not None and t.shape != shapes[i]:
-            raise ValueError("%s[%d]: expected shape %s, got %s" % (name, i, tuple(shapes[i]), tuple(t.shape)))
-        if written and t.numel():
-            if t.data_ptr() in seen or any(st == 0 and n > 1 for st, n in zip(t.stride(), t.shape)):
-                raise ValueError("%s[%d] is written to and must not share memory with itself or another of them" % (name, i))
-            seen.add(t.data_ptr())
-    return [t.shape for t in tensors]
+                             (name, i, dev, dtype, t.device, t.dtype))
+        if t.dim() != 2 or (like is not None and t.shape != like[i].shape):
+            raise ValueError("%s[%d]: expected %s, got shape %s" %
+                             (name, i, "a matrix" if like is None else "shape %s" % (tuple(like[i].shape),), tuple(t.shape)))
+        dense = dense and t.is_contiguous()
+    return [t.data_ptr() if t.numel() else 0 for t in tensors], dense
 
 
-def _pointers(tensors):
-    return (ctypes.c_void_p * len(tensors))(*[t.data_ptr() for t in tensors])
+def _written(tensors, pointers, dense, name):
+    """What is written must not overlap itself; the addresses of its matrices, without the empty ones'."""
+    if not dense and any(st == 0 and n > 1 for t in tensors for st, n in zip(t.stride(), t.shape)):
+        raise ValueError("%s: a matrix that is written to must not share memory with itself" % name)
+    seen = {p for p in pointers if p}
+    if len(seen) != sum(1 for p in pointers if p):
+        raise ValueError("%s: the matrices are written to and must not share memory" % name)
+    return seen
 
 
-def _shape_array(shapes):
-    return (ctypes.c_int64 * (2 * len(shapes)))(*[n for s in shapes for n in s])
+def _pointers(addresses):
+    return (ctypes.c_void_p * len(addresses))(*addresses)
+
+
+def _shape_array(tensors):
+    return (ctypes.c_int64 * (2 * len(tensors)))(*[n for t in tensors for n in t.shape])
 
 
 def _stride_array(*lists):
-    """[count][6] element strides of up to three lists of matrices, or None when all are dense."""
-    if all(t.is_contiguous() for ts in lists for t in ts):
-        return None
+    """[count][6] element strides of up to three lists of matrices."""
     lists = lists + (lists[0],) * (3 - len(lists))
     return (ctypes.c_int64 * (6 * len(lists[0])))(*[v for ts in zip(*lists) for t in ts for v in t.stride()])
 
@@ -184,14 +189,15 @@ def orthogonalize(matrices, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7):
     src = [m for t in flat for m in (t.unbind(0) if t.dim() == 3 else (t,))]
     dst = [m for t in out for m in (t.unbind(0) if t.dim() == 3 else (t,))]
     if src:
-        shapes = _shape_array(_matrices(src, "matrices"))
+        pointers, dense = _matrices(src, "matrices")
+        shapes = _shape_array(src)
         dev = src[0].device
-        a, b, c = (float(v) for v in coefficients)
+        a, b, c = coefficients
         ws = _newton_schulz_workspace(shapes, len(src), dev)
         with torch.cuda.device(dev):
-            L.check(L.lib().grlhip_orthogonalize(_pointers(src), _pointers(dst), shapes, _stride_array(src, dst), len(src),
-                                                 _ELEM[src[0].dtype], int(steps), a, b, c, float(eps), _ptr(ws), ws.numel(),
-                                                 _stream(dev)))
+            L.check(L.lib().grlhip_orthogonalize(_pointers(pointers), _pointers([t.data_ptr() for t in dst]), shapes,
+                                                 None if dense else _stride_array(src, dst), len(src), _ELEM[src[0].dtype],
+                                                 int(steps), a, b, c, eps, _ptr(ws), ws.numel(), _stream(dev)))
     out = [o.view(t.shape) for o, t in zip(out, tensors)]
     return out[0] if single else out
 
@@ -214,28 +220,25 @@ def muon_step(params, grads, momentum_buffers, lr, momentum=0.95, nesterov=True,
         raise ValueError("adjust_lr: expected 'original' or 'match_rms_adamw', got %r" % (adjust_lr,))
     if not params:
         return
-    shapes = _matrices(params, "params", written=True)
-    _matrices(grads, "grads", shapes)
-    _matrices(bufs, "momentum_buffers", shapes, written=True)
-    dev = params[0].device
+    (pp, pd), (gp, gd), (bp, bd) = _matrices(params, "params"), _matrices(grads, "grads", params), _matrices(bufs, "momentum_buffers", params)
     for name, ts in (("params", params), ("grads", grads), ("momentum_buffers", bufs)):
         if ts[0].dtype != torch.float32:
             raise TypeError("%s: expected float32, got %s" % (name, ts[0].dtype))
-        if ts[0].device != dev:
-            raise ValueError("%s are on %s, the parameters on %s" % (name, ts[0].device, dev))
-    if {t.data_ptr() for t in bufs if t.numel()} & {t.data_ptr() for ts in (params, grads) for t in ts if t.numel()} \
-            or {t.data_ptr() for t in params if t.numel()} & {t.data_ptr() for t in grads if t.numel()}:
+    ps, bs = _written(params, pp, pd, "params"), _written(bufs, bp, bd, "momentum_buffers")
+    if not bs.isdisjoint(ps) or not bs.isdisjoint(gp) or not ps.isdisjoint(gp):
         raise ValueError("muon_step: parameters, gradients and momentum buffers must not share memory")
-    rates = (ctypes.c_float * len(params))(*[
-        lr * (math.sqrt(max(1.0, r / max(c, 1))) if adjust_lr == "original" else 0.2 * math.sqrt(max(r, c))) for r, c in shapes])
-    shape_arr = _shape_array(shapes)
-    a, b, c = (float(v) for v in coefficients)
-    ws = _newton_schulz_workspace(shape_arr, len(params), dev)
+    sides = [t.shape for t in params]
+    rates = (ctypes.c_float * len(params))(*(
+        [lr * math.sqrt(max(1.0, r / max(c, 1))) for r, c in sides] if adjust_lr == "original" else
+        [lr * 0.2 * math.sqrt(max(r, c)) for r, c in sides]))
+    shapes, dev = _shape_array(params), params[0].device
+    a, b, c = coefficients
+    ws = _newton_schulz_workspace(shapes, len(params), dev)
     with torch.cuda.device(dev):
-        L.check(L.lib().grlhip_muon_step(_pointers(params), _pointers(grads), _pointers(bufs), shape_arr,
-                                         _stride_array(grads, params, bufs), rates, len(params), float(momentum),
-                                         int(nesterov), float(1.0 - lr * weight_decay), int(steps), a, b, c, float(eps),
-                                         _ptr(ws), ws.numel(), _stream(dev)))
+        L.check(L.lib().grlhip_muon_step(_pointers(pp), _pointers(gp), _pointers(bp), shapes,
+                                         None if pd and gd and bd else _stride_array(grads, params, bufs), rates, len(params),
+                                         momentum, int(nesterov), 1.0 - lr * weight_decay, int(steps), a, b, c, eps, _ptr(ws),
+                                         ws.numel(), _stream(dev)))
 
 
 class FlatMuon(FlatAdam):
