@@ -2,6 +2,7 @@
 discretised actions (behaviour cloning, or advantage-weighted with ``row_weight``), beside the fused losses of the continuous
 models.  ``grlhip_linear_ce_forward`` / ``grlhip_linear_ce_backward``."""
 import ctypes
+import weakref
 
 import torch
 
@@ -64,9 +65,38 @@ class _Head:
         return gh, gw, gb
 
 
+class _Graph:
+    """Lives as long as the autograd graph of one eager loss; `leaves`: the tensors it ends in."""
+    __slots__ = ("leaves", "__weakref__")
+
+    def __init__(self, leaves):
+        self.leaves = leaves
+
+
+_ON_DEFAULT_STREAM = weakref.WeakSet()
+
+
+def _watch(ctx, *tensors):
+    """autograd adds up a leaf's gradient on the stream where the leaf first entered a live graph.  If that is the default
+    stream, a backward pass under capture reaches for a stream that cannot be captured, and the process ends: such a
+    call is refused while it is still a call."""
+    leaves = [t for t in tensors if t is not None and t.requires_grad and t.is_leaf]
+    if not leaves:
+        return
+    if torch.cuda.is_current_stream_capturing():
+        for graph in list(_ON_DEFAULT_STREAM):
+            if any(t is u for t in leaves for u in graph.leaves):
+                raise L.GrlHipError("linear_cross_entropy under graph capture: an eager loss of the same leaves, computed on the "
+                                    "default stream, is still alive; drop it (del loss) before the capture")
+    elif torch.cuda.current_stream(leaves[0].device).cuda_stream == 0:
+        ctx.graph = _Graph(leaves)
+        _ON_DEFAULT_STREAM.add(ctx.graph)
+
+
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, bias, target, row_weight, ignore_index, reduction):
+        _watch(ctx, hidden, weight, bias)
         head = _Head(hidden, weight, bias, target, row_weight, ignore_index, reduction)
         losses, lse, total, count = head.forward()
         ctx.save_for_backward(hidden, weight, bias, target, row_weight, lse, count)
@@ -95,7 +125,7 @@ def linear_cross_entropy(hidden, weight, target, bias=None, row_weight=None, ign
     Differentiable (once) with respect to hidden, weight and bias; the gradients have the operands' types.  Logits are never stored:
     the forward pass keeps one logsumexp per row, the backward pass recomputes them in pieces of the vocabulary.  With
     ``reduction="none"`` and no gradient this is the negative log-probability of single tokens (serving).  While a HIP graph is
-    captured, no eager autograd graph over the same leaves may be alive (drop the earlier losses first)."""
+    captured, no eager loss over the same leaves from the default stream may be alive: such a call is refused."""
     if reduction not in _REDUCE:
         raise ValueError("reduction: expected 'none', 'mean' or 'sum', got %r" % (reduction,))
     if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1]:

@@ -327,6 +327,30 @@ def test_gpu_captured_step_replays():
 
 
 @pytest.mark.gpu
+def test_gpu_capture_beside_a_live_eager_loss_is_refused(monkeypatch):
+    """autograd would add up the leaves' gradients on the default stream, which cannot be captured."""
+    h, w, t, _, _ = inputs(20, 64, 50, F32)
+    w.requires_grad_()
+    loss = linear_cross_entropy(h, w, t)
+    other = w.detach().clone().requires_grad_()
+    side = torch.cuda.Stream(device=DEV)
+    with torch.cuda.stream(side):
+        elsewhere = linear_cross_entropy(h, other, t)
+    with monkeypatch.context() as m:      # as it looks from inside a capture; nothing is captured here
+        m.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+        with pytest.raises(L.GrlHipError, match="still alive"):
+            linear_cross_entropy(h, w, t)
+        linear_cross_entropy(h, other, t).backward()       # the live loss of another stream
+        linear_cross_entropy(h, w.detach(), t)             # no gradient, no graph
+        (2 * linear_cross_entropy(h, w * 1.0, t)).detach()    # w is no leaf of this call
+        loss.backward()
+        del loss
+        linear_cross_entropy(h, w, t).backward()
+    torch.cuda.synchronize()
+    assert elsewhere.requires_grad
+
+
+@pytest.mark.gpu
 def test_gpu_a_head_over_a_network_trains_with_flat_muon():
     """The operators together: features of a HIP network, the head's loss over discretised actions with advantage weights,
     gradients through both, a FlatMuon step of the network and a muon_step of the head."""
