@@ -83,9 +83,9 @@ PROTOTYPES = {
                                         _vp, _sz, _vp]),
     "grlhip_linear_ce_workspace_bytes": (_sz, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, ctypes.c_int, ctypes.c_int]),
     "grlhip_linear_ce_forward": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _i64, _i64, ctypes.c_int,
-                                                ctypes.c_int, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+                                                ctypes.c_int, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "grlhip_linear_ce_backward": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _i64, _i64, ctypes.c_int,
-                                                 ctypes.c_int, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _sz, _vp]),
+                                                 ctypes.c_int, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _sz, _vp]),
     "grlhip_cep_loss_fwd_bwd": (ctypes.c_int, [_vp, _vp, ctypes.c_int, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _vp,
                                                _i64, _vp, _sz, _vp]),
 }

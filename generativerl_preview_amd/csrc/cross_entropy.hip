@@ -134,7 +134,7 @@ __device__ __forceinline__ void pack_rows(E* out, int64_t cols, int r0, int rows
   }
 }
 template <class T>
-__global__ __launch_bounds__(256) void k_ce_pack(Job h, Job w, Scale g, Scalars* s) {
+__global__ __launch_bounds__(256) void k_ce_pack(Job h, Job w, Scale g, Scalars* s, float* largest, bool known) {
   constexpr bool TWO = sizeof(T) == 4, SCALED = !__is_same(T, _Float16);
   __shared__ float tile[64][65], sh[4];
   if ((int)blockIdx.x >= h.blocks + w.blocks) {
@@ -162,9 +162,14 @@ __global__ __launch_bounds__(256) void k_ce_pack(Job h, Job w, Scale g, Scalars*
   const int b = is_h ? blockIdx.x : blockIdx.x - h.blocks;
   float f = 1.f;
   if (SCALED) {
-    const float most = is_h ? block_max(threadIdx.x < HMAX ? s->hpart[threadIdx.x] : 0.f, sh) : block_max(s->wpart[threadIdx.x], sh);
+    float most;
+    if (known) most = largest[is_h ? 0 : 1];   // the forward call's
+    else most = is_h ? block_max(threadIdx.x < HMAX ? s->hpart[threadIdx.x] : 0.f, sh) : block_max(s->wpart[threadIdx.x], sh);
     f = scale_of(most);
-    if (b == 0 && threadIdx.x == 0) (is_h ? s->h : s->w) = most;
+    if (b == 0 && threadIdx.x == 0) {
+      (is_h ? s->h : s->w) = most;
+      if (largest && !known) largest[is_h ? 0 : 1] = most;
+    }
   }
   const int across = (a.v.cols + 63) / 64, i0 = b / across * 64, j0 = b % across * 64, tid = threadIdx.x;
   const bool along = a.v.s1 <= a.v.s0;
@@ -706,7 +711,7 @@ struct Call {
   const void* w; int64_t w0, w1;
   const float* bias; const int64_t* target; const float* row_weight;
   int64_t ignore; int reduction;
-  float* losses; float* lse; float* total; float* count;
+  float* losses; float* lse; float* total; float* count; float* largest;
   const float* grad; int64_t grad_stride;
   void* gh; void* gw; float* gb;
   char* ws; size_t ws_bytes; hipStream_t stream;
@@ -739,12 +744,12 @@ void absmax_launch(const Call& a, Scalars* s) {
 }
 // Packs hidden (h null: not in this launch) and a weight piece, and takes the rows' gradients.
 template <class T>
-void pack_launch(const Call& a, Job h, Job w, Scale g, Scalars* s) {
+void pack_launch(const Call& a, Job h, Job w, Scale g, Scalars* s, bool known) {
   auto blocks = [](Job& j) { j.blocks = j.n || j.t ? (int)(up(j.v.cols, 64) / 64 * (up(j.v.rows, 64) / 64)) : 0; };
   blocks(h);
   blocks(w);
   const int all = h.blocks + w.blocks + g.blocks;
-  if (all > 0) hipLaunchKernelGGL(k_ce_pack<T>, dim3(all), dim3(256), 0, a.stream, h, w, g, s);
+  if (all > 0) hipLaunchKernelGGL(k_ce_pack<T>, dim3(all), dim3(256), 0, a.stream, h, w, g, s, a.largest, known);
 }
 
 template <class K, class... A>
@@ -807,7 +812,7 @@ int forward(const Call& a) {
     const View w = weight_piece<T>(a, v0, a.c.vocab - v0 < l.piece ? a.c.vocab - v0 : l.piece);
     Job jh{hidden_of(a), v0 == 0 && l.pack_h ? a.ws + l.hp : nullptr, l.kp, nullptr, 0, false, 0};
     Job jw{w, l.pack_w ? a.ws + l.wp : nullptr, l.kp, nullptr, 0, false, 0};
-    pack_launch<T>(a, jh, jw, Scale{}, s);
+    pack_launch<T>(a, jh, jw, Scale{}, s, false);
     Logits g = logits_call<T>(a, l, w, v0, s);
     g.part = (float2*)(a.ws + l.part) + (int64_t)tiles * a.c.rows;
     g.picked = (float*)(a.ws + l.picked);
@@ -826,7 +831,8 @@ int backward(const Call& a) {
   const Layout l = layout_of(a.c, direct(a.h, a.h0, a.h1, a.c), direct(a.w, a.w0, a.w1, a.c), true, a.gb != nullptr);
   if (!a.ws || (int64_t)a.ws_bytes < l.bytes) return set_error(GRLHIP_ERR_WORKSPACE, "linear_ce_backward: workspace too small: need " + std::to_string(l.bytes));
   Scalars* s = (Scalars*)(a.ws + l.scalars);
-  if (!__is_same(T, _Float16)) absmax_launch<T>(a, s);
+  const bool known = P == 2 && a.largest;   // an fp32 forward call has them
+  if (!__is_same(T, _Float16) && !known) absmax_launch<T>(a, s);
   float* scale = (float*)(a.ws + l.scale);
   const int side = SIDE[l.kind_z];
   const int64_t tn = up(a.c.rows, side) / side;
@@ -839,7 +845,7 @@ int backward(const Call& a) {
     int64_t gblocks = (a.c.rows + 255) / 256;
     if (gblocks > GMAX) gblocks = GMAX;
     const Scale sc{a.grad, a.grad_stride, a.row_weight, a.count, a.target, a.ignore, (int)a.c.rows, (int)a.c.vocab, a.reduction, first ? (int)gblocks : 0, scale};
-    pack_launch<T>(a, jh, jw, sc, s);
+    pack_launch<T>(a, jh, jw, sc, s, known);
 
     Logits g = logits_call<T>(a, l, w, v0, s);
     g.lse = a.lse;
@@ -928,7 +934,7 @@ size_t grlhip_linear_ce_workspace_bytes(const void* hidden, const int64_t* hidde
 
 int grlhip_linear_ce_forward(const void* hidden, const int64_t* hidden_strides, const void* weight, const int64_t* weight_strides, const float* bias,
                              const int64_t* target, int64_t ignore_index, const float* row_weight, int64_t rows, int64_t features, int64_t vocab,
-                             int elem, int reduction, float* losses, float* lse, float* total, float* count, void* workspace, size_t workspace_bytes, void* stream) {
+                             int elem, int reduction, float* losses, float* lse, float* total, float* count, float* largest, void* workspace, size_t workspace_bytes, void* stream) {
   return guarded([&]() -> int {
     Call a = {};
     a.c = {rows, features, vocab, elem};
@@ -947,6 +953,7 @@ int grlhip_linear_ce_forward(const void* hidden, const int64_t* hidden_strides, 
     a.lse = lse;
     a.total = total;
     a.count = count;
+    a.largest = largest;
     a.ws = (char*)workspace;
     a.ws_bytes = workspace_bytes;
     a.stream = (hipStream_t)stream;
@@ -960,7 +967,7 @@ int grlhip_linear_ce_forward(const void* hidden, const int64_t* hidden_strides, 
 
 int grlhip_linear_ce_backward(const void* hidden, const int64_t* hidden_strides, const void* weight, const int64_t* weight_strides, const float* bias,
                               const int64_t* target, int64_t ignore_index, const float* row_weight, int64_t rows, int64_t features, int64_t vocab,
-                              int elem, int reduction, const float* lse, const float* count, const float* grad, int64_t grad_stride,
+                              int elem, int reduction, const float* lse, const float* count, const float* largest, const float* grad, int64_t grad_stride,
                               void* grad_hidden, void* grad_weight, float* grad_bias, void* workspace, size_t workspace_bytes, void* stream) {
   return guarded([&]() -> int {
     Call a = {};
@@ -978,6 +985,7 @@ int grlhip_linear_ce_backward(const void* hidden, const int64_t* hidden_strides,
     a.reduction = reduction;
     a.lse = const_cast<float*>(lse);
     a.count = const_cast<float*>(count);
+    a.largest = const_cast<float*>(largest);
     a.grad = grad;
     a.grad_stride = grad_stride;
     a.gh = grad_hidden;

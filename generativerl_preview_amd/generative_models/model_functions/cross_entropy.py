@@ -44,23 +44,26 @@ class _Head:
             stream = torch.cuda.current_stream(self.device).cuda_stream
             L.check(getattr(lib, name)(*self.arguments, *rest, ws.data_ptr(), need, stream))
 
-    def forward(self):
-        """(losses, logsumexp, reduced loss, number of rows that are not ignored)"""
+    def forward(self, train=False):
+        """(losses, logsumexp, reduced loss, [number of rows that are not ignored, largest magnitudes of the operands])"""
         rows, dev = self.shape[0], self.device
         losses, lse = torch.empty(rows, dtype=torch.float32, device=dev), torch.empty(rows, dtype=torch.float32, device=dev)
-        total = count = None
+        total, numbers, count = None, None, None
+        if train or self.reduction != L.REDUCE_NONE:
+            numbers = torch.empty(3, dtype=torch.float32, device=dev)
         if self.reduction != L.REDUCE_NONE:
-            total, count = torch.empty((), dtype=torch.float32, device=dev), torch.empty((), dtype=torch.float32, device=dev)
-        self.call("grlhip_linear_ce_forward", 0, losses.data_ptr(), lse.data_ptr(), _address(total), _address(count))
-        return losses, lse, total, count
+            total, count = torch.empty((), dtype=torch.float32, device=dev), numbers.data_ptr()
+        self.call("grlhip_linear_ce_forward", 0, losses.data_ptr(), lse.data_ptr(), _address(total), count,
+                  numbers.data_ptr() + 4 if train else None)
+        return losses, lse, total, numbers
 
-    def backward(self, lse, count, grad, need_hidden, need_weight, need_bias):
+    def backward(self, lse, numbers, grad, need_hidden, need_weight, need_bias):
         rows, features, vocab = self.shape
         dev = self.device
         gh = torch.empty(rows, features, dtype=self.dtype, device=dev) if need_hidden else None
         gw = torch.empty(vocab, features, dtype=self.dtype, device=dev) if need_weight else None
         gb = torch.empty(vocab, dtype=torch.float32, device=dev) if need_bias else None
-        self.call("grlhip_linear_ce_backward", 1, lse.data_ptr(), _address(count), grad.data_ptr(),
+        self.call("grlhip_linear_ce_backward", 1, lse.data_ptr(), numbers.data_ptr(), numbers.data_ptr() + 4, grad.data_ptr(),
                   0 if grad.dim() == 0 else grad.stride(0), _address(gh), _address(gw), _address(gb))
         return gh, gw, gb
 
@@ -98,17 +101,17 @@ class _LinearCrossEntropy(torch.autograd.Function):
     def forward(ctx, hidden, weight, bias, target, row_weight, ignore_index, reduction):
         _watch(ctx, hidden, weight, bias)
         head = _Head(hidden, weight, bias, target, row_weight, ignore_index, reduction)
-        losses, lse, total, count = head.forward()
-        ctx.save_for_backward(hidden, weight, bias, target, row_weight, lse, count)
+        losses, lse, total, numbers = head.forward(train=True)
+        ctx.save_for_backward(hidden, weight, bias, target, row_weight, lse, numbers)
         ctx.numbers = ignore_index, reduction
         return losses if reduction == L.REDUCE_NONE else total
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        hidden, weight, bias, target, row_weight, lse, count = ctx.saved_tensors
+        hidden, weight, bias, target, row_weight, lse, numbers = ctx.saved_tensors
         head = _Head(hidden, weight, bias, target, row_weight, *ctx.numbers)
-        gh, gw, gb = head.backward(lse, count, grad.float(), *ctx.needs_input_grad[:3])
+        gh, gw, gb = head.backward(lse, numbers, grad.float(), *ctx.needs_input_grad[:3])
         return gh, gw, None if gb is None else gb.to(bias.dtype), None, None, None, None
 
 

@@ -379,6 +379,8 @@ typedef enum { GRLHIP_REDUCE_NONE = 0, GRLHIP_REDUCE_MEAN = 1, GRLHIP_REDUCE_SUM
  *   losses[i] = row_weight[i] (logsumexp_v z[i][v] - z[i][target[i]]);   lse[i] = logsumexp_v z[i][v]
  *   *total = sum of the losses (GRLHIP_REDUCE_SUM, _NONE) or that over *count (_MEAN); *count = number of rows whose target is
  *   not ignore_index, at least 1.  Both may be NULL for GRLHIP_REDUCE_NONE.
+ *   largest[2] = largest finite magnitudes of hidden and weight, written for GRLHIP_ELEM_F32 only (the backward call may take
+ *   them instead of reading the operands once more); may be NULL.
  * hidden [rows][features], weight [vocab][features]: element type `elem`, element strides {row, column} in HOST arrays (NULL:
  * dense).  bias [vocab] fp32 or NULL; -inf masks an entry.  target [rows] int64; row_weight [rows] fp32 or NULL (1).
  * A row whose target is ignore_index or whose weight is 0 has loss 0 and contributes nothing, whatever its hidden row holds.  Any other
@@ -391,18 +393,18 @@ size_t grlhip_linear_ce_workspace_bytes(const void* hidden, const int64_t* hidde
 int grlhip_linear_ce_forward(const void* hidden, const int64_t* hidden_strides, const void* weight,
                              const int64_t* weight_strides, const float* bias, const int64_t* target, int64_t ignore_index,
                              const float* row_weight, int64_t rows, int64_t features, int64_t vocab, int elem, int reduction,
-                             float* losses, float* lse, float* total, float* count, void* workspace, size_t workspace_bytes,
-                             void* stream);
+                             float* losses, float* lse, float* total, float* count, float* largest, void* workspace,
+                             size_t workspace_bytes, void* stream);
 
-/* The gradients of it: `lse` and `count` as the forward call left them; `grad`: DEVICE, the gradient of each loss at stride
+/* The gradients of it: `lse`, `count` and (GRLHIP_ELEM_F32; may be NULL) `largest` as the forward call left them; `grad`: DEVICE, the gradient of each loss at stride
  * `grad_stride` (GRLHIP_REDUCE_NONE) or of the reduced loss (grad_stride 0).  grad_hidden [rows][features] and grad_weight
  * [vocab][features] (type `elem`, dense), grad_bias [vocab] (fp32) are overwritten; each may be NULL.  The logits are recomputed in
  * pieces of the vocabulary.  Workspace: grlhip_linear_ce_workspace_bytes (backward = 1). */
 int grlhip_linear_ce_backward(const void* hidden, const int64_t* hidden_strides, const void* weight,
                               const int64_t* weight_strides, const float* bias, const int64_t* target, int64_t ignore_index,
                               const float* row_weight, int64_t rows, int64_t features, int64_t vocab, int elem, int reduction,
-                              const float* lse, const float* count, const float* grad, int64_t grad_stride, void* grad_hidden,
-                              void* grad_weight, float* grad_bias, void* workspace, size_t workspace_bytes, void* stream);
+                              const float* lse, const float* count, const float* largest, const float* grad,
+                              int64_t grad_stride, void* grad_hidden, void* grad_weight, float* grad_bias, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -412,10 +412,10 @@ def test_c_entry_points_check_their_arguments_without_a_gpu():
     p = ctypes.c_void_p((ctypes.addressof(buf) + 255) // 256 * 256)
 
     def fwd(h=p, w=p, t=p, n=4, k=8, v=10, elem=L.ELEM_F32, red=L.REDUCE_MEAN, losses=p, lse=p, total=p, count=p, ws=p, bytes_=1):
-        return lib.grlhip_linear_ce_forward(h, None, w, None, None, t, -100, None, n, k, v, elem, red, losses, lse, total, count, ws, bytes_, None)
+        return lib.grlhip_linear_ce_forward(h, None, w, None, None, t, -100, None, n, k, v, elem, red, losses, lse, total, count, None, ws, bytes_, None)
 
     def bwd(h=p, w=p, t=p, n=4, red=L.REDUCE_MEAN, lse=p, count=p, grad=p, gh=p, ws=p, bytes_=1):
-        return lib.grlhip_linear_ce_backward(h, None, w, None, None, t, -100, None, n, 8, 10, L.ELEM_F32, red, lse, count, grad, 0, gh, None, None, ws, bytes_, None)
+        return lib.grlhip_linear_ce_backward(h, None, w, None, None, t, -100, None, n, 8, 10, L.ELEM_F32, red, lse, count, None, grad, 0, gh, None, None, ws, bytes_, None)
 
     assert fwd() == -4 and bwd() == -4 and b"workspace" in lib.grlhip_last_error()
     assert fwd(total=None, count=None) == -1 and fwd(total=None, count=None, red=L.REDUCE_NONE) == -4
