@@ -10,9 +10,9 @@
 //
 // Precision.  z: 16-bit operands are used as they are, fp32 ones as two fp16 pieces a value (gemm_core.hip.inc), scaled by a
 // power of two per tensor that brings the largest entry to 2^13..2^14: what is lost of a value is at most 2^-23 of it or 2^-39 of the
-// largest.  D lies in [-1, 1] and is held times 2^14 in fp16: one piece for 16-bit operands (off by 2^-11 at most, below the
-// gradients' own rounding; in bf16, 2^-8, it would be as large as that), two for fp32.  W^T and hidden^T beside it are fp16 for that: bf16
-// entries fit its 11 bits exactly, scaled as above.  All sums are fp32 or wider and taken in a fixed order: results repeat bit for bit.
+// largest.  D lies in [-1, 1] and is held times 2^14 in fp16: one piece for bf16 operands (off by 2^-11 at most, an eighth of the
+// gradients' own rounding; held in bf16 it would be off by as much as that), two for fp16 and fp32 (one would be off by as much as an fp16
+// gradient's own rounding).  W^T and hidden^T beside it are fp16 for that: bf16 entries fit its 11 bits exactly, scaled as above.  All sums are fp32 or wider and taken in a fixed order: results repeat bit for bit.
 #include <cmath>
 #include <string>
 
@@ -133,6 +133,8 @@ __device__ __forceinline__ void pack_rows(E* out, int64_t cols, int r0, int rows
       *(e8*)(out + (int64_t)(r0 + row) * (TWO ? 2 : 1) * cols + (TWO ? ((c0 + col) >> 5) * 64 + (chunk >> 2) * 32 + (chunk & 3) * 8 : c0 + col)) = x;
   }
 }
+// pieces of D and of what it is multiplied by; 3: two, of which the other factor needs one
+template <class T> struct GradPieces { static constexpr int P = __is_same(T, float) ? 2 : __is_same(T, _Float16) ? 3 : 1, N = P == 1 ? 1 : 2; };
 template <class T>
 __global__ __launch_bounds__(256) void k_ce_pack(Job h, Job w, Scale g, Scalars* s, float* largest, bool known) {
   constexpr bool TWO = sizeof(T) == 4, SCALED = !__is_same(T, _Float16);
@@ -189,7 +191,7 @@ __global__ __launch_bounds__(256) void k_ce_pack(Job h, Job w, Scale g, Scalars*
     else pack_rows<T, false>((T*)a.n, a.n_cols, i0, a.v.rows, j0, [&](int r, int c) { return tile[r][c]; });
   }
   if (a.t) {
-    if constexpr (TWO) pack_rows<_Float16, true>((_Float16*)a.t, a.t_cols, j0, a.v.cols, i0, [&](int r, int c) { return tile[c][r]; });
+    if constexpr (GradPieces<T>::N == 2) pack_rows<_Float16, true>((_Float16*)a.t, a.t_cols, j0, a.v.cols, i0, [&](int r, int c) { return tile[c][r]; });
     else pack_rows<_Float16, false>((_Float16*)a.t, a.t_cols, j0, a.v.cols, i0, [&](int r, int c) { return tile[c][r] * f; });
   }
 }
@@ -393,7 +395,8 @@ __global__ __launch_bounds__(256) void k_ce_total(Finish a) {
 
 constexpr float DSCALE = 16384.f;   // D lies in [-2^14, 2^14]
 
-template <class T, int P, class C>
+// N: pieces of D
+template <class T, int P, int N, class C>
 __global__ __launch_bounds__(C::THREADS, C::LDS > 81920 ? C::THREADS / 256 : C::THREADS / 128) void k_ce_d(Logits a, int tm, int tn) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
   int im, in;
@@ -452,11 +455,11 @@ __global__ __launch_bounds__(C::THREADS, C::LDS > 81920 ? C::THREADS / 256 : C::
         z[r] *= DSCALE;
       }
       if (nb < a.rows && mb < a.d_cols) {
-        if constexpr (P == 2) store_t_f16x2((_Float16*)a.d + (int64_t)nb * 2 * a.d_cols + mb * 2, 2 * a.d_cols, patch, L, a.rows - nb, z);
+        if constexpr (N == 2) store_t_f16x2((_Float16*)a.d + (int64_t)nb * 2 * a.d_cols + mb * 2, 2 * a.d_cols, patch, L, a.rows - nb, z);
         else store_t_16<_Float16>((_Float16*)a.d + (int64_t)nb * a.d_cols + mb, a.d_cols, patch, L, a.rows - nb, z);
       }
       if (nb < a.dt_cols && mb < a.cols) {
-        if constexpr (P == 2) store_n_f16x2((_Float16*)a.dt + (int64_t)mb * 2 * a.dt_cols + nb * 2, 2 * a.dt_cols, patch, L, a.cols - mb, v);
+        if constexpr (N == 2) store_n_f16x2((_Float16*)a.dt + (int64_t)mb * 2 * a.dt_cols + nb * 2, 2 * a.dt_cols, patch, L, a.cols - mb, v);
         else store_n_16<_Float16>((_Float16*)a.dt + (int64_t)mb * a.dt_cols + nb, a.dt_cols, patch, L, a.cols - mb, v);
       }
     }
@@ -602,6 +605,7 @@ __global__ __launch_bounds__(256) void k_ce_join(Join a) {
 // ------------------------------------------------------------------------------------------------------------- host
 struct Shape { int64_t rows, hidden, vocab; int elem; };
 int pieces(int elem) { return elem == GRLHIP_ELEM_F32 ? 2 : 1; }
+int grad_pieces(int elem) { return elem == GRLHIP_ELEM_BF16 ? 1 : 2; }
 
 // The shapes of tiles.  Measured per K block (128 bytes a row), one or two pieces: a tile alone on its CU, and the CU's time for one on
 // a full chip.  4096 x 4096 x 8192 in bf16: 446, 282, 245 us (616, 976, 1123 TFLOP/s); 1024 x 1024 x 1024: 7.5, 12, 24 us.
@@ -644,9 +648,8 @@ void plan_gradients(Layout& l, const Shape& c, int64_t vp, int p) {
   double best = 0;
   for (int k = 0; k < KINDS; ++k) {
     const int64_t th = tiles_of(c.hidden, c.rows, k), tw = tiles_of(c.hidden, l.piece, k);
-    for (int sh = 1; sh <= 32; sh *= 2)
-      for (int sw = 1; sw <= 32; sw *= 2) {
-        if ((sh > 1 && kh / sh < 4) || (sw > 1 && kw / sw < 4)) continue;
+    for (int sh = 1; sh <= 32 && (sh == 1 || kh / sh >= 4); sh *= 2)
+      for (int sw = 1; sw <= 32 && (sw == 1 || kw / sw >= 4); sw *= 2) {
         const double parts = (sh > 1 ? (double)sh * c.rows * c.hidden : 0) + (sw > 1 ? (double)sw * l.piece * c.hidden : 0);
         const double cus = device_cus(), epilogue = SIDE[k] * SIDE[k] * 0.3e-3 + 0.8;
         const double sum = th * sh * ((double)kh / sh * FULL[p - 1][k] + epilogue) + tw * sw * ((double)kw / sw * FULL[p - 1][k] + epilogue);
@@ -678,7 +681,7 @@ Layout layout_of(const Shape& c, bool direct_h, bool direct_w, bool backward, bo
   l.piece = up((c.vocab + l.pieces_n - 1) / l.pieces_n, 256);
   if (l.piece > c.vocab) l.piece = c.vocab;
   l.pieces_n = (c.vocab + l.piece - 1) / l.piece;
-  l.kind_z = kind_for(l.piece, c.rows, l.kp * per / KBLOCK, p, backward ? d_ns(p) : FORWARD_NS);
+  l.kind_z = kind_for(l.piece, c.rows, l.kp * per / KBLOCK, p, backward ? d_ns(grad_pieces(c.elem)) : FORWARD_NS);
   const int side = SIDE[l.kind_z];
   int64_t at = 0;
   auto take = [&](int64_t bytes) { const int64_t o = at; at += up(bytes, 256); return o; };
@@ -691,13 +694,14 @@ Layout layout_of(const Shape& c, bool direct_h, bool direct_w, bool backward, bo
     l.sums = take(up(c.rows, 4) / 4 * 16);
   } else {
     const int64_t vp = up(l.piece, 64);
-    l.ht = take(c.hidden * l.np * per);
-    l.wt = take(c.hidden * vp * per);
-    l.d = take(c.rows * vp * per);
-    l.dt = take(l.piece * l.np * per);
+    const int64_t gper = grad_pieces(c.elem) * 2;
+    l.ht = take(c.hidden * l.np * gper);
+    l.wt = take(c.hidden * vp * gper);
+    l.d = take(c.rows * vp * gper);
+    l.dt = take(l.piece * l.np * gper);
     l.scale = take(c.rows * 4);
     if (bias) l.bpart = take(up(c.rows, side) / side * l.piece * 4);
-    plan_gradients(l, c, vp, p);
+    plan_gradients(l, c, vp, grad_pieces(c.elem));
     if (l.split_h > 1 || l.pieces_n > 1) l.hslots = take(l.split_h * c.rows * c.hidden * 4);
     if (l.split_w > 1) l.wslots = take(l.split_w * l.piece * c.hidden * 4);
   }
@@ -827,7 +831,7 @@ int forward(const Call& a) {
 
 template <class T>
 int backward(const Call& a) {
-  constexpr int P = sizeof(T) == 4 ? 2 : 1;
+  constexpr int P = sizeof(T) == 4 ? 2 : 1, N = GradPieces<T>::N;
   const Layout l = layout_of(a.c, direct(a.h, a.h0, a.h1, a.c), direct(a.w, a.w0, a.w1, a.c), true, a.gb != nullptr);
   if (!a.ws || (int64_t)a.ws_bytes < l.bytes) return set_error(GRLHIP_ERR_WORKSPACE, "linear_ce_backward: workspace too small: need " + std::to_string(l.bytes));
   Scalars* s = (Scalars*)(a.ws + l.scalars);
@@ -856,7 +860,7 @@ int backward(const Call& a) {
     g.dt_cols = l.np;
     g.bpart = a.gb ? (float*)(a.ws + l.bpart) : nullptr;
     const int tm = (int)(up(cols, side) / side);
-#define CALL(C) tile_launch(k_ce_d<typename Operands<T>::type, P, C>, tm * tn, C::THREADS, C::LDS, a.stream, g, tm, (int)tn)
+#define CALL(C) tile_launch(k_ce_d<typename Operands<T>::type, P, N, C>, tm * tn, C::THREADS, C::LDS, a.stream, g, tm, (int)tn)
     if (const int rc = BY_KIND(l.kind_z, CALL)) return rc;
 #undef CALL
 
@@ -864,11 +868,11 @@ int backward(const Call& a) {
     Grad &gh = j.both.g[0], &gw = j.both.g[1];
     j.both.s = s;
     if (a.gh) {
-      gh.a = {a.ws + l.wt, vp * 2 * P};
-      gh.b = {a.ws + l.d, vp * 2 * P};
+      gh.a = {a.ws + l.wt, vp * 2 * N};
+      gh.b = {a.ws + l.d, vp * 2 * N};
       gh.m = (int)a.c.hidden;
       gh.n = (int)a.c.rows;
-      gh.nkb = (int)(vp * 2 * P / KBLOCK);
+      gh.nkb = (int)(vp * 2 * N / KBLOCK);
       gh.split = l.split_h;
       gh.tiles = (int)tiles_of(gh.m, gh.n, l.kind_g) * gh.split;
       gh.slots = l.hslots ? (float*)(a.ws + l.hslots) : nullptr;
@@ -879,11 +883,11 @@ int backward(const Call& a) {
       if (gh.slots && last) j.blocks[0] = join_blocks(gh);
     }
     if (a.gw) {
-      gw.a = {a.ws + l.ht, l.np * 2 * P};
-      gw.b = {a.ws + l.dt, l.np * 2 * P};
+      gw.a = {a.ws + l.ht, l.np * 2 * N};
+      gw.b = {a.ws + l.dt, l.np * 2 * N};
       gw.m = (int)a.c.hidden;
       gw.n = (int)cols;
-      gw.nkb = (int)(l.np * 2 * P / KBLOCK);
+      gw.nkb = (int)(l.np * 2 * N / KBLOCK);
       gw.split = l.split_w;
       gw.tiles = (int)tiles_of(gw.m, gw.n, l.kind_g) * gw.split;
       gw.slots = l.wslots ? (float*)(a.ws + l.wslots) : nullptr;
@@ -891,7 +895,7 @@ int backward(const Call& a) {
       if (gw.slots) j.blocks[1] = join_blocks(gw);
     }
     if (gh.tiles + gw.tiles > 0) {
-#define CALL(C) tile_launch(k_ce_grad<T, P, C>, gh.tiles + gw.tiles, C::THREADS, C::LDS, a.stream, j.both)
+#define CALL(C) tile_launch(k_ce_grad<T, GradPieces<T>::P, C>, gh.tiles + gw.tiles, C::THREADS, C::LDS, a.stream, j.both)
       if (const int rc = BY_KIND(l.kind_g, CALL)) return rc;
 #undef CALL
     }

@@ -5,7 +5,7 @@ Tolerances, entry by entry, from the arithmetic (K features, N rows, u the half 
       16 products in fp32: (K / 16 + 16) 2^-24 of sum_k |h| |w|.
   loss: the largest error of z in the row twice (logsumexp and the target), 2^-21 of the magnitudes for exp, log and sums.
   D = softmax - onehot: twice the error of z and exp's own |z - lse| 2^-22 relative to the softmax, then the rounding of D
-      (u of fp16, 2^-21 for two pieces, 2^-38 absolute for fp16's smallest numbers).
+      (bf16 operands: u of fp16; others: 2^-21 for two pieces; 2^-38 absolute for fp16's smallest numbers).
   dh, dW: these times |W|, |h|; the fp32 sum over V or N; the result's own rounding (u, and fp16's smallest number)."""
 import ctypes
 import math
@@ -72,7 +72,7 @@ def oracle(h, w, t, b, rw, reduction, upstream=None):
     ep = p * (2 * e_row.unsqueeze(1) + (torch.where(z.isfinite(), (z - lse.unsqueeze(1)).abs(), 0.0) + 2) * 2.0 ** -22)
     d = p.clone()
     d.scatter_add_(1, at, torch.full_like(d[:, :1], -1.0))
-    u = 2.0 ** -21 if kind == F32 else torch.finfo(F16).eps / 2
+    u = torch.finfo(F16).eps / 2 if kind == BF16 else 2.0 ** -21
     ed = ep + u * d.abs() + 2.0 ** -38
     d, ed = torch.where(kept.unsqueeze(1), d, 0.0), torch.where(kept.unsqueeze(1), ed, 0.0)
     g = torch.where(kept, g, 0.0)
@@ -154,6 +154,21 @@ def test_gpu_pieces_of_the_vocabulary(dtype):
     out = oracle(h, w, t, b, rw, "mean")
     near(loss.detach(), "total", out)
     for g, name in zip(grads, ("dh", "dw", "db")):
+        near(g, name, out)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_gpu_a_vocabulary_that_is_packed_in_pieces(dtype):
+    """A weight that has to be laid out anew (its rows are no whole K blocks), larger than one piece of it, few rows."""
+    h, w, t, b, rw = inputs(3, 2001, 70000, dtype, seed=6, ignored=0.0)
+    h.requires_grad_(), w.requires_grad_()
+    t[2] = 69999
+    b[69999] = 0.0
+    loss = linear_cross_entropy(h, w, t, bias=b, row_weight=rw, reduction="sum")
+    out = oracle(h, w, t, b, rw, "sum")
+    near(loss.detach(), "total", out)
+    for g, name in zip(torch.autograd.grad(loss, [h, w]), ("dh", "dw")):
         near(g, name, out)
 
 

@@ -110,6 +110,10 @@ def test_gpu_orthogonalize_takes_strides_batches_and_lists():
     for g, m in zip(got[:29], many):
         assert off(g, polar(m)) <= TOL
     assert optim.orthogonalize([]) == []
+    # more descriptions than one launch carries, too large for one workgroup each; the longest sums are not the first ones
+    long_list = [grad_like(70 + k, 75 + 9 * ((k * 7) % 40), seed=k) for k in range(41)]
+    for g, m in zip(optim.orthogonalize(long_list), long_list):
+        assert off(g, polar(m)) <= TOL
 
 
 @pytest.mark.gpu
