@@ -360,7 +360,7 @@ __global__ __launch_bounds__(256) void k_ce_finish(Finish a) {
       // a target outside the vocabulary has no loss: NaN, not a number that looks like one
       float loss = t >= 0 && t < a.vocab ? (lse - a.picked[n]) * w : NAN;
       if (!kept || w == 0.f) loss = 0.f;
-      a.lse[n] = lse;
+      if (a.lse) a.lse[n] = lse;
       a.losses[n] = loss;
       s[r] = loss;
       c[r] = kept ? 1.0 : 0.0;
@@ -733,7 +733,7 @@ int check(const char* who, const Call& a) {
   if (c.rows * c.hidden > 1ll << 34 || c.vocab * c.hidden > 1ll << 34) return set_error(GRLHIP_ERR_UNSUPPORTED, w + "over 2^34 entries of hidden or weight");
   if (c.elem != GRLHIP_ELEM_F32 && c.elem != GRLHIP_ELEM_BF16 && c.elem != GRLHIP_ELEM_F16) return set_error(GRLHIP_ERR_INVALID, w + "unknown element type");
   if (a.reduction < 0 || a.reduction > 2) return set_error(GRLHIP_ERR_INVALID, w + "unknown reduction");
-  if (!a.h || !a.w || !a.target || !a.lse) return set_error(GRLHIP_ERR_INVALID, w + "null hidden, weight, target or lse");
+  if (!a.h || !a.w || !a.target) return set_error(GRLHIP_ERR_INVALID, w + "null hidden, weight or target");
   return 0;
 }
 template <class T>
@@ -999,7 +999,7 @@ int grlhip_linear_ce_backward(const void* hidden, const int64_t* hidden_strides,
     a.ws_bytes = workspace_bytes;
     a.stream = (hipStream_t)stream;
     if (const int rc = check("linear_ce_backward", a)) return rc;
-    if (!grad || (!count && reduction == GRLHIP_REDUCE_MEAN)) return set_error(GRLHIP_ERR_INVALID, "linear_ce_backward: null gradient or count");
+    if (!lse || !grad || (!count && reduction == GRLHIP_REDUCE_MEAN)) return set_error(GRLHIP_ERR_INVALID, "linear_ce_backward: null lse, gradient or count");
     if ((size_t)workspace & 255) return set_error(GRLHIP_ERR_INVALID, "linear_ce_backward: the workspace must be aligned to 256 bytes");
     if (!grad_hidden && !grad_weight && !grad_bias) return 0;
     return elem == GRLHIP_ELEM_F32 ? backward<float>(a) : elem == GRLHIP_ELEM_BF16 ? backward<__bf16>(a) : backward<_Float16>(a);

@@ -14,6 +14,22 @@ def _stream(device):
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+class _on:
+    """``torch.cuda.device(device)`` that costs next to nothing where the device is current already."""
+    __slots__ = ("other",)
+
+    def __init__(self, device):
+        self.other = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.other is not None:
+            self.other.__enter__()
+
+    def __exit__(self, *exc):
+        if self.other is not None:
+            self.other.__exit__(*exc)
+
+
 def _f32c(t, name, shape=None):
     if t is None:
         return None

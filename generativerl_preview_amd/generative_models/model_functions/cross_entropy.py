@@ -7,6 +7,7 @@ import weakref
 import torch
 
 from ... import _lib as L
+from ...engine import _on
 
 _ELEM = {torch.float32: L.ELEM_F32, torch.bfloat16: L.ELEM_BF16, torch.float16: L.ELEM_F16}
 _REDUCE = {"none": L.REDUCE_NONE, "mean": L.REDUCE_MEAN, "sum": L.REDUCE_SUM}
@@ -39,21 +40,24 @@ class _Head:
         if need == 0:
             raise L.GrlHipError(lib.grlhip_last_error().decode())
         # one workspace per call: calls on different streams and captured graphs must not share it
-        with torch.cuda.device(self.device):
+        with _on(self.device):
             ws = torch.empty(need, dtype=torch.uint8, device=self.device)
             stream = torch.cuda.current_stream(self.device).cuda_stream
             L.check(getattr(lib, name)(*self.arguments, *rest, ws.data_ptr(), need, stream))
 
     def forward(self, train=False):
-        """(losses, logsumexp, reduced loss, [number of rows that are not ignored, largest magnitudes of the operands])"""
+        """(losses, logsumexp, reduced loss, [number of rows that are not ignored, largest magnitudes of the operands]); the
+        backward pass needs the second and the last"""
         rows, dev = self.shape[0], self.device
-        losses, lse = torch.empty(rows, dtype=torch.float32, device=dev), torch.empty(rows, dtype=torch.float32, device=dev)
-        total, numbers, count = None, None, None
+        losses = torch.empty(rows, dtype=torch.float32, device=dev)
+        lse = total = numbers = count = None
+        if train:
+            lse = torch.empty(rows, dtype=torch.float32, device=dev)
         if train or self.reduction != L.REDUCE_NONE:
             numbers = torch.empty(3, dtype=torch.float32, device=dev)
         if self.reduction != L.REDUCE_NONE:
             total, count = torch.empty((), dtype=torch.float32, device=dev), numbers.data_ptr()
-        self.call("grlhip_linear_ce_forward", 0, losses.data_ptr(), lse.data_ptr(), _address(total), count,
+        self.call("grlhip_linear_ce_forward", 0, losses.data_ptr(), _address(lse), _address(total), count,
                   numbers.data_ptr() + 4 if train else None)
         return losses, lse, total, numbers
 

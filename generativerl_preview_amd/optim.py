@@ -22,7 +22,7 @@ import torch
 
 from . import _lib as L
 from .distributed import attach_flat_grads
-from .engine import _ptr, _stream
+from .engine import _on, _ptr, _stream
 
 NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)   # a, b, c: 5 steps bring singular values from 0.002 on into [0.68, 1.21]
 _ELEM = {torch.float32: L.ELEM_F32, torch.bfloat16: L.ELEM_BF16, torch.float16: L.ELEM_F16}
@@ -194,7 +194,7 @@ def orthogonalize(matrices, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7):
         dev = src[0].device
         a, b, c = coefficients
         ws = _newton_schulz_workspace(shapes, len(src), dev)
-        with torch.cuda.device(dev):
+        with _on(dev):
             L.check(L.lib().grlhip_orthogonalize(_pointers(pointers), _pointers([t.data_ptr() for t in dst]), shapes,
                                                  None if dense else _stride_array(src, dst), len(src), _ELEM[src[0].dtype],
                                                  int(steps), a, b, c, eps, _ptr(ws), ws.numel(), _stream(dev)))
@@ -234,7 +234,7 @@ def muon_step(params, grads, momentum_buffers, lr, momentum=0.95, nesterov=True,
     shapes, dev = _shape_array(params), params[0].device
     a, b, c = coefficients
     ws = _newton_schulz_workspace(shapes, len(params), dev)
-    with torch.cuda.device(dev):
+    with _on(dev):
         L.check(L.lib().grlhip_muon_step(_pointers(pp), _pointers(gp), _pointers(bp), shapes,
                                          None if pd and gd and bd else _stride_array(grads, params, bufs), rates, len(params),
                                          momentum, int(nesterov), 1.0 - lr * weight_decay, int(steps), a, b, c, eps, _ptr(ws),

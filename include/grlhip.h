@@ -376,7 +376,7 @@ typedef enum { GRLHIP_REDUCE_NONE = 0, GRLHIP_REDUCE_MEAN = 1, GRLHIP_REDUCE_SUM
 
 /* No counterpart in the reference (its policies are continuous).  Softmax cross entropy of a linear head over a large
  * vocabulary (discretised actions), without storing the logits z = hidden weight^T + bias:
- *   losses[i] = row_weight[i] (logsumexp_v z[i][v] - z[i][target[i]]);   lse[i] = logsumexp_v z[i][v]
+ *   losses[i] = row_weight[i] (logsumexp_v z[i][v] - z[i][target[i]]);   lse[i] = logsumexp_v z[i][v]  (may be NULL)
  *   *total = sum of the losses (GRLHIP_REDUCE_SUM, _NONE) or that over *count (_MEAN); *count = number of rows whose target is
  *   not ignore_index, at least 1.  Both may be NULL for GRLHIP_REDUCE_NONE.
  *   largest[2] = largest finite magnitudes of hidden and weight, written for GRLHIP_ELEM_F32 only (the backward call may take

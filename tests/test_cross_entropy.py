@@ -434,7 +434,8 @@ def test_c_entry_points_check_their_arguments_without_a_gpu():
 
     assert fwd() == -4 and bwd() == -4 and b"workspace" in lib.grlhip_last_error()
     assert fwd(total=None, count=None) == -1 and fwd(total=None, count=None, red=L.REDUCE_NONE) == -4
-    for bad in ("h", "w", "t", "losses", "lse", "total", "count"):
+    assert fwd(lse=None) == -4
+    for bad in ("h", "w", "t", "losses", "total", "count"):
         assert fwd(**{bad: None}) == -1, bad
     for bad in ("h", "w", "t", "lse", "count", "grad"):
         assert bwd(**{bad: None}) == -1, bad
