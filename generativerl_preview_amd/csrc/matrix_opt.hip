@@ -209,7 +209,7 @@ __global__ __launch_bounds__(256) void k_orth_split(Table t, Numbers g) {
 
 // One product of every matrix.  k: which X is read.
 template <class C, int STAGE, class T, bool MUON>
-__global__ __launch_bounds__(C::THREADS, C::LDS > 81920 ? C::THREADS / 256 : C::THREADS / 128) void k_orth_product(Table t, Numbers g, int k) {
+__global__ __launch_bounds__(C::THREADS, C::LDS > 81920 || C::THREADS < 256 ? (C::THREADS + 255) / 256 : C::THREADS / 128) void k_orth_product(Table t, Numbers g, int k) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
   constexpr bool SYM = STAGE == GRAM || STAGE == POLY;
   constexpr int FIRST = STAGE == LAST ? 3 : STAGE + 1;
@@ -552,21 +552,25 @@ int check_coefficients(const char* who, float a, float b, float c, int steps) {
 }
 
 // The shapes of tiles.  Measured per K block of 32 (two pieces, 3 MFMAs), operands from beyond the L2 as the launch before left them:
-// a tile alone on its CU, and the CU's time for one on a full chip (730, 720, 940, 760, 1070, 1190, 1180 TFLOP/s of MFMAs at best).
-// 512 x 512 x 512: 4.0, 6.1, 7.5, -, 11.3, 12.5, 30 us; 1024 x 1024 x 1024: 17.8, 10.4, 12.8, -, 20, 23, 57 us; 2048 x 4096 x 2048: 225,
-// 141, 110, -, 90, 87, 125 us; 1536 x 1536 x 4096: -, 98, -, 63, 77 us; 8192 x 8192 x 2048: 774 (128), 698 us (256).
-typedef Tile<32, 32, 1, 1, 3, 4> Orth32;
-typedef Tile<64, 64, 2, 2, 3, 2> Orth64K;      // 96 KiB: one a CU, for launches of no more tiles than CUs; three stages cover the latency
-typedef Tile<64, 64, 2, 2, 2, 2> Orth64;
-typedef Tile<96, 96, 1, 3, 2, 3> Orth96K;      // one a CU again: the triangle of 2048 is 253 of these, and 136 of 128
-typedef Tile<128, 128, 2, 2, 2, 2> Orth128K;   // one a CU again
-typedef Tile<128, 128, 2, 2, 2> Orth128;
-typedef Tile<256, 256, 2, 4, 2> Orth256;
-constexpr int KINDS = 7, SIDE[KINDS] = {32, 64, 64, 96, 128, 128, 256};
-constexpr double ALONE[KINDS] = {0.095, 0.27, 0.33, 0.47, 0.60, 0.67, 1.9}, FULL[KINDS] = {0.11, 0.28, 0.215, 0.60, 0.75, 0.68, 2.73};
-// The epilogue moves 12 bytes an entry at a CU's share of the memory and hardly overlaps with products (all tiles of a launch
-// take the same time); what a tile costs besides.
-constexpr double EPILOGUE = 12 / 15e3, FIXED[KINDS] = {2.5, 0.8, 0.8, 0.8, 0.8, 0.8, 0.8};
+// ALONE, a tile on its CU, and FULL, the CU's time for one on a full chip.  us by kind in the order below:
+//   512 x 512 x 512: 4.0, 4.5, 5.6, 6.1, 7.5, -, 11.3, 12.5, 30;  1024 x 768 x 256: 7.4, 5.8, 4.6, 4.5, 5.0;
+//   1024 x 1024 x 1024: 17.8, 14.4, 12.1, 10.4, 12.8, -, 20, 23, 57;  1536 x 1536 x 4096: 63 (96), 77 (128K);
+//   2048 x 4096 x 2048: 225, -, -, 141, 110, -, 90, 87, 125;  8192 x 8192 x 2048: 774 (128), 698 (256: 1180 TFLOP/s of MFMAs).
+typedef Tile<32, 32, 1, 1, 3, 4> Orth32K;      // 96 KiB, one a CU: three stages cover the latency of few tiles
+typedef Tile<32, 32, 1, 1, 2, 4> Orth32;       // 64 KiB, two a CU
+typedef Tile<32, 32, 1, 1, 2, 2> Orth32S;      // 32 KiB, five a CU: many short tiles
+typedef Tile<64, 64, 2, 2, 3, 2> Orth64K;      // 96 KiB
+typedef Tile<64, 64, 2, 2, 2, 2> Orth64;       // 64 KiB
+typedef Tile<96, 96, 1, 3, 2, 3> Orth96K;      // 144 KiB: the triangle of 2048 is 253 of these, and 136 of 128
+typedef Tile<128, 128, 2, 2, 2, 2> Orth128K;   // 128 KiB
+typedef Tile<128, 128, 2, 2, 2> Orth128;       // 64 KiB
+typedef Tile<256, 256, 2, 4, 2> Orth256;       // 128 KiB
+constexpr int KINDS = 9, SIDE[KINDS] = {32, 32, 32, 64, 64, 96, 128, 128, 256}, BESIDE[KINDS] = {1, 2, 5, 1, 2, 1, 1, 2, 1};   // workgroups a CU
+constexpr double ALONE[KINDS] = {0.095, 0.106, 0.21, 0.27, 0.33, 0.47, 0.60, 0.67, 1.9};
+constexpr double FULL[KINDS] = {0.11, 0.083, 0.08, 0.28, 0.215, 0.60, 0.75, 0.68, 2.73};
+// Besides: what a tile costs whatever its length, shared by the workgroups beside each other; and the epilogue's 12 bytes an entry
+// at a CU's share of the memory, which hardly overlap with products (all tiles of a launch take the same time).
+constexpr double FIXED[KINDS] = {2.5, 2.5, 2.5, 0.8, 1.6, 0.8, 0.8, 1.6, 0.8}, EPILOGUE = 12 / 15e3;
 
 int64_t tiles_of(const Parts& p, int stage, int side) {
   const int64_t tm = (p.mp + side - 1) / side, tn = (p.np + side - 1) / side;
@@ -587,7 +591,7 @@ Plan plan_of(const int64_t* shapes, int count) {
         const double kb = (double)(s == GRAM ? p.np : p.mp) / 32;
         const int64_t t = tiles_of(p, s, SIDE[k]);
         tiles[s][k] += t;
-        sum[s][k] += t * (kb * FULL[k] + FIXED[k]);
+        sum[s][k] += t * (kb * FULL[k] + FIXED[k] / BESIDE[k]);
         longest[s][k] = std::fmax(longest[s][k], kb * ALONE[k]);
       }
   }
@@ -616,12 +620,14 @@ int launch(const Table& t, const Numbers& num, int k, int64_t tiles, hipStream_t
 template <int STAGE, class T, bool MUON>
 int product_launch(int kind, const Table& t, const Numbers& num, int k, int64_t tiles, hipStream_t stream) {
   switch (kind) {
-    case 0: return launch<Orth32, STAGE, T, MUON>(t, num, k, tiles, stream);
-    case 1: return launch<Orth64K, STAGE, T, MUON>(t, num, k, tiles, stream);
-    case 2: return launch<Orth64, STAGE, T, MUON>(t, num, k, tiles, stream);
-    case 3: return launch<Orth96K, STAGE, T, MUON>(t, num, k, tiles, stream);
-    case 4: return launch<Orth128K, STAGE, T, MUON>(t, num, k, tiles, stream);
-    case 5: return launch<Orth128, STAGE, T, MUON>(t, num, k, tiles, stream);
+    case 0: return launch<Orth32K, STAGE, T, MUON>(t, num, k, tiles, stream);
+    case 1: return launch<Orth32, STAGE, T, MUON>(t, num, k, tiles, stream);
+    case 2: return launch<Orth32S, STAGE, T, MUON>(t, num, k, tiles, stream);
+    case 3: return launch<Orth64K, STAGE, T, MUON>(t, num, k, tiles, stream);
+    case 4: return launch<Orth64, STAGE, T, MUON>(t, num, k, tiles, stream);
+    case 5: return launch<Orth96K, STAGE, T, MUON>(t, num, k, tiles, stream);
+    case 6: return launch<Orth128K, STAGE, T, MUON>(t, num, k, tiles, stream);
+    case 7: return launch<Orth128, STAGE, T, MUON>(t, num, k, tiles, stream);
     default: return launch<Orth256, STAGE, T, MUON>(t, num, k, tiles, stream);
   }
 }
