@@ -235,7 +235,8 @@ __global__ __launch_bounds__(C::THREADS, C::LDS > 81920 || C::THREADS < 256 ? (C
   const Lane L = lane_of();
   const int wm = L.wave / C::WN % C::WM, wn = L.wave % C::WN;
   // The operand that the epilogue adds (A of the polynomial, X of the update; read transposed: 4 consecutive entries).  Small
-  // tiles ask for it before the product: its latency, 1 us from another XCD's stores, is a good part of such a launch.
+  // tiles ask for it before their last block: its latency, 1 us from another XCD's stores, is a good part of such a launch.  (Asked for
+  // before the product it stood in front of the tiles' own loads: a product of 256 x 256 took 4.0 us instead of 2.7.)
   constexpr bool OWN = STAGE != GRAM, EARLY = OWN && C::TM * C::TN == 1;
   f16x4 own[EARLY ? 8 : 1];
   auto load_own = [&](int64_t mb, int64_t n, f16x4* hi, f16x4* lo) {
@@ -246,19 +247,19 @@ __global__ __launch_bounds__(C::THREADS, C::LDS > 81920 || C::THREADS < 256 ? (C
       lo[c] = *(const f16x4*)(o + 32 + 8 * c + 4 * L.h);
     }
   };
-  if constexpr (EARLY) {
+  auto late = [&] {
     const int64_t mb = m0 + wm * 32, nb = n0 + wn * 32;
-    if (mb < p.mp && nb < (SYM ? p.mp : p.np)) load_own(mb, nb + L.j, own, own + 4);
-  }
+    if (EARLY && mb < p.mp && nb < (SYM ? p.mp : p.np)) load_own(mb, nb + L.j, own, own + (EARLY ? 4 : 0));
+  };
   if (STAGE == GRAM) {
     const char* x = (const char*)p.X(a.ws, k);
     if (!product<_Float16, 2, C>(x + m0 * xp, xp, p.mp - m0, x + n0 * xp, xp, p.mp - n0, (int)(p.np / 32), lds, acc)) return;
   } else if (STAGE == POLY) {
     const char* x = (const char*)p.A(a.ws);
-    if (!product<_Float16, 2, C>(x + m0 * ap, ap, p.mp - m0, x + n0 * ap, ap, p.mp - n0, (int)(p.mp / 32), lds, acc)) return;
+    if (!product<_Float16, 2, C>(x + m0 * ap, ap, p.mp - m0, x + n0 * ap, ap, p.mp - n0, (int)(p.mp / 32), lds, acc, late)) return;
   } else {
     if (!product<_Float16, 2, C>((const char*)p.B(a.ws) + m0 * ap, ap, p.mp - m0, (const char*)p.XT(a.ws, k) + n0 * ap, ap, p.np - n0,
-                                 (int)(p.mp / 32), lds, acc)) return;
+                                 (int)(p.mp / 32), lds, acc, late)) return;
   }
   unsigned* patch = (unsigned*)(lds + L.wave * PATCH);
 #pragma unroll
