@@ -64,9 +64,16 @@ __device__ __forceinline__ float largest_gradient(const Scalars* s) { return wav
 
 struct View { const void* p; int64_t s0, s1; int rows, cols; };   // element strides
 
-// the largest finite magnitudes of hidden (blocks [0, HMAX)) and weight (the others)
+// What leaves a row of hidden (its target, its weight) or of the weight (a bias of -inf) out of everything.
+struct Left { const int64_t* target; const float* row_weight; int64_t ignore; const float* bias; };
+__device__ __forceinline__ bool row_counts(const Left& l, int row) { return l.target[row] != l.ignore && !(l.row_weight && l.row_weight[row] == 0.f); }
+__device__ __forceinline__ bool masked(const float* bias, int v) { return bias && bias[v] == -INFINITY; }
+
+// The largest finite magnitudes of hidden (blocks [0, HMAX)) and weight (the others), of the rows that are not left out: padding may
+// hold anything, and a scale that follows it would cost the others their bits.  Whether a row counts is asked only for an
+// entry that would raise the maximum.
 template <class T>
-__global__ __launch_bounds__(256) void k_ce_absmax(View h, View w, Scalars* s) {
+__global__ __launch_bounds__(256) void k_ce_absmax(View h, View w, Left left, Scalars* s) {
   __shared__ float sh[4];
   const bool is_h = blockIdx.x < HMAX;
   const View& v = is_h ? h : w;
@@ -74,22 +81,47 @@ __global__ __launch_bounds__(256) void k_ce_absmax(View h, View w, Scalars* s) {
   constexpr int E = 16 / sizeof(T);
   typedef T vec __attribute__((ext_vector_type(E)));
   float m = 0.f;
+  auto counts = [&](int row) { return is_h ? row_counts(left, row) : !masked(left.bias, row); };
   if (v.s1 == 1 && v.s0 == v.cols && ((size_t)v.p & 15) == 0) {   // dense: 16 bytes a thread
-    const int64_t all = (int64_t)v.rows * v.cols, whole = all / E;
+    const int64_t all = (int64_t)v.rows * v.cols, whole = all / E, step = (int64_t)n * 256;
     const vec* p = (const vec*)v.p;
-#pragma unroll 4
-    for (int64_t k = (int64_t)b * 256 + threadIdx.x; k < whole; k += (int64_t)n * 256) {
-      const vec x = p[k];
+    for (int64_t k = (int64_t)b * 256 + threadIdx.x; k < whole; k += 4 * step) {
+      vec x[4];
 #pragma unroll
-      for (int e = 0; e < E; ++e) m = fmaxf(m, finite((float)x[e]));
+      for (int u = 0; u < 4; ++u) x[u] = p[k + u * step < whole ? k + u * step : k];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        float top = 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) top = fmaxf(top, finite((float)x[u][e]));
+        if (top > m) {
+          const int64_t first = (k + u * step < whole ? k + u * step : k) * E;
+          int row = (int)(first / v.cols), col = (int)(first - (int64_t)row * v.cols);
+          bool in = counts(row);
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            if (in) m = fmaxf(m, finite((float)x[u][e]));
+            if (++col == v.cols && e + 1 < E) {
+              col = 0;
+              in = counts(++row < v.rows ? row : v.rows - 1);
+            }
+          }
+        }
+      }
     }
-    if (b == 0 && threadIdx.x < all - whole * E) m = fmaxf(m, finite((float)((const T*)v.p)[whole * E + threadIdx.x]));
+    if (b == 0 && threadIdx.x < all - whole * E) {
+      const int64_t k = whole * E + threadIdx.x;
+      if (counts((int)(k / v.cols))) m = fmaxf(m, finite((float)((const T*)v.p)[k]));
+    }
   } else {
     const bool along = v.s1 <= v.s0;   // lanes along the axis that is closer in memory
     const int outer = along ? v.rows : v.cols, inner = along ? v.cols : v.rows;
     const int64_t so = along ? v.s0 : v.s1, si = along ? v.s1 : v.s0;
     for (int o = b * 4 + (threadIdx.x >> 6); o < outer; o += n * 4)
-      for (int i = threadIdx.x & 63; i < inner; i += 64) m = fmaxf(m, finite((float)((const T*)v.p)[o * so + i * si]));
+      for (int i = threadIdx.x & 63; i < inner; i += 64) {
+        const float x = finite((float)((const T*)v.p)[o * so + i * si]);
+        if (x > m && counts(along ? o : i)) m = x;
+      }
   }
   m = block_max(m, sh);
   if (threadIdx.x == 0) (is_h ? s->hpart : s->wpart)[b] = m;
@@ -97,18 +129,19 @@ __global__ __launch_bounds__(256) void k_ce_absmax(View h, View w, Scalars* s) {
 
 // A view -> operands: as it stands (n: rows of the view, type E) and transposed (t: its columns, fp16), either may be null; columns
 // beyond the view and up to the pitch become zeros.  fp32: two scaled fp16 pieces both ways.  bf16 transposed: scaled.  A row that
-// does not count becomes zeros: whatever it holds must not reach a sum over rows.
+// does not count becomes zeros: whatever it holds must not reach a sum over rows; so do the finite entries of a masked row of the weight,
+// which the scale does not know.
 struct Job {
   View v;
   void* n; int64_t n_cols;
   void* t; int64_t t_cols;
-  bool mask; int blocks;
+  bool mask; const float* bias;   // leaves out rows: of hidden, of the weight
+  int blocks;
 };
 // The gradient of each row's own loss, and the largest of them.
 struct Scale {
   const float* grad; int64_t grad_stride;
-  const float* row_weight; const float* count;
-  const int64_t* target; int64_t ignore;
+  const float* count;
   int rows, vocab, reduction, blocks;
   float* scale;
 };
@@ -138,17 +171,17 @@ __device__ __forceinline__ void pack_rows(E* out, int64_t cols, int r0, int rows
 // pieces of D and of what it is multiplied by; 3: two, of which the other factor needs one
 template <class T> struct GradPieces { static constexpr int P = __is_same(T, float) ? 2 : __is_same(T, _Float16) ? 3 : 1, N = P == 1 ? 1 : 2; };
 template <class T>
-__global__ __launch_bounds__(256) void k_ce_pack(Job h, Job w, Scale g, Scalars* s, float* largest, bool known) {
+__global__ __launch_bounds__(256) void k_ce_pack(Job h, Job w, Scale g, Left left, Scalars* s, float* largest, bool known) {
   constexpr bool TWO = sizeof(T) == 4, SCALED = !__is_same(T, _Float16);
   __shared__ float tile[64][65], sh[4];
   if ((int)blockIdx.x >= h.blocks + w.blocks) {
     const int b = blockIdx.x - h.blocks - w.blocks;
     float most = 0.f;
     for (int n = b * 256 + threadIdx.x; n < g.rows; n += g.blocks * 256) {
-      const int64_t t = g.target[n];
-      const float rw = g.row_weight ? g.row_weight[n] : 1.f;
+      const int64_t t = left.target[n];
+      const float rw = left.row_weight ? left.row_weight[n] : 1.f;
       float v = 0.f;
-      if (t != g.ignore && rw != 0.f) {
+      if (t != left.ignore && rw != 0.f) {
         v = g.grad[n * g.grad_stride] * rw;
         if (g.reduction == GRLHIP_REDUCE_MEAN) v /= *g.count;
         if (t < 0 || t >= g.vocab) v = NAN;
@@ -182,8 +215,8 @@ __global__ __launch_bounds__(256) void k_ce_pack(Job h, Job w, Scale g, Scalars*
     const int i = along ? (tid >> 6) + 4 * k : tid & 63, j = along ? tid & 63 : (tid >> 6) + 4 * k;
     float x = 0.f;
     if (i0 + i < a.v.rows && j0 + j < a.v.cols) {
-      const bool counts = !a.mask || (g.target[i0 + i] != g.ignore && !(g.row_weight && g.row_weight[i0 + i] == 0.f));
-      if (counts) x = (float)((const T*)a.v.p)[(int64_t)(i0 + i) * a.v.s0 + (int64_t)(j0 + j) * a.v.s1];
+      if (!a.mask || row_counts(left, i0 + i)) x = (float)((const T*)a.v.p)[(int64_t)(i0 + i) * a.v.s0 + (int64_t)(j0 + j) * a.v.s1];
+      if (masked(a.bias, i0 + i) && __builtin_isfinite(x)) x = 0.f;
     }
     tile[i][j] = TWO ? x * f : x;
   }
@@ -744,9 +777,11 @@ View weight_piece(const Call& a, int64_t v0, int64_t cols) {
 }
 View hidden_of(const Call& a) { return {a.h, a.h0, a.h1, (int)a.c.rows, (int)a.c.hidden}; }
 
+Left left_of(const Call& a) { return {a.target, a.row_weight, a.ignore, a.bias}; }
+
 template <class T>
 void absmax_launch(const Call& a, Scalars* s) {
-  hipLaunchKernelGGL(k_ce_absmax<T>, dim3(HMAX + WMAX), dim3(256), 0, a.stream, hidden_of(a), weight_piece<T>(a, 0, a.c.vocab), s);
+  hipLaunchKernelGGL(k_ce_absmax<T>, dim3(HMAX + WMAX), dim3(256), 0, a.stream, hidden_of(a), weight_piece<T>(a, 0, a.c.vocab), left_of(a), s);
 }
 // Packs hidden (h null: not in this launch) and a weight piece, and takes the rows' gradients.
 template <class T>
@@ -755,7 +790,7 @@ void pack_launch(const Call& a, Job h, Job w, Scale g, Scalars* s, bool known) {
   blocks(h);
   blocks(w);
   const int all = h.blocks + w.blocks + g.blocks;
-  if (all > 0) hipLaunchKernelGGL(k_ce_pack<T>, dim3(all), dim3(256), 0, a.stream, h, w, g, s, a.largest, known);
+  if (all > 0) hipLaunchKernelGGL(k_ce_pack<T>, dim3(all), dim3(256), 0, a.stream, h, w, g, left_of(a), s, a.largest, known);
 }
 
 template <class K, class... A>
@@ -816,8 +851,8 @@ int forward(const Call& a) {
   int tiles = 0;
   for (int64_t v0 = 0; v0 < a.c.vocab; v0 += l.piece) {
     const View w = weight_piece<T>(a, v0, a.c.vocab - v0 < l.piece ? a.c.vocab - v0 : l.piece);
-    Job jh{hidden_of(a), v0 == 0 && l.pack_h ? a.ws + l.hp : nullptr, l.kp, nullptr, 0, false, 0};
-    Job jw{w, l.pack_w ? a.ws + l.wp : nullptr, l.kp, nullptr, 0, false, 0};
+    Job jh{hidden_of(a), v0 == 0 && l.pack_h ? a.ws + l.hp : nullptr, l.kp, nullptr, 0, false, nullptr, 0};
+    Job jw{w, l.pack_w ? a.ws + l.wp : nullptr, l.kp, nullptr, 0, false, a.bias ? a.bias + v0 : nullptr, 0};
     pack_launch<T>(a, jh, jw, Scale{}, s, false);
     Logits g = logits_call<T>(a, l, w, v0, s);
     g.part = (float2*)(a.ws + l.part) + (int64_t)tiles * a.c.rows;
@@ -846,11 +881,11 @@ int backward(const Call& a) {
     const bool first = v0 == 0, last = v0 + l.piece >= a.c.vocab;
     const int64_t cols = last ? a.c.vocab - v0 : l.piece, vp = up(cols, 64);
     const View w = weight_piece<T>(a, v0, cols);
-    const Job jh{hidden_of(a), first && l.pack_h ? a.ws + l.hp : nullptr, l.kp, first && a.gw ? a.ws + l.ht : nullptr, l.np, true, 0};
-    const Job jw{w, l.pack_w ? a.ws + l.wp : nullptr, l.kp, a.gh ? a.ws + l.wt : nullptr, vp, false, 0};
+    const Job jh{hidden_of(a), first && l.pack_h ? a.ws + l.hp : nullptr, l.kp, first && a.gw ? a.ws + l.ht : nullptr, l.np, true, nullptr, 0};
+    const Job jw{w, l.pack_w ? a.ws + l.wp : nullptr, l.kp, a.gh ? a.ws + l.wt : nullptr, vp, false, a.bias ? a.bias + v0 : nullptr, 0};
     int64_t gblocks = (a.c.rows + 255) / 256;
     if (gblocks > GMAX) gblocks = GMAX;
-    const Scale sc{a.grad, a.grad_stride, a.row_weight, a.count, a.target, a.ignore, (int)a.c.rows, (int)a.c.vocab, a.reduction, first ? (int)gblocks : 0, scale};
+    const Scale sc{a.grad, a.grad_stride, a.count, (int)a.c.rows, (int)a.c.vocab, a.reduction, first ? (int)gblocks : 0, scale};
     pack_launch<T>(a, jh, jw, sc, s, known);
 
     Logits g = logits_call<T>(a, l, w, v0, s);

@@ -191,6 +191,34 @@ def test_gpu_padding_may_hold_anything(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("features", [64, 7, 3])
+def test_gpu_large_numbers_in_padding_cost_the_others_nothing(features, dtype):
+    """Finite ones, in ignored rows, rows of weight 0 and masked rows of the vocabulary: they must not set the operands' scale."""
+    h, w, t, b, rw = inputs(130, features, 301, dtype, seed=16)
+    t[5], t[77], t[9] = -100, -100, 3
+    rw[9] = 0.0
+    b[[4, 300]] = -math.inf
+    t[(t == 4) | (t == 300)] = 3
+    b[3] = 0.0
+    gone = (b == -math.inf).nonzero()[0, 0].item(), 300
+    huge = 6e4 if dtype == F16 else 1e30
+    first = [x.clone() for x in (h, w)]
+    second = [x.clone() for x in (h, w)]
+    second[0][[5, 77, 9]] = huge
+    second[1][[gone[0], gone[1]]] = torch.where(torch.arange(features, device=DEV) % 2 == 0, huge, -huge).to(dtype)
+    for layout in (lambda x: x, lambda x: x.t().contiguous().t()):
+        results = []
+        for hh, ww in (first, second):
+            leaves = [layout(hh).requires_grad_(), layout(ww).requires_grad_()]
+            loss = linear_cross_entropy(*leaves, t, bias=b, row_weight=rw)
+            results.append([loss.detach(), *torch.autograd.grad(loss, leaves)])
+        for got, want in zip(results[1], results[0]):
+            assert torch.equal(got, want)
+        near(results[1][0], "total", oracle(h, w, t, b, rw, "mean"))
+
+
+@pytest.mark.gpu
 def test_gpu_all_rows_ignored_and_no_rows():
     h, w, t, b, rw = inputs(40, 64, 90, BF16)
     t.fill_(-100)
