@@ -73,30 +73,50 @@ class _Head:
 
 
 class _Graph:
-    """Lives as long as the autograd graph of one eager loss; `leaves`: the tensors it ends in."""
-    __slots__ = ("leaves", "__weakref__")
+    """Lives as long as the autograd graph of one eager loss; `roots`: where that graph goes on, leaves or the nodes of others."""
+    __slots__ = ("roots", "__weakref__")
 
-    def __init__(self, leaves):
-        self.leaves = leaves
+    def __init__(self, roots):
+        self.roots = roots
 
 
 _ON_DEFAULT_STREAM = weakref.WeakSet()
 
 
+def _leaves(roots):
+    """{id: leaf} of the tensors that the graphs of `roots` end in."""
+    found, seen, queue = {}, set(), []
+    for r in roots:
+        if torch.is_tensor(r):
+            found[id(r)] = r
+        else:
+            queue.append(r)
+    while queue:
+        node = queue.pop()
+        if node is None or node in seen:
+            continue
+        seen.add(node)
+        leaf = getattr(node, "variable", None)
+        if torch.is_tensor(leaf):
+            found[id(leaf)] = leaf
+        queue.extend(n for n, _ in node.next_functions)
+    return found
+
+
 def _watch(ctx, *tensors):
     """autograd adds up a leaf's gradient on the stream where the leaf first entered a live graph.  If that is the default
     stream, a backward pass under capture reaches for a stream that cannot be captured, and the process ends: such a
-    call is refused while it is still a call."""
-    leaves = [t for t in tensors if t is not None and t.requires_grad and t.is_leaf]
-    if not leaves:
+    call is refused while it is still a call.  The graphs are walked under capture only."""
+    roots = [t if t.is_leaf else t.grad_fn for t in tensors if t is not None and t.requires_grad]
+    if not roots:
         return
     if torch.cuda.is_current_stream_capturing():
-        for graph in list(_ON_DEFAULT_STREAM):
-            if any(t is u for t in leaves for u in graph.leaves):
-                raise L.GrlHipError("linear_cross_entropy under graph capture: an eager loss of the same leaves, computed on the "
-                                    "default stream, is still alive; drop it (del loss) before the capture")
-    elif torch.cuda.current_stream(leaves[0].device).cuda_stream == 0:
-        ctx.graph = _Graph(leaves)
+        live = [r for graph in list(_ON_DEFAULT_STREAM) for r in graph.roots]
+        if live and _leaves(roots).keys() & _leaves(live).keys():
+            raise L.GrlHipError("linear_cross_entropy under graph capture: an eager loss of the same leaves, computed on the "
+                                "default stream, is still alive; drop it (del loss) before the capture")
+    elif torch.cuda.current_stream(tensors[0].device).cuda_stream == 0:
+        ctx.graph = _Graph(roots)
         _ON_DEFAULT_STREAM.add(ctx.graph)
 
 
@@ -132,7 +152,10 @@ def linear_cross_entropy(hidden, weight, target, bias=None, row_weight=None, ign
     Differentiable (once) with respect to hidden, weight and bias; the gradients have the operands' types.  Logits are never stored:
     the forward pass keeps one logsumexp per row, the backward pass recomputes them in pieces of the vocabulary.  With
     ``reduction="none"`` and no gradient this is the negative log-probability of single tokens (serving).  While a HIP graph is
-    captured, no eager loss over the same leaves from the default stream may be alive: such a call is refused."""
+    captured, no eager loss over the same leaves from the default stream may be alive: such a call is refused.
+
+    Types: 16-bit operands are multiplied as they are, fp32 ones at fp32's precision as long as they are above 2^-39 of their tensor's
+    largest entry (rows that do not count apart); the gradients' products hold operands down to 2^-38 of it."""
     if reduction not in _REDUCE:
         raise ValueError("reduction: expected 'none', 'mean' or 'sum', got %r" % (reduction,))
     if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1]:

@@ -385,12 +385,29 @@ def test_gpu_capture_beside_a_live_eager_loss_is_refused(monkeypatch):
             linear_cross_entropy(h, w, t)
         linear_cross_entropy(h, other, t).backward()       # the live loss of another stream
         linear_cross_entropy(h, w.detach(), t)             # no gradient, no graph
-        (2 * linear_cross_entropy(h, w * 1.0, t)).detach()    # w is no leaf of this call
+        for again in (lambda: linear_cross_entropy(h, w * 1.0, t), lambda: linear_cross_entropy(h * w[:1], w.detach(), t)):
+            with pytest.raises(L.GrlHipError, match="still alive"):
+                again()                                    # the leaf stands behind other operations
         loss.backward()
         del loss
         linear_cross_entropy(h, w, t).backward()
     torch.cuda.synchronize()
     assert elsewhere.requires_grad
+
+
+@pytest.mark.gpu
+def test_gpu_capture_beside_a_live_loss_of_a_batch_of_sequences_is_refused(monkeypatch):
+    """hidden of three dimensions is a leaf behind a view."""
+    h, w, t, _, _ = inputs(20, 64, 50, F32)
+    cube = h.view(4, 5, 64).requires_grad_()
+    loss = linear_cross_entropy(cube, w, t.view(4, 5), reduction="sum")
+    with monkeypatch.context() as m:
+        m.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+        with pytest.raises(L.GrlHipError, match="still alive"):
+            linear_cross_entropy(cube, w, t.view(4, 5), reduction="sum")
+        del loss
+        linear_cross_entropy(cube, w, t.view(4, 5), reduction="sum").backward()
+    torch.cuda.synchronize()
 
 
 @pytest.mark.gpu
