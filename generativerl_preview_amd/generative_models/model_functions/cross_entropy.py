@@ -152,7 +152,8 @@ def linear_cross_entropy(hidden, weight, target, bias=None, row_weight=None, ign
     Differentiable (once) with respect to hidden, weight and bias; the gradients have the operands' types.  Logits are never stored:
     the forward pass keeps one logsumexp per row, the backward pass recomputes them in pieces of the vocabulary.  With
     ``reduction="none"`` and no gradient this is the negative log-probability of single tokens (serving).  While a HIP graph is
-    captured, no eager loss over the same leaves from the default stream may be alive: such a call is refused.
+    captured, no eager loss over the same leaves from the default stream may be alive: such a call is refused
+    (graphs that other operations keep alive are not seen: PyTorch's own rule for them holds).
 
     Types: 16-bit operands are multiplied as they are, fp32 ones at fp32's precision as long as they are above 2^-39 of their tensor's
     largest entry (rows that do not count apart); the gradients' products hold operands down to 2^-38 of it."""
