@@ -568,7 +568,7 @@ typedef Tile<128, 128, 2, 2, 2> Orth128;       // 64 KiB
 typedef Tile<256, 256, 2, 4, 2> Orth256;       // 128 KiB
 constexpr int KINDS = 9, SIDE[KINDS] = {32, 32, 32, 64, 64, 96, 128, 128, 256}, BESIDE[KINDS] = {1, 2, 5, 1, 2, 1, 1, 2, 1};   // workgroups a CU
 constexpr double ALONE[KINDS] = {0.095, 0.106, 0.21, 0.245, 0.33, 0.47, 0.60, 0.67, 1.9};
-constexpr double FULL[KINDS] = {0.11, 0.083, 0.08, 0.25, 0.215, 0.60, 0.75, 0.68, 2.73};
+constexpr double FULL[KINDS] = {0.11, 0.083, 0.08, 0.265, 0.215, 0.60, 0.75, 0.68, 2.73};
 // Besides: what a tile costs whatever its length, shared by the workgroups beside each other; and the epilogue's 12 bytes an entry
 // at a CU's share of the memory, which hardly overlap with products (all tiles of a launch take the same time).
 constexpr double FIXED[KINDS] = {2.5, 2.5, 2.5, 0.8, 1.6, 0.8, 0.8, 1.6, 0.8}, EPILOGUE = 12 / 15e3;
