@@ -552,11 +552,9 @@ int check_coefficients(const char* who, float a, float b, float c, int steps) {
   return 0;
 }
 
-// The shapes of tiles.  Measured per K block of 32 (two pieces, 3 MFMAs), operands from beyond the L2 as the launch before left them:
-// ALONE, a tile on its CU, and FULL, the CU's time for one on a full chip.  us by kind in the order below:
-//   512 x 512 x 512: 4.0, 4.5, 5.6, 6.1, 7.5, -, 11.3, 12.5, 30;  1024 x 768 x 256: 7.4, 5.8, 4.6, 4.5, 5.0;
-//   1024 x 1024 x 1024: 17.8, 14.4, 12.1, 10.4, 12.8, -, 20, 23, 57;  1536 x 1536 x 4096: 63 (96), 77 (128K);
-//   2048 x 4096 x 2048: 225, -, -, 141, 110, -, 90, 87, 125;  8192 x 8192 x 2048: 774 (128), 698 (256: 1180 TFLOP/s of MFMAs).
+// The shapes of tiles.  Products of plain square operands by kind in the order below, us:
+//   512 x 512 x 512: 4.2, 4.6, 5.7, 6.2, 7.5, 9.4, 11.4, 12.5, 30;  1024 x 1024 x 1024: 18, 15, 12.5, 10.7, 13.3, 16.6, 20.5, 23.6, 57;
+//   2048 x 2048 x 1024: -, -, -, 38, -, 35, 25.4, 28.3, 61;  8192 x 8192 x 2048: 774 (128), 698 (256: 1180 TFLOP/s of MFMAs).
 typedef Tile<32, 32, 1, 1, 3, 4> Orth32K;      // 96 KiB, one a CU: three stages cover the latency of few tiles
 typedef Tile<32, 32, 1, 1, 2, 4> Orth32;       // 64 KiB, two a CU
 typedef Tile<32, 32, 1, 1, 2, 2> Orth32S;      // 32 KiB, five a CU: many short tiles
@@ -567,11 +565,13 @@ typedef Tile<128, 128, 2, 2, 2, 2> Orth128K;   // 128 KiB
 typedef Tile<128, 128, 2, 2, 2> Orth128;       // 64 KiB
 typedef Tile<256, 256, 2, 4, 2> Orth256;       // 128 KiB
 constexpr int KINDS = 9, SIDE[KINDS] = {32, 32, 32, 64, 64, 96, 128, 128, 256}, BESIDE[KINDS] = {1, 2, 5, 1, 2, 1, 1, 2, 1};   // workgroups a CU
-constexpr double ALONE[KINDS] = {0.095, 0.106, 0.21, 0.245, 0.33, 0.47, 0.60, 0.67, 1.9};
-constexpr double FULL[KINDS] = {0.11, 0.083, 0.08, 0.265, 0.215, 0.60, 0.75, 0.68, 2.73};
-// Besides: what a tile costs whatever its length, shared by the workgroups beside each other; and the epilogue's 12 bytes an entry
-// at a CU's share of the memory, which hardly overlap with products (all tiles of a launch take the same time).
-constexpr double FIXED[KINDS] = {2.5, 2.5, 2.5, 0.8, 1.6, 0.8, 0.8, 1.6, 0.8}, EPILOGUE = 12 / 15e3;
+// A launch, in us: ALONE is a K block of 32 (two pieces, 3 MFMAs) of a tile with its CU to itself, FULL the CU's time for one of a full chip,
+// FIXED what a tile costs whatever its length, shared by the workgroups beside each other, EPILOGUE an entry's stores and loads.
+// Fitted to the times of 28 groups of matrices (one of 128 x 128 to 24 of 1024 x 4096) with each kind in each of the three products in turn:
+// in all of them but one the kind that the rule takes is within 1.5 % of the best call, and in that one within 3 %; 18 other groups: 2 %, and 5 % in one.
+constexpr double ALONE[KINDS] = {0.096, 0.131, 0.26, 0.224, 0.333, 0.48, 0.584, 0.646, 1.58};
+constexpr double FULL[KINDS] = {0.104, 0.09, 0.093, 0.222, 0.212, 0.474, 0.641, 0.563, 2.24};
+constexpr double FIXED[KINDS] = {1.74, 1.46, 1.19, 1.79, 1.16, 0.88, 2.72, 3.17, 2.64}, EPILOGUE = 1.2e-3;
 
 int64_t tiles_of(const Parts& p, int stage, int side) {
   const int64_t tm = (p.mp + side - 1) / side, tn = (p.np + side - 1) / side;
