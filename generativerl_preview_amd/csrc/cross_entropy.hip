@@ -621,6 +621,7 @@ __global__ __launch_bounds__(256) void k_ce_join(Join a) {
     const int v = (b - a.blocks[0] - a.blocks[1]) * 256 + threadIdx.x;
     if (v >= a.cols) return;
     float s = 0.f;
+#pragma unroll 8
     for (int t = 0; t < a.btiles; ++t) s += a.bpart[(int64_t)t * a.cols + v];
     a.gb[v] = s;
     return;
@@ -631,6 +632,7 @@ __global__ __launch_bounds__(256) void k_ce_join(Join a) {
   const int64_t all = (int64_t)g.n * g.m, step = (int64_t)a.blocks[k] * 256;
   for (int64_t i = (int64_t)(k ? b - a.blocks[0] : b) * 256 + threadIdx.x; i < all; i += step) {
     float s = 0.f;
+#pragma unroll 8
     for (int p = 0; p < g.split; ++p) s += g.slots[p * all + i];
     const float row = g.scale ? g.scale[i / g.m] : 1.f;
     ((T*)g.out)[i] = g.scale && row == 0.f ? (T)0.f : (T)(s * f.f * f.f2 * row);
@@ -647,7 +649,7 @@ int grad_pieces(int elem) { return elem == GRLHIP_ELEM_BF16 ? 1 : 2; }
 typedef Tile<64, 64, 2, 2, 2, 2> Ce64;
 typedef Tile<128, 128, 2, 2, 2> Ce128;
 typedef Tile<256, 256, 2, 4, 2> Ce256;
-constexpr int KINDS = 3, SIDE[KINDS] = {64, 128, 256};
+constexpr int KINDS = 3, SIDE[KINDS] = {64, 128, 256}, BESIDE[KINDS] = {2, 2, 1};   // workgroups a CU
 constexpr double ALONE[2][KINDS] = {{0.30, 0.61, 1.28}, {0.33, 0.67, 1.9}}, FULL[2][KINDS] = {{0.21, 0.55, 1.91}, {0.22, 0.72, 2.73}};
 int64_t tiles_of(int64_t m, int64_t n, int k) { return up(m, SIDE[k]) / SIDE[k] * (up(n, SIDE[k]) / SIDE[k]); }
 // Time of a launch: its longest tile, or its tiles together on all CUs, in whole tiles a CU; `entry_ns` is a CU's time for one
@@ -676,8 +678,12 @@ struct Layout {
   // offsets
   int64_t scalars, hp, wp, ht, wt, d, dt, part, picked, sums, scale, bpart, hslots, wslots, bytes;
 };
-// Both gradients are one launch: the tiles and the parts of the sums that make it shortest.  A part costs writing and reading back
-// fp32 sums, 8 bytes an entry at 4 TB/s, and a second launch.
+// Both gradients are one launch, dH's (long) tiles first: the tiles and the parts of the sums that make it shortest.  A part costs writing
+// and reading back fp32 sums and a second launch.  The constants, us by pieces of D as above, are fitted to 70 calls (1 to 20 000 rows, 64
+// to 4096 features, 256 to 128 000 entries) with every kind and up to 32 parts of each sum: of 30 calls timed afterwards the rule's
+// choice was 2 % over the best on average and 15 % in the worst.
+constexpr double GRAD_ALONE[2][KINDS] = {{0.252, 0.684, 1.311}, {0.341, 0.691, 1.758}}, GRAD_FULL[2][KINDS] = {{0.15, 0.373, 1.152}, {0.184, 0.493, 1.645}};
+constexpr double GRAD_FIXED = 1.09, GRAD_ENTRY = 0.07e-3, TAIL = 0.74, JOIN = 1.5, JOIN_BYTES = 5.3e6;   // a tile; an entry of it; a join, its bytes a us
 void plan_gradients(Layout& l, const Shape& c, int64_t vp, int p) {
   const int64_t kb = p == 2 ? 32 : 64, kh = vp / kb, kw = l.np / kb;
   double best = 0;
@@ -686,10 +692,12 @@ void plan_gradients(Layout& l, const Shape& c, int64_t vp, int p) {
     for (int sh = 1; sh <= 32 && (sh == 1 || kh / sh >= 4); sh *= 2)
       for (int sw = 1; sw <= 32 && (sw == 1 || kw / sw >= 4); sw *= 2) {
         const double parts = (sh > 1 ? (double)sh * c.rows * c.hidden : 0) + (sw > 1 ? (double)sw * l.piece * c.hidden : 0);
-        const double cus = device_cus(), epilogue = SIDE[k] * SIDE[k] * 0.3e-3 + 0.8;
-        const double sum = th * sh * ((double)kh / sh * FULL[p - 1][k] + epilogue) + tw * sw * ((double)kw / sw * FULL[p - 1][k] + epilogue);
-        const double tiles = (double)(th * sh + tw * sw), longest = std::fmax((double)kh / sh, (double)kw / sw) * ALONE[p - 1][k] + epilogue;
-        const double us = (tiles <= cus ? longest : std::fmax(longest, sum / cus * std::ceil(tiles / cus) / (tiles / cus))) + (parts > 0 ? 4.0 + parts * 8 / 4e6 : 0);
+        const double cus = device_cus(), epilogue = SIDE[k] * SIDE[k] * GRAD_ENTRY + GRAD_FIXED, alone = GRAD_ALONE[p - 1][k], full = GRAD_FULL[p - 1][k];
+        const double one_h = (double)kh / sh * full + epilogue, one_w = (double)kw / sw * full + epilogue, tiles = (double)(th * sh + tw * sw);
+        // on a full chip the longest tile has others beside it, and the last ones leave some of the chip idle
+        const double longest = std::fmax((double)kh / sh, (double)kw / sw) * (tiles <= cus ? alone : std::fmax(alone, full * BESIDE[k])) + epilogue;
+        const double us = (tiles <= cus ? longest : std::fmax(longest, (th * sh * one_h + tw * sw * one_w) / cus + TAIL * one_w)) +
+                          (parts > 0 ? JOIN + parts * 8 / JOIN_BYTES : 0);
         if ((k == 0 && sh == 1 && sw == 1) || us < best) {
           best = us;
           l.kind_g = k;
@@ -822,7 +830,7 @@ template <class T> struct Operands { typedef T type; };
 template <> struct Operands<float> { typedef _Float16 type; };
 
 int join_blocks(const Grad& g) {
-  const int64_t blocks = ((int64_t)g.n * g.m + 1023) / 1024;
+  const int64_t blocks = ((int64_t)g.n * g.m + 255) / 256;   // an entry a thread while that is few blocks: all parts of all entries in flight
   return (int)(blocks > 4096 ? 4096 : blocks);
 }
 
