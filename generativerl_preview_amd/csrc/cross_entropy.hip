@@ -85,26 +85,33 @@ __global__ __launch_bounds__(256) void k_ce_absmax(View h, View w, Left left, Sc
   if (v.s1 == 1 && v.s0 == v.cols && ((size_t)v.p & 15) == 0) {   // dense: 16 bytes a thread
     const int64_t all = (int64_t)v.rows * v.cols, whole = all / E, step = (int64_t)n * 256;
     const vec* p = (const vec*)v.p;
+    const bool asked = is_h || left.bias;
+    const double inverse = 1.0 / v.cols;
     for (int64_t k = (int64_t)b * 256 + threadIdx.x; k < whole; k += 4 * step) {
       vec x[4];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) x[u] = p[k + u * step < whole ? k + u * step : k];
+      int row[4];
+      bool in[4];
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        float top = 0.f;
+        const int64_t at = k + u * step < whole ? k + u * step : k;
+        x[u] = p[at];
+        row[u] = (int)((double)(at * E) * inverse);   // off by one at most
+        if ((int64_t)row[u] * v.cols > at * E) --row[u];
+        else if ((int64_t)(row[u] + 1) * v.cols <= at * E) ++row[u];
+      }
 #pragma unroll
-        for (int e = 0; e < E; ++e) top = fmaxf(top, finite((float)x[u][e]));
-        if (top > m) {
-          const int64_t first = (k + u * step < whole ? k + u * step : k) * E;
-          int row = (int)(first / v.cols), col = (int)(first - (int64_t)row * v.cols);
-          bool in = counts(row);
+      for (int u = 0; u < 4; ++u) in[u] = !asked || counts(row[u]);
 #pragma unroll
-          for (int e = 0; e < E; ++e) {
-            if (in) m = fmaxf(m, finite((float)x[u][e]));
-            if (++col == v.cols && e + 1 < E) {
-              col = 0;
-              in = counts(++row < v.rows ? row : v.rows - 1);
-            }
+      for (int u = 0; u < 4; ++u) {
+        const int64_t at = k + u * step < whole ? k + u * step : k;
+        int col = (int)(at * E - (int64_t)row[u] * v.cols);
+        const bool one = !asked || col + E <= v.cols;   // all of it in one row
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          if (in[u]) m = fmaxf(m, finite((float)x[u][e]));
+          if (!one && ++col == v.cols && e + 1 < E) {
+            col = 0;
+            in[u] = counts(++row[u] < v.rows ? row[u] : v.rows - 1);
           }
         }
       }
