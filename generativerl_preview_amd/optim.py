@@ -210,7 +210,8 @@ def muon_step(params, grads, momentum_buffers, lr, momentum=0.95, nesterov=True,
         param = (1 - lr weight_decay) param - lr' orthogonalize(u)
     with lr' = lr sqrt(max(1, rows / cols)) for ``adjust_lr="original"`` and 0.2 lr sqrt(max(rows, cols)) for
     ``"match_rms_adamw"`` (updates of the size of Adam's).  Any strides; the three lists must not share memory.  ``lr`` and the
-    other numbers are read on the host: a captured graph keeps the ones it was captured with."""
+    other numbers are read on the host: a captured graph keeps the ones it was captured with.  The call counts as an in-place
+    operation on the parameters and buffers (their version counters move; a replay of a captured graph moves none)."""
     params, grads, bufs = list(params), list(grads), list(momentum_buffers)
     if not len(params) == len(grads) == len(bufs):
         raise ValueError("muon_step: %d parameters, %d gradients, %d momentum buffers" % (len(params), len(grads), len(bufs)))
@@ -239,6 +240,9 @@ def muon_step(params, grads, momentum_buffers, lr, momentum=0.95, nesterov=True,
                                          None if pd and gd and bd else _stride_array(grads, params, bufs), rates, len(params),
                                          momentum, int(nesterov), 1.0 - lr * weight_decay, int(steps), a, b, c, eps, _ptr(ws),
                                          ws.numel(), _stream(dev)))
+    # the library wrote behind torch's back: packed weight images are keyed on these counters, and autograd checks them for
+    # what it saved
+    torch.autograd.graph.increment_version(params + bufs)
 
 
 class FlatMuon(FlatAdam):
@@ -264,7 +268,7 @@ class FlatMuon(FlatAdam):
                 self.matrix_names.append(name)
                 chosen.append((p, off, cnt))
         views = lambda flat: [flat[off:off + cnt].view(p.shape) for p, off, cnt in chosen]  # noqa: E731
-        self._matrices = views(self.flat_params), views(self.fg.flat), views(self.exp_avg)
+        self._matrices = [p for p, _, _ in chosen], views(self.fg.flat), views(self.exp_avg)
         taken = {off for _, off, _ in chosen}
         self.ranges = []
         for p, off, cnt in sorted(self.fg.slices, key=lambda s: s[1]):

@@ -267,6 +267,47 @@ def test_gpu_flat_muon_replays_from_a_captured_graph():
     assert oa.step_count == ob.step_count == 5
 
 
+def _residual_net():
+    from generativerl_preview_amd.generative_models.intrinsic_model import IntrinsicModel
+    return IntrinsicModel(dict(t_encoder=dict(type="GaussianFourierProjectionTimeEncoder", args=dict(embed_dim=32, scale=1.0)),
+                               backbone=dict(type="TemporalSpatialResidualNet",
+                                             args=dict(hidden_sizes=[64, 32], input_dim=11, output_dim=9, t_dim=32)))).to(DEV)
+
+
+def _value_net():
+    from generativerl_preview_amd.rl_modules.value_network.value_network import VNetwork
+    return VNetwork(dict(backbone=dict(type="MultiLayerPerceptron", args=dict(hidden_sizes=[17, 64, 64], output_size=1, activation="relu")))).to(DEV)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("make,inputs", [(_residual_net, ((50,), (50, 11))), (_value_net, ((50, 17),))])
+def test_gpu_muon_step_of_a_networks_matrices_is_seen_by_its_next_forward_pass(make, inputs):
+    """The networks keep a packed image of their weights, which follows the parameters' version counters."""
+    torch.manual_seed(11)
+    net, fresh = make(), make()
+    x = [torch.rand(s, device=DEV) for s in inputs]
+    with torch.no_grad():
+        first = net(*x).clone()
+        matrices = [p for p in net.parameters() if p.dim() == 2 and p.requires_grad]
+        grads, bufs = [grad_like(*p.shape, seed=k) for k, p in enumerate(matrices)], [torch.zeros_like(p) for p in matrices]
+        versions = [t._version for t in (*matrices, *bufs)]
+        optim.muon_step(matrices, grads, bufs, lr=0.1)
+        assert all(t._version > v for t, v in zip((*matrices, *bufs), versions))
+        fresh.load_state_dict(net.state_dict())
+        second = net(*x)
+        assert torch.equal(second, fresh(*x)) and not torch.equal(second, first)
+
+
+@pytest.mark.gpu
+def test_gpu_a_weight_stepped_between_forward_and_backward_is_noticed():
+    from generativerl_preview_amd.generative_models.model_functions import linear_cross_entropy
+    w, h = torch.nn.Parameter(torch.randn(40, 16, device=DEV)), torch.randn(8, 16, device=DEV)
+    loss = linear_cross_entropy(h, w, torch.arange(8, device=DEV))
+    optim.muon_step([w], [grad_like(40, 16)], [torch.zeros(40, 16, device=DEV)], lr=0.1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
 # ------------------------------------------------------------------------------------------------- refusals, on the CPU
 def test_refusals_of_the_python_calls():
     m = torch.randn(4, 5)
