@@ -42,11 +42,11 @@ __device__ __forceinline__ float scale_of(float most) {
   e = e < -100 ? -100 : e;
   return __builtin_ldexpf(1.f, 13 - e);
 }
-// a power of two that no gradient factor passes
+// a power of two that no gradient factor passes; not below 2^-112, so that DSCALE over it is a number too
 __device__ __forceinline__ float ceil_of(float most) {
   if (most == 0.f) return 1.f;
   const int e = __builtin_amdgcn_frexp_expf(most);
-  return __builtin_ldexpf(1.f, e > 127 ? 127 : e);
+  return __builtin_ldexpf(1.f, e > 127 ? 127 : e < -112 ? -112 : e);
 }
 __device__ __forceinline__ float finite(float v) { return __builtin_isfinite(v) ? fabsf(v) : 0.f; }
 __device__ __forceinline__ float wave_max(float m) {

@@ -303,6 +303,28 @@ def test_gpu_fp32_operands_of_any_magnitude(scale):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_gpu_tiny_gradients_of_the_rows(dtype):
+    """Row weights or an upstream gradient far below 2^-114: the gradients are the same ones, smaller by that power of two, down
+    to where the type's own numbers end (half its smallest one, scaled back)."""
+    h, w, t, b, rw = inputs(90, 64, 200, dtype, seed=31, weights=True)
+    leaves = [h.requires_grad_(), w.requires_grad_(), b.requires_grad_()]
+    out = oracle(h, w, t, b, rw, "sum")
+    tiny = 2.0 ** -118
+    end = {F32: 2.0 ** -150, BF16: 2.0 ** -134, F16: 2.0 ** -25}
+    for case in range(3):
+        if case == 0:
+            loss, up = linear_cross_entropy(h, w, t, bias=b, row_weight=rw * tiny, reduction="sum"), None
+            near(loss.detach().double() / tiny, "total", out)
+        else:
+            loss = linear_cross_entropy(h, w, t, bias=b, row_weight=rw, reduction="sum" if case == 1 else "none")
+            up = torch.full_like(loss, tiny)
+        for g, name, kind in zip(torch.autograd.grad(loss, leaves, grad_outputs=up), ("dh", "dw", "db"), (dtype, dtype, F32)):
+            want, tol = out[name]
+            near(g.double() / tiny, name, {name: (want, tol + end[kind] / tiny)})
+
+
+@pytest.mark.gpu
 def test_gpu_gradient_matches_differences():
     """Central differences of the loss along a direction: (f(x + s d) - f(x - s d)) / 2 s is off by s^2 f''' / 6 and by the
     loss' own rounding over s; at s = 2^-6, |f'''| <= 1 and a loss of about 7 to 2^-21 that is 4e-5 + 2e-4."""
