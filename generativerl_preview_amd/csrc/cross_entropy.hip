@@ -136,8 +136,7 @@ __global__ __launch_bounds__(256) void k_ce_absmax(View h, View w, Left left, Sc
 
 // A view -> operands: as it stands (n: rows of the view, type E) and transposed (t: its columns, fp16), either may be null; columns
 // beyond the view and up to the pitch become zeros.  fp32: two scaled fp16 pieces both ways.  bf16 transposed: scaled.  A row that
-// does not count becomes zeros: whatever it holds must not reach a sum over rows; so do the finite entries of a masked row of the weight,
-// which the scale does not know.
+// does not count becomes zeros: whatever it holds must not reach a sum over rows; so does a masked row of the weight, whose D is 0.
 struct Job {
   View v;
   void* n; int64_t n_cols;
@@ -223,7 +222,7 @@ __global__ __launch_bounds__(256) void k_ce_pack(Job h, Job w, Scale g, Left lef
     float x = 0.f;
     if (i0 + i < a.v.rows && j0 + j < a.v.cols) {
       if (!a.mask || row_counts(left, i0 + i)) x = (float)((const T*)a.v.p)[(int64_t)(i0 + i) * a.v.s0 + (int64_t)(j0 + j) * a.v.s1];
-      if (masked(a.bias, i0 + i) && __builtin_isfinite(x)) x = 0.f;
+      if (masked(a.bias, i0 + i)) x = 0.f;
     }
     tile[i][j] = TWO ? x * f : x;
   }
@@ -271,8 +270,9 @@ __device__ __forceinline__ void logits_of(const Logits& a, f32x16 (&acc)[TN], in
     for (int r = 0; r < 16; ++r) {
       const int m = mb + 8 * (r >> 2) + 4 * h + (r & 3);
       const float b = a.bias[m < a.cols ? m : a.cols - 1];
+      // a masked entry is -inf whatever its product came to: inf and NaN do not become -inf by adding it
 #pragma unroll
-      for (int x = 0; x < TN; ++x) acc[x][r] += b;
+      for (int x = 0; x < TN; ++x) acc[x][r] = b == -INFINITY ? b : acc[x][r] + b;
     }
 }
 

@@ -143,9 +143,10 @@ def linear_cross_entropy(hidden, weight, target, bias=None, row_weight=None, ign
     """Cross entropy of ``softmax(hidden @ weight.T + bias)`` at ``target``.
 
     ``hidden`` (..., features) and ``weight`` (vocabulary, features): fp32, bf16 or fp16, of one type, any strides;
-    ``target`` (...): int64 (or int32); ``bias`` (vocabulary,): any floating type, -inf masks an action; ``row_weight``
-    (...): a factor of every row's loss (an advantage weight), no gradient is taken to it.  Rows whose target is ``ignore_index`` or
-    whose weight is 0 (padding) contribute nothing, whatever their hidden row holds; any other target outside the vocabulary gives NaN.
+    ``target`` (...): int64 (or int32); ``bias`` (vocabulary,): any floating type, -inf masks an action, whatever its row of the
+    weight holds; ``row_weight`` (...): a factor of every row's loss (an advantage weight), no gradient is taken to it.  Rows whose
+    target is ``ignore_index`` or whose weight is 0 (padding) contribute nothing, whatever their hidden row holds; any other target
+    outside the vocabulary gives NaN.
     ``reduction``: ``"none"`` (losses of target's shape), ``"sum"``, or ``"mean"`` -- the weighted sum over the number of rows
     that are not ignored (0 when there are none).  The loss is fp32.
 

@@ -382,7 +382,7 @@ typedef enum { GRLHIP_REDUCE_NONE = 0, GRLHIP_REDUCE_MEAN = 1, GRLHIP_REDUCE_SUM
  *   largest[2] = largest finite magnitudes of hidden and weight, in rows that count and are not masked, written for GRLHIP_ELEM_F32 only (the backward call may take
  *   them instead of reading the operands once more); may be NULL.
  * hidden [rows][features], weight [vocab][features]: element type `elem`, element strides {row, column} in HOST arrays (NULL:
- * dense).  bias [vocab] fp32 or NULL; -inf masks an entry, whatever finite numbers its row of the weight holds.  target [rows] int64; row_weight [rows] fp32 or NULL (1).
+ * dense).  bias [vocab] fp32 or NULL; -inf masks an entry, whatever its row of the weight holds.  target [rows] int64; row_weight [rows] fp32 or NULL (1).
  * A row whose target is ignore_index or whose weight is 0 has loss 0 and contributes nothing, whatever its hidden row holds.  Any other
  * target outside [0, vocab): loss and gradients NaN.  A row with every entry masked: NaN.
  * rows, features, vocab: 1 to 2^20, 2^16, 2^21, and at most 2^34 entries of hidden and of weight.  Results repeat bit for bit.  Workspace: grlhip_linear_ce_workspace_bytes for the

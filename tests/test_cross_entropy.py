@@ -219,6 +219,30 @@ def test_gpu_large_numbers_in_padding_cost_the_others_nothing(features, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("features", [64, 128, 65])
+def test_gpu_masked_entries_may_hold_anything(features, dtype):
+    """The type's largest numbers, whose products leave fp32's range, infinities and NaN in masked rows of the weight reach nothing, whether
+    the weight is read where it lies (16-bit rows of whole K blocks) or laid out anew."""
+    h, w, t, b, rw = inputs(100, features, 300, dtype, seed=33)
+    b[[4, 299]] = -math.inf
+    t[(t == 4) | (t == 299)] = 3
+    b[3] = 0.0
+    signs = torch.where(torch.arange(features, device=DEV) % 2 == 0, 1.0, -1.0)
+    results = []
+    for fill in (0.0, torch.finfo(dtype).max, math.inf, math.nan):
+        x, y, bias = h.clone().requires_grad_(), w.clone(), b.clone().requires_grad_()
+        y[[4, 299]] = (signs * fill if math.isfinite(fill) else signs + fill).to(dtype)
+        y.requires_grad_()
+        loss = linear_cross_entropy(x, y, t, bias=bias, row_weight=rw)
+        results.append([loss.detach(), *torch.autograd.grad(loss, [x, y, bias])])
+    for got in results:
+        assert all(bool(g.isfinite().all()) for g in got)
+        assert all(torch.equal(g, want) for g, want in zip(got, results[0]))
+    near(results[0][0], "total", oracle(h, w, t, b, rw, "mean"))
+
+
+@pytest.mark.gpu
 def test_gpu_all_rows_ignored_and_no_rows():
     h, w, t, b, rw = inputs(40, 64, 90, BF16)
     t.fill_(-100)
