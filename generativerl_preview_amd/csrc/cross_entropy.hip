@@ -35,18 +35,19 @@ __host__ __device__ inline int64_t up(int64_t v, int64_t m) { return (v + m - 1)
 // What the launches share: largest finite magnitudes of hidden, weight and the rows' gradients, by block and joined.
 struct Scalars { float h, w; float hpart[HMAX], wpart[WMAX], gpart[GMAX]; };
 
-// the power of two that brings the largest magnitude to 2^13..2^14; 1 for nothing but zeros
-__device__ __forceinline__ float scale_of(float most) {
-  if (most == 0.f) return 1.f;
-  int e = __builtin_amdgcn_frexp_expf(most) - 1;
-  e = e < -100 ? -100 : e;
-  return __builtin_ldexpf(1.f, 13 - e);
+// 13 - e: the exponent of the power of two that brings the largest magnitude to 2^13..2^14; 0 for nothing but zeros.  Scales are undone by the
+// sum of their exponents: a product of one scale's reciprocal with the sum may leave fp32's range where the result does not.
+__device__ __forceinline__ int scale_exponent(float most) {
+  if (most == 0.f) return 0;
+  const int e = __builtin_amdgcn_frexp_expf(most) - 1;
+  return 13 - (e < -100 ? -100 : e);
 }
-// a power of two that no gradient factor passes; not below 2^-112, so that DSCALE over it is a number too
-__device__ __forceinline__ float ceil_of(float most) {
-  if (most == 0.f) return 1.f;
+__device__ __forceinline__ float scale_of(float most) { return __builtin_ldexpf(1.f, scale_exponent(most)); }
+// of a power of two that no gradient factor passes; not below -112, so that 2^14 over it is a number too
+__device__ __forceinline__ int ceil_exponent(float most) {
+  if (most == 0.f) return 0;
   const int e = __builtin_amdgcn_frexp_expf(most);
-  return __builtin_ldexpf(1.f, e > 127 ? 127 : e < -112 ? -112 : e);
+  return e > 127 ? 127 : e < -112 ? -112 : e;
 }
 __device__ __forceinline__ float finite(float v) { return __builtin_isfinite(v) ? fabsf(v) : 0.f; }
 __device__ __forceinline__ float wave_max(float m) {
@@ -261,10 +262,12 @@ struct Logits {
 
 // The accumulators of 32 rows of the tile (vocabulary entries from mb on) become z, in place.
 template <int P, int TN>
-__device__ __forceinline__ void logits_of(const Logits& a, f32x16 (&acc)[TN], int mb, int h, float fh, float fw) {
+__device__ __forceinline__ void logits_of(const Logits& a, f32x16 (&acc)[TN], int mb, int h, int undo) {
   if (P == 2)
 #pragma unroll
-    for (int x = 0; x < TN; ++x) acc[x] = acc[x] * fh * fw;   // one at a time: their product may leave fp32's range
+    for (int x = 0; x < TN; ++x)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[x][r] = __builtin_ldexpf(acc[x][r], undo);
   if (a.bias)
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
@@ -288,13 +291,13 @@ __global__ __launch_bounds__(C::THREADS, C::LDS > 81920 ? C::THREADS / 256 : C::
   if (!product<T, P, C>(a.w.p + m0 * a.w.pitch, a.w.pitch, a.cols - m0, a.h.p + n0 * a.h.pitch, a.h.pitch, a.rows - n0, a.nkb, lds, acc)) return;
   const Lane L = lane_of();
   const int wm = L.wave / C::WN, wn = L.wave % C::WN;
-  const float fh = P == 2 ? 1.f / scale_of(a.s->h) : 1.f, fw = P == 2 ? 1.f / scale_of(a.s->w) : 1.f;
+  const int undo = P == 2 ? -scale_exponent(a.s->h) - scale_exponent(a.s->w) : 0;
   float* tops = (float*)lds;                  // [WM][BN] maxima, then sums
   float* sums = tops + C::WM * C::BN;
 #pragma unroll
   for (int y = 0; y < C::TM; ++y) {
     const int mb = m0 + (wm * C::TM + y) * 32;
-    logits_of<P>(a, acc[y], mb, L.h, fh, fw);
+    logits_of<P>(a, acc[y], mb, L.h, undo);
     if (mb + 32 > a.cols)
 #pragma unroll
       for (int r = 0; r < 16; ++r)
@@ -435,7 +438,8 @@ __global__ __launch_bounds__(256) void k_ce_total(Finish a) {
   }
 }
 
-constexpr float DSCALE = 16384.f;   // D lies in [-2^14, 2^14]
+constexpr int DBITS = 14;
+constexpr float DSCALE = 1 << DBITS;   // D lies in [-2^14, 2^14]
 
 // N: pieces of D
 template <class T, int P, int N, class C>
@@ -448,8 +452,8 @@ __global__ __launch_bounds__(C::THREADS, C::LDS > 81920 ? C::THREADS / 256 : C::
   if (!product<T, P, C>(a.w.p + m0 * a.w.pitch, a.w.pitch, a.cols - m0, a.h.p + n0 * a.h.pitch, a.h.pitch, a.rows - n0, a.nkb, lds, acc)) return;
   const Lane L = lane_of();
   const int wm = L.wave / C::WN, wn = L.wave % C::WN;
-  const float fh = P == 2 ? 1.f / scale_of(a.s->h) : 1.f, fw = P == 2 ? 1.f / scale_of(a.s->w) : 1.f;
-  const float per = DSCALE / ceil_of(largest_gradient(a.s));
+  const int undo = P == 2 ? -scale_exponent(a.s->h) - scale_exponent(a.s->w) : 0;
+  const float per = __builtin_ldexpf(1.f, DBITS - ceil_exponent(largest_gradient(a.s)));
   unsigned* patch = (unsigned*)(lds + L.wave * PATCH);
   float* bsum = (float*)(lds + C::WAVES * PATCH);   // [WN][BM]
   float lse[C::TN], g[C::TN];
@@ -464,7 +468,7 @@ __global__ __launch_bounds__(C::THREADS, C::LDS > 81920 ? C::THREADS / 256 : C::
 #pragma unroll
   for (int y = 0; y < C::TM; ++y) {
     const int mb = m0 + (wm * C::TM + y) * 32;
-    logits_of<P>(a, acc[y], mb, L.h, fh, fw);
+    logits_of<P>(a, acc[y], mb, L.h, undo);
     float bs[16];
 #pragma unroll
     for (int r = 0; r < 16; ++r) bs[r] = 0.f;
@@ -535,16 +539,15 @@ struct Grad {
   int add;                  // to what the slots hold
   void* out;                // dense rows
   const float* scale;       // per row, or null
-  int by_w;                 // the operands' factors: W's (dH) or hidden's and the gradient's (dW)
+  int by_w;                 // the operands' scales: W's (dH) or hidden's and the gradient's (dW)
 };
 struct Grads { Grad g[2]; const Scalars* s; };   // one launch: dH's tiles, then dW's
-struct Factor { float f, f2; };
 template <class T>
-__device__ __forceinline__ Factor factor_of(const Grad& g, const Scalars* s) {
-  Factor f{1.f / DSCALE, 1.f};
-  if (!__is_same(T, _Float16)) f.f *= 1.f / scale_of(g.by_w ? s->w : s->h);
-  if (!g.by_w) f.f2 = ceil_of(largest_gradient(s));
-  return f;
+__device__ __forceinline__ int undo_of(const Grad& g, const Scalars* s) {
+  int e = -DBITS;
+  if (!__is_same(T, _Float16)) e -= scale_exponent(g.by_w ? s->w : s->h);
+  if (!g.by_w) e += ceil_exponent(largest_gradient(s));
+  return e;
 }
 template <class T, int P, class C>
 __global__ __launch_bounds__(C::THREADS, C::LDS > 81920 ? C::THREADS / 256 : C::THREADS / 128) void k_ce_grad(Grads both) {
@@ -562,7 +565,7 @@ __global__ __launch_bounds__(C::THREADS, C::LDS > 81920 ? C::THREADS / 256 : C::
                                g.b.pitch, g.n - n0, k1 - k0, lds, acc)) return;
   const Lane L = lane_of();
   const int wm = L.wave / C::WN, wn = L.wave % C::WN;
-  const Factor f = factor_of<T>(g, both.s);
+  const int undo = undo_of<T>(g, both.s);
   float* patch = (float*)(lds + L.wave * PATCH);
   const bool to_slots = g.slots != nullptr;
   // whole 16-byte stores where the rows allow them
@@ -601,7 +604,7 @@ __global__ __launch_bounds__(C::THREADS, C::LDS > 81920 ? C::THREADS / 256 : C::
       const float r = g.scale ? g.scale[n] : 1.f;
       T w[16];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) w[i] = g.scale && r == 0.f ? (T)0.f : (T)(v[i] * f.f * f.f2 * r);
+      for (int i = 0; i < 16; ++i) w[i] = g.scale && r == 0.f ? (T)0.f : (T)(__builtin_ldexpf(v[i], undo) * r);
       T* o = (T*)g.out + (int64_t)n * g.m + m;
       if (wide && m + 16 <= g.m) {
         constexpr int E = 16 / sizeof(T);
@@ -635,14 +638,14 @@ __global__ __launch_bounds__(256) void k_ce_join(Join a) {
   }
   const int k = b >= a.blocks[0];
   const Grad& g = a.both.g[k];
-  const Factor f = factor_of<T>(g, a.both.s);
+  const int undo = undo_of<T>(g, a.both.s);
   const int64_t all = (int64_t)g.n * g.m, step = (int64_t)a.blocks[k] * 256;
   for (int64_t i = (int64_t)(k ? b - a.blocks[0] : b) * 256 + threadIdx.x; i < all; i += step) {
     float s = 0.f;
 #pragma unroll 8
     for (int p = 0; p < g.split; ++p) s += g.slots[p * all + i];
     const float row = g.scale ? g.scale[i / g.m] : 1.f;
-    ((T*)g.out)[i] = g.scale && row == 0.f ? (T)0.f : (T)(s * f.f * f.f2 * row);
+    ((T*)g.out)[i] = g.scale && row == 0.f ? (T)0.f : (T)(__builtin_ldexpf(s, undo) * row);
   }
 }
 

@@ -327,6 +327,31 @@ def test_gpu_fp32_operands_of_any_magnitude(scale):
 
 
 @pytest.mark.gpu
+def test_gpu_large_logits_of_operands_at_the_ends_of_the_range():
+    """Logits of 5e4 from hidden of 1e35: what the operands were multiplied by is undone at once, not one factor after the other."""
+    h, w, t, b, rw = inputs(64, 96, 150, F32, seed=9)
+    h, w = (h * 1e35).requires_grad_(), (w * 1e-31).requires_grad_()
+    loss = linear_cross_entropy(h, w, t, bias=b, row_weight=rw, reduction="none")
+    near(loss.detach(), "losses", oracle(h, w, t, b, rw, "none"))
+    assert all(bool(g.isfinite().all()) for g in torch.autograd.grad(loss.sum() / 64, [h, w]))
+
+
+@pytest.mark.gpu
+def test_gpu_sums_over_many_rows_of_large_numbers():
+    """40 000 rows of 1e35: their sum before the mean's factor passes fp32's range, the gradient does not."""
+    n, k, v = 40000, 8, 8
+    h = torch.full((n, k), 1e35, device=DEV)
+    w = torch.linspace(-1, 1, v, device=DEV).unsqueeze(1).expand(v, k).contiguous() * 1e-35
+    t = torch.zeros(n, dtype=torch.int64, device=DEV)
+    w.requires_grad_()
+    loss = linear_cross_entropy(h, w, t)
+    out = oracle(h, w, t, None, None, "mean")
+    near(loss.detach(), "total", out)
+    (g,) = torch.autograd.grad(loss, [w])
+    near(g, "dw", out)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES)
 def test_gpu_tiny_gradients_of_the_rows(dtype):
     """Row weights or an upstream gradient far below 2^-114: the gradients are the same ones, smaller by that power of two, down
