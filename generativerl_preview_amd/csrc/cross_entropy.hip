@@ -668,9 +668,9 @@ double launch_us(double tiles, double kb, int p, int k, double entry_ns) {
   const double cus = device_cus(), epilogue = SIDE[k] * SIDE[k] * entry_ns * 1e-3 + 0.8;
   return tiles <= cus ? kb * ALONE[p - 1][k] + epilogue : std::ceil(tiles / cus) * (kb * FULL[p - 1][k] + epilogue);
 }
-int kind_for(int64_t m, int64_t n, int64_t kb, int p, double entry_ns) {
-  int best = 0;
-  for (int k = 1; k < KINDS; ++k)
+int kind_for(int64_t m, int64_t n, int64_t kb, int p, double entry_ns, int from = 0) {
+  int best = from;
+  for (int k = from + 1; k < KINDS; ++k)
     if (launch_us((double)tiles_of(m, n, k), (double)kb, p, k, entry_ns) < launch_us((double)tiles_of(m, n, best), (double)kb, p, best, entry_ns)) best = k;
   return best;
 }
@@ -734,7 +734,11 @@ Layout layout_of(const Shape& c, bool direct_h, bool direct_w, bool backward, bo
   l.piece = up((c.vocab + l.pieces_n - 1) / l.pieces_n, 256);
   if (l.piece > c.vocab) l.piece = c.vocab;
   l.pieces_n = (c.vocab + l.piece - 1) / l.piece;
-  l.kind_z = kind_for(l.piece, c.rows, l.kp * per / KBLOCK, p, backward ? d_ns(grad_pieces(c.elem)) : FORWARD_NS);
+  // The backward pass takes its logits' exponentials against the forward pass' logsumexp: both need the same bits (a saturated row of logits of
+  // 1e5 has half steps of 2^-8).  The 64-wide tiles add up K in two parts, the others in one: what the forward pass takes decides for both.
+  const int64_t kb = l.kp * per / KBLOCK;
+  if (!backward) l.kind_z = kind_for(l.piece, c.rows, kb, p, FORWARD_NS);
+  else if (layout_of(c, direct_h, direct_w, false, false).kind_z > 0) l.kind_z = kind_for(l.piece, c.rows, kb, p, d_ns(grad_pieces(c.elem)), 1);
   const int side = SIDE[l.kind_z];
   int64_t at = 0;
   auto take = [&](int64_t bytes) { const int64_t o = at; at += up(bytes, 256); return o; };

@@ -373,6 +373,33 @@ def test_gpu_tiny_gradients_of_the_rows(dtype):
             near(g.double() / tiny, name, {name: (want, tol + end[kind] / tiny)})
 
 
+# by the rules of the tiles alone, the forward pass would take wide tiles here and the backward pass, whose epilogue is longer, 64-wide ones,
+# which add up K in two parts: fp32 and fp16, bf16 and fp16
+SATURATED = [(300, 200, 9000), (174, 70, 34497)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("size", SATURATED)
+def test_gpu_a_saturated_row_has_no_gradient(size, dtype):
+    """Logits of 1e5 whose target wins by far: softmax - onehot is 0, as long as the logits of the backward pass are the bits of
+    the forward pass'; one half step of 1e5 in fp32 is 2^-8, and exp of that is no 1 any more."""
+    n, k, v = size
+    gen = torch.Generator().manual_seed(51)
+    h = torch.randn(n, k, generator=gen).to(dtype).to(DEV)
+    w = (torch.randn(v, k, generator=gen) * 3e4 / math.sqrt(k)).to(dtype).to(DEV)
+    z = h.double() @ w.double().t()
+    two = z.topk(2, dim=1)
+    t = two.indices[:, 0].contiguous()
+    t[two.values[:, 0] - two.values[:, 1] < 100.0] = -100       # the error of a logit of 1e5 is 1e5 (k / 16 + 16) 2^-24 < 1
+    assert int((t != -100).sum()) > n // 2
+    leaves = [h.requires_grad_(), w.requires_grad_()]
+    loss = linear_cross_entropy(*leaves, t)
+    assert float(loss.detach()) == 0.0
+    for g in torch.autograd.grad(loss, leaves):
+        assert not g.any()
+
+
 @pytest.mark.gpu
 def test_gpu_gradient_matches_differences():
     """Central differences of the loss along a direction: (f(x + s d) - f(x - s d)) / 2 s is off by s^2 f''' / 6 and by the
