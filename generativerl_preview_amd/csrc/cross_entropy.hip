@@ -205,14 +205,14 @@ __global__ __launch_bounds__(256) void k_ce_pack(Job h, Job w, Scale g, Left lef
   const Job& a = is_h ? h : w;
   const int b = is_h ? blockIdx.x : blockIdx.x - h.blocks;
   float f = 1.f;
-  if (SCALED) {
+  if (SCALED && (TWO || a.t)) {   // 16-bit operands that stand as they are have no scale
     float most;
     if (known) most = largest[is_h ? 0 : 1];   // the forward call's
     else most = is_h ? block_max(threadIdx.x < HMAX ? s->hpart[threadIdx.x] : 0.f, sh) : block_max(s->wpart[threadIdx.x], sh);
     f = scale_of(most);
     if (b == 0 && threadIdx.x == 0) {
       (is_h ? s->h : s->w) = most;
-      if (largest && !known) largest[is_h ? 0 : 1] = most;
+      if (TWO && largest && !known) largest[is_h ? 0 : 1] = most;
     }
   }
   const int across = (a.v.cols + 63) / 64, i0 = b / across * 64, j0 = b % across * 64, tid = threadIdx.x;

@@ -541,6 +541,33 @@ def test_gpu_a_head_over_a_network_trains_with_flat_muon():
         assert bool(head.isfinite().all())
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_gpu_c_calls_write_the_magnitudes_as_the_header_says(dtype):
+    """`largest`: by the forward call, for fp32 only."""
+    h, w, t, _, _ = inputs(70, 100, 130, dtype, seed=17, bias=False, weights=False, ignored=0.1)
+    lib, elem = L.lib(), {F32: L.ELEM_F32, BF16: L.ELEM_BF16, F16: L.ELEM_F16}[dtype]
+    f = lambda n: torch.full((n,), -7.0, device=DEV)  # noqa: E731
+    losses, lse, total, count, largest, gh = f(70), f(70), f(1), f(1), f(4), torch.empty_like(h)
+    one = torch.ones((), device=DEV)
+    stream = ctypes.c_void_p(torch.cuda.current_stream(DEV).cuda_stream)
+    spaces = []
+    for back in (0, 1):
+        need = lib.grlhip_linear_ce_workspace_bytes(h.data_ptr(), None, w.data_ptr(), None, 70, 100, 130, elem, back)
+        spaces.append(torch.full((need,), 0x3f, dtype=torch.uint8, device=DEV))
+    args = (h.data_ptr(), None, w.data_ptr(), None, None, t.data_ptr(), -100, None, 70, 100, 130, elem, L.REDUCE_MEAN)
+    L.check(lib.grlhip_linear_ce_forward(*args, losses.data_ptr(), lse.data_ptr(), total.data_ptr(), count.data_ptr(), largest.data_ptr(),
+                                         spaces[0].data_ptr(), spaces[0].numel(), stream))
+    want = torch.tensor([float(h[t != -100].abs().max()), float(w.abs().max()), -7.0, -7.0]) if dtype == F32 else torch.full((4,), -7.0)
+    assert torch.equal(largest.cpu(), want)
+    L.check(lib.grlhip_linear_ce_backward(*args, lse.data_ptr(), count.data_ptr(), largest.data_ptr(), one.data_ptr(), 0, gh.data_ptr(), None, None,
+                                          spaces[1].data_ptr(), spaces[1].numel(), stream))
+    assert torch.equal(largest.cpu(), want)
+    out = oracle(h, w, t, None, None, "mean")
+    near(total[0], "total", out)
+    near(gh, "dh", out)
+
+
 # ------------------------------------------------------------------------------------------------- refusals, on the CPU
 def test_refusals_of_the_python_call():
     h, w, t = torch.randn(4, 8), torch.randn(10, 8), torch.zeros(4, dtype=torch.int64)
