@@ -13,7 +13,7 @@ LIB_PATH = os.environ.get("GRLHIP_LIB") or os.path.join(_HERE, "libgrlhip.so")
 
 MAX_HIDDEN = 8
 F32, BF16 = 0, 1
-ELEM_F32, ELEM_BF16, ELEM_F16 = 0, 1, 2
+ELEM_F32, ELEM_BF16, ELEM_F16, ELEM_SCALES = 0, 1, 2, 0x100
 REDUCE_NONE, REDUCE_MEAN, REDUCE_SUM = 0, 1, 2
 NET_RESNET, NET_CONCAT_MLP, NET_QNET = 0, 1, 2
 COEF_STRIDE = 12
@@ -82,6 +82,7 @@ PROTOTYPES = {
     "grlhip_muon_step": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i32, ctypes.c_double, ctypes.c_int, _f, _i32, _f, _f, _f, _f,
                                         _vp, _sz, _vp]),
     "grlhip_linear_ce_workspace_bytes": (_sz, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, ctypes.c_int, ctypes.c_int]),
+    "grlhip_linear_ce_scales_bytes": (_sz, [_i64, _i64]),
     "grlhip_linear_ce_forward": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _i64, _i64, ctypes.c_int,
                                                 ctypes.c_int, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "grlhip_linear_ce_backward": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _i64, _i64, ctypes.c_int,

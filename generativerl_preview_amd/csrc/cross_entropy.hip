@@ -8,11 +8,15 @@
 // flops; the workspace holds D of one piece.  Recomputing z costs a third more products than keeping it would, and N V
 // floats less memory.
 //
-// Precision.  z: 16-bit operands are used as they are, fp32 ones as two fp16 pieces a value (gemm_core.hip.inc), scaled by a
-// power of two per tensor that brings the largest entry to 2^13..2^14: what is lost of a value is at most 2^-23 of it or 2^-39 of the
-// largest.  D lies in [-1, 1] and is held times 2^14 in fp16: one piece for bf16 operands (off by 2^-11 at most, an eighth of the
-// gradients' own rounding; held in bf16 it would be off by as much as that), two for fp16 and fp32 (one would be off by as much as an fp16
-// gradient's own rounding).  W^T and hidden^T beside it are fp16 for that: bf16 entries fit its 11 bits exactly, scaled as above.  All sums are fp32 or wider and taken in a fixed order: results repeat bit for bit.
+// Precision.  z: 16-bit operands are used as they are, fp32 ones as two fp16 pieces a value (gemm_core.hip.inc), each row of hidden and of the
+// weight scaled by a power of two of its own that brings its largest entry to 2^13..2^14: what is lost of a value is at most 2^-23 of it or 2^-38
+// of the largest of its row.  D lies in [-1, 1] and is held times 2^14 in fp16: one piece for bf16 operands (off by 2^-11 at most, an eighth
+// of the gradients' own rounding; held in bf16 it would be off by as much as that), two for fp16 and fp32 (one would be off by as much as an
+// fp16 gradient's own rounding; two lose 2^-22 of it or 2^-39).  W^T and hidden^T beside it are fp16 for that: fp16 entries stand as they are, bf16
+// ones fit its 11 bits exactly (down to 2^-28 of the tensor's largest, to which they are scaled), fp32 ones are two pieces.  These products sum over
+// rows, so that fp32 rows cannot each have their scale there: a row whose largest entry is 2^d below the tensor's stands 2^(d - d/2) below, and D
+// beside it is divided by 2^(d/2).  Its entries lose up to 2^(d/2 - 38) of its largest, D up to 2^(d/2 - 39): fp32's 2^-24 for rows up to
+// 2^28 apart.  All sums are fp32 or wider and taken in a fixed order: results repeat bit for bit.
 #include <cmath>
 #include <string>
 
@@ -29,11 +33,14 @@ constexpr int64_t MAX_ROWS = 1 << 20, MAX_VOCAB = 1 << 21, MAX_HIDDEN = 1 << 16;
 // entries of D in one piece of the vocabulary: 512 MiB of D both ways round beside bf16 operands.  8192 x 2048 x 65536 in 8.26 ms; with pieces
 // of 2^26 8.34, of 2^25 9.14 (each adds to all of dH)
 constexpr int64_t PIECE = 1ll << 27;
-constexpr int HMAX = 64, WMAX = 256, GMAX = 64;   // blocks of the maxima
+constexpr int HMAX = 64, WMAX = 512, GMAX = 64;   // blocks of the maxima; k_ce_pack joins WMAX by 2 a thread
 __host__ __device__ inline int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 
-// What the launches share: largest finite magnitudes of hidden, weight and the rows' gradients, by block and joined.
-struct Scalars { float h, w; float hpart[HMAX], wpart[WMAX], gpart[GMAX]; };
+// What the launches of a call share: largest finite magnitudes of hidden and weight, and of the rows' gradients by block.
+struct Scalars { float h, w; float gpart[GMAX]; };
+// What the pass over the operands' magnitudes leaves: the largest by block, and for fp32 the exponents of the scales of hidden's rows, then
+// of the weight's.  In the workspace, or kept by the caller from the forward call to the backward call.
+struct Parts { float hpart[HMAX], wpart[WMAX]; };
 
 // 13 - e: the exponent of the power of two that brings the largest magnitude to 2^13..2^14; 0 for nothing but zeros.  Scales are undone by the
 // sum of their exponents: a product of one scale's reciprocal with the sum may leave fp32's range where the result does not.
@@ -43,6 +50,8 @@ __device__ __forceinline__ int scale_exponent(float most) {
   return 13 - (e < -100 ? -100 : e);
 }
 __device__ __forceinline__ float scale_of(float most) { return __builtin_ldexpf(1.f, scale_exponent(most)); }
+// How far a row's scale is above the largest row's (the common one's exponent; a row of zeros has no scale to speak of)
+__device__ __forceinline__ int apart_of(int row, int common) { return row > common ? row - common : 0; }
 // of a power of two that no gradient factor passes; not below -112, so that 2^14 over it is a number too
 __device__ __forceinline__ int ceil_exponent(float most) {
   if (most == 0.f) return 0;
@@ -70,79 +79,118 @@ struct Left { const int64_t* target; const float* row_weight; int64_t ignore; co
 __device__ __forceinline__ bool row_counts(const Left& l, int row) { return l.target[row] != l.ignore && !(l.row_weight && l.row_weight[row] == 0.f); }
 __device__ __forceinline__ bool masked(const float* bias, int v) { return bias && bias[v] == -INFINITY; }
 
-// The largest finite magnitudes of hidden (blocks [0, HMAX)) and weight (the others), of the rows that are not left out: padding may
-// hold anything, and a scale that follows it would cost the others their bits.  Whether a row counts is asked only for an
-// entry that would raise the maximum.
+// The largest finite magnitude of each row of hidden (blocks [0, HMAX)) and of the weight (the others), left behind as the exponent of the
+// row's scale (hs, ws, or null), and of all rows of a block.  A row that is left out counts as zeros: padding may hold anything, and a
+// scale that follows it would cost the others their bits.  One pass at the rate of the loads: `team` lanes a row, 4 loads of 16 bytes a lane
+// in flight, the last one of a row moved back to where the row ends (a maximum may meet an entry twice).
+constexpr int MAG_THREADS = 1024, SCALES_END = 256;   // exponents behind the last row: a tile reads its rows' by fours
 template <class T>
-__global__ __launch_bounds__(256) void k_ce_absmax(View h, View w, Left left, Scalars* s) {
-  __shared__ float sh[4];
+__global__ __launch_bounds__(MAG_THREADS, 8) void k_ce_magnitudes(View h, View w, Left left, Parts* parts, int* hs, int* ws) {
+  __shared__ float sh[MAG_THREADS / 64][64];
   const bool is_h = blockIdx.x < HMAX;
   const View& v = is_h ? h : w;
-  const int b = is_h ? blockIdx.x : blockIdx.x - HMAX, n = is_h ? HMAX : WMAX;
+  int* const out = is_h ? hs : ws;
+  const int b = is_h ? blockIdx.x : blockIdx.x - HMAX, n = is_h ? HMAX : WMAX, tid = threadIdx.x, wave = tid >> 6;
   constexpr int E = 16 / sizeof(T);
-  typedef T vec __attribute__((ext_vector_type(E)));
-  float m = 0.f;
-  auto counts = [&](int row) { return is_h ? row_counts(left, row) : !masked(left.bias, row); };
-  if (v.s1 == 1 && v.s0 == v.cols && ((size_t)v.p & 15) == 0) {   // dense: 16 bytes a thread
-    const int64_t all = (int64_t)v.rows * v.cols, whole = all / E, step = (int64_t)n * 256;
-    const vec* p = (const vec*)v.p;
-    const bool asked = is_h || left.bias;
-    const double inverse = 1.0 / v.cols;
-    for (int64_t k = (int64_t)b * 256 + threadIdx.x; k < whole; k += 4 * step) {
-      vec x[4];
-      int row[4];
-      bool in[4];
+  typedef T vec __attribute__((ext_vector_type(E), aligned(sizeof(T))));
+  float most = 0.f;
+  if (out && b == 0 && tid < SCALES_END) out[v.rows + tid] = 0;
+  auto done = [&](int row, float m) {   // by one thread a row
+    if (!(is_h ? row_counts(left, row) : !masked(left.bias, row))) m = 0.f;
+    if (out) out[row] = scale_exponent(m);
+    most = fmaxf(most, m);
+  };
+  if (v.s1 <= v.s0 || v.rows == 1) {
+    const bool wide = v.s1 == 1 && v.cols >= E;
+    const int chunks = wide ? (v.cols + E - 1) / E : v.cols;
+    int team = 1;
+    while (team < chunks && team < 64) team *= 2;
+    if (chunks > 1024) team = MAG_THREADS;
+    const bool few = chunks <= team;   // a load a lane: 4 rows at a time
+    const int R = MAG_THREADS / team, lane = tid & (team - 1), mine = tid / team, step = few ? 4 * R : R;
+    auto load = [&](int row, int chunk) {
+      const T* p = (const T*)v.p + (row < v.rows ? row : v.rows - 1) * v.s0;
+      float m = 0.f;
+      if (wide) {
+        const vec x = *(const vec*)(p + (chunk * E < v.cols - E ? chunk * E : v.cols - E));
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int64_t at = k + u * step < whole ? k + u * step : k;
-        x[u] = p[at];
-        row[u] = (int)((double)(at * E) * inverse);   // off by one at most
-        if ((int64_t)row[u] * v.cols > at * E) --row[u];
-        else if ((int64_t)(row[u] + 1) * v.cols <= at * E) ++row[u];
+        for (int e = 0; e < E; ++e) m = fmaxf(m, finite((float)x[e]));
+      } else {
+        m = finite((float)p[(chunk < v.cols ? chunk : v.cols - 1) * v.s1]);
       }
+      return m;
+    };
+    auto over_team = [&](float m) {
+      for (int d = (team < 64 ? team : 64) / 2; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
+      return m;
+    };
+    for (int r0 = b * step; r0 < v.rows; r0 += n * step) {
+      float m[4];
+      if (few) {
 #pragma unroll
-      for (int u = 0; u < 4; ++u) in[u] = !asked || counts(row[u]);
+        for (int u = 0; u < 4; ++u) m[u] = load(r0 + u * R + mine, lane);
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int64_t at = k + u * step < whole ? k + u * step : k;
-        int col = (int)(at * E - (int64_t)row[u] * v.cols);
-        const bool one = !asked || col + E <= v.cols;   // all of it in one row
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          if (in[u]) m = fmaxf(m, finite((float)x[u][e]));
-          if (!one && ++col == v.cols && e + 1 < E) {
-            col = 0;
-            in[u] = counts(++row[u] < v.rows ? row[u] : v.rows - 1);
-          }
+        for (int u = 0; u < 4; ++u) {
+          m[u] = over_team(m[u]);
+          if (lane == 0 && r0 + u * R + mine < v.rows) done(r0 + u * R + mine, m[u]);
         }
+        continue;
       }
-    }
-    if (b == 0 && threadIdx.x < all - whole * E) {
-      const int64_t k = whole * E + threadIdx.x;
-      if (counts((int)(k / v.cols))) m = fmaxf(m, finite((float)((const T*)v.p)[k]));
-    }
-  } else {
-    const bool along = v.s1 <= v.s0;   // lanes along the axis that is closer in memory
-    const int outer = along ? v.rows : v.cols, inner = along ? v.cols : v.rows;
-    const int64_t so = along ? v.s0 : v.s1, si = along ? v.s1 : v.s0;
-    for (int o = b * 4 + (threadIdx.x >> 6); o < outer; o += n * 4)
-      for (int i = threadIdx.x & 63; i < inner; i += 64) {
-        const float x = finite((float)((const T*)v.p)[o * so + i * si]);
-        if (x > m && counts(along ? o : i)) m = x;
+      float all = 0.f;
+      for (int c = lane; c < chunks; c += 4 * team) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) m[u] = load(r0 + mine, c + u * team);
+        all = fmaxf(all, fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])));
       }
+      all = over_team(all);
+      if (team > 64) {   // the block's only row
+        if ((tid & 63) == 0) sh[wave][0] = all;
+        __syncthreads();
+        if (tid == 0)
+          for (int k = 1; k < MAG_THREADS / 64; ++k) all = fmaxf(all, sh[k][0]);
+        __syncthreads();
+      }
+      if (lane == 0 && r0 + mine < v.rows) done(r0 + mine, all);
+    }
+  } else {   // rows closer in memory than columns: a lane a row, the waves take the columns in turn
+    const int q = MAG_THREADS / 64, lane = tid & 63;
+    for (int r0 = b * 64; r0 < v.rows; r0 += n * 64) {
+      const int row = r0 + lane;
+      const T* p = (const T*)v.p + (row < v.rows ? row : v.rows - 1) * v.s0;
+      float all = 0.f;
+      for (int c = wave; c < v.cols; c += 4 * q) {
+        float m[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) m[u] = finite((float)p[(c + u * q < v.cols ? c + u * q : v.cols - 1) * v.s1]);
+        all = fmaxf(all, fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])));
+      }
+      sh[wave][lane] = all;
+      __syncthreads();
+      if (wave == 0) {
+        for (int k = 1; k < q; ++k) all = fmaxf(all, sh[k][lane]);
+        if (row < v.rows) done(row, all);
+      }
+      __syncthreads();
+    }
   }
-  m = block_max(m, sh);
-  if (threadIdx.x == 0) (is_h ? s->hpart : s->wpart)[b] = m;
+  most = wave_max(most);
+  if ((tid & 63) == 0) sh[wave][0] = most;
+  __syncthreads();
+  if (tid == 0) {
+    for (int k = 1; k < MAG_THREADS / 64; ++k) most = fmaxf(most, sh[k][0]);
+    (is_h ? parts->hpart : parts->wpart)[b] = most;
+  }
 }
 
 // A view -> operands: as it stands (n: rows of the view, type E) and transposed (t: its columns, fp16), either may be null; columns
-// beyond the view and up to the pitch become zeros.  fp32: two scaled fp16 pieces both ways.  bf16 transposed: scaled.  A row that
+// beyond the view and up to the pitch become zeros.  fp32: two fp16 pieces both ways, each row by its own scale as it stands.  bf16 transposed: scaled.  A row that
 // does not count becomes zeros: whatever it holds must not reach a sum over rows; so does a masked row of the weight, whose D is 0.
 struct Job {
   View v;
   void* n; int64_t n_cols;
   void* t; int64_t t_cols;
   bool mask; const float* bias;   // leaves out rows: of hidden, of the weight
+  const int* scales;              // fp32: the exponents of the rows' scales
   int blocks;
 };
 // The gradient of each row's own loss, and the largest of them.
@@ -178,9 +226,10 @@ __device__ __forceinline__ void pack_rows(E* out, int64_t cols, int r0, int rows
 // pieces of D and of what it is multiplied by; 3: two, of which the other factor needs one
 template <class T> struct GradPieces { static constexpr int P = __is_same(T, float) ? 2 : __is_same(T, _Float16) ? 3 : 1, N = P == 1 ? 1 : 2; };
 template <class T>
-__global__ __launch_bounds__(256) void k_ce_pack(Job h, Job w, Scale g, Left left, Scalars* s, float* largest, bool known) {
+__global__ __launch_bounds__(256) void k_ce_pack(Job h, Job w, Scale g, Left left, const Parts* parts, Scalars* s, float* largest) {
   constexpr bool TWO = sizeof(T) == 4, SCALED = !__is_same(T, _Float16);
   __shared__ float tile[64][65], sh[4];
+  __shared__ int own[64], shared[64];   // fp32: exponents of the rows' scales as they stand, and from there to the common one
   if ((int)blockIdx.x >= h.blocks + w.blocks) {
     const int b = blockIdx.x - h.blocks - w.blocks;
     float most = 0.f;
@@ -204,18 +253,24 @@ __global__ __launch_bounds__(256) void k_ce_pack(Job h, Job w, Scale g, Left lef
   const bool is_h = (int)blockIdx.x < h.blocks;
   const Job& a = is_h ? h : w;
   const int b = is_h ? blockIdx.x : blockIdx.x - h.blocks;
+  const int across = (a.v.cols + 63) / 64, i0 = b / across * 64, j0 = b % across * 64, tid = threadIdx.x;
   float f = 1.f;
   if (SCALED && (TWO || a.t)) {   // 16-bit operands that stand as they are have no scale
-    float most;
-    if (known) most = largest[is_h ? 0 : 1];   // the forward call's
-    else most = is_h ? block_max(threadIdx.x < HMAX ? s->hpart[threadIdx.x] : 0.f, sh) : block_max(s->wpart[threadIdx.x], sh);
+    const float most = block_max(is_h ? (tid < HMAX ? parts->hpart[tid] : 0.f) : fmaxf(parts->wpart[tid], parts->wpart[tid + 256]), sh);
     f = scale_of(most);
-    if (b == 0 && threadIdx.x == 0) {
+    if (b == 0 && tid == 0) {
       (is_h ? s->h : s->w) = most;
-      if (TWO && largest && !known) largest[is_h ? 0 : 1] = most;
+      if (TWO && largest) largest[is_h ? 0 : 1] = most;
+    }
+    if (TWO) {
+      if (tid < 64) {
+        const int e = a.scales[i0 + tid < a.v.rows ? i0 + tid : a.v.rows - 1], apart = apart_of(e, scale_exponent(most));
+        own[tid] = e;
+        shared[tid] = (apart >> 1) - apart;
+      }
+      __syncthreads();
     }
   }
-  const int across = (a.v.cols + 63) / 64, i0 = b / across * 64, j0 = b % across * 64, tid = threadIdx.x;
   const bool along = a.v.s1 <= a.v.s0;
 #pragma unroll 4
   for (int k = 0; k < 16; ++k) {
@@ -225,7 +280,7 @@ __global__ __launch_bounds__(256) void k_ce_pack(Job h, Job w, Scale g, Left lef
       if (!a.mask || row_counts(left, i0 + i)) x = (float)((const T*)a.v.p)[(int64_t)(i0 + i) * a.v.s0 + (int64_t)(j0 + j) * a.v.s1];
       if (masked(a.bias, i0 + i)) x = 0.f;
     }
-    tile[i][j] = TWO ? x * f : x;
+    tile[i][j] = TWO ? __builtin_ldexpf(x, own[i]) : x;
   }
   __syncthreads();
   if (a.n) {
@@ -233,7 +288,8 @@ __global__ __launch_bounds__(256) void k_ce_pack(Job h, Job w, Scale g, Left lef
     else pack_rows<T, false>((T*)a.n, a.n_cols, i0, a.v.rows, j0, [&](int r, int c) { return tile[r][c]; });
   }
   if (a.t) {
-    if constexpr (GradPieces<T>::N == 2) pack_rows<_Float16, true>((_Float16*)a.t, a.t_cols, j0, a.v.cols, i0, [&](int r, int c) { return tile[c][r]; });
+    if constexpr (GradPieces<T>::N == 2)
+      pack_rows<_Float16, true>((_Float16*)a.t, a.t_cols, j0, a.v.cols, i0, [&](int r, int c) { return TWO ? __builtin_ldexpf(tile[c][r], shared[c]) : tile[c][r]; });
     else pack_rows<_Float16, false>((_Float16*)a.t, a.t_cols, j0, a.v.cols, i0, [&](int r, int c) { return tile[c][r] * f; });
   }
 }
@@ -248,6 +304,7 @@ struct Logits {
   const float* lse;         // backward
   const float* scale;       // backward: gradient of each row's loss (0: the row does not count)
   const Scalars* s;
+  const int *hs, *ws;       // fp32: the exponents of the rows' scales, of hidden and of the piece
   int64_t ignore;
   int rows, v0, cols;       // rows; first vocabulary entry and entries of the piece
   int nkb;                  // K blocks
@@ -260,14 +317,18 @@ struct Logits {
   float* bpart;             // [row tiles][cols] partial sums of the bias' gradient, or null
 };
 
-// The accumulators of 32 rows of the tile (vocabulary entries from mb on) become z, in place.
+// The accumulators of 32 rows of the tile (vocabulary entries from mb on) become z, in place.  `hs`: the exponents of the columns' scales; `ws`:
+// those of the rows' are left there, 0 behind the piece.
 template <int P, int TN>
-__device__ __forceinline__ void logits_of(const Logits& a, f32x16 (&acc)[TN], int mb, int h, int undo) {
-  if (P == 2)
+__device__ __forceinline__ void logits_of(const Logits& a, f32x16 (&acc)[TN], int mb, int h, const int (&hs)[TN], i32x4 (&ws)[4]) {
+  if (P == 2) {
 #pragma unroll
-    for (int x = 0; x < TN; ++x)
+    for (int q = 0; q < 4; ++q) ws[q] = *(const i32x4*)(a.ws + mb + 8 * q + 4 * h);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) acc[x][r] = __builtin_ldexpf(acc[x][r], undo);
+    for (int r = 0; r < 16; ++r)
+#pragma unroll
+      for (int x = 0; x < TN; ++x) acc[x][r] = __builtin_ldexpf(acc[x][r], -(ws[r >> 2][r & 3] + hs[x]));
+  }
   if (a.bias)
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
@@ -291,13 +352,19 @@ __global__ __launch_bounds__(C::THREADS, C::LDS > 81920 ? C::THREADS / 256 : C::
   if (!product<T, P, C>(a.w.p + m0 * a.w.pitch, a.w.pitch, a.cols - m0, a.h.p + n0 * a.h.pitch, a.h.pitch, a.rows - n0, a.nkb, lds, acc)) return;
   const Lane L = lane_of();
   const int wm = L.wave / C::WN, wn = L.wave % C::WN;
-  const int undo = P == 2 ? -scale_exponent(a.s->h) - scale_exponent(a.s->w) : 0;
+  int hs[C::TN];
+#pragma unroll
+  for (int x = 0; x < C::TN; ++x) {
+    const int n = n0 + (wn * C::TN + x) * 32 + L.j;
+    hs[x] = P == 2 ? a.hs[n < a.rows ? n : a.rows - 1] : 0;
+  }
   float* tops = (float*)lds;                  // [WM][BN] maxima, then sums
   float* sums = tops + C::WM * C::BN;
 #pragma unroll
   for (int y = 0; y < C::TM; ++y) {
     const int mb = m0 + (wm * C::TM + y) * 32;
-    logits_of<P>(a, acc[y], mb, L.h, undo);
+    i32x4 ws[4];
+    logits_of<P>(a, acc[y], mb, L.h, hs, ws);
     if (mb + 32 > a.cols)
 #pragma unroll
       for (int r = 0; r < 16; ++r)
@@ -452,8 +519,14 @@ __global__ __launch_bounds__(C::THREADS, C::LDS > 81920 ? C::THREADS / 256 : C::
   if (!product<T, P, C>(a.w.p + m0 * a.w.pitch, a.w.pitch, a.cols - m0, a.h.p + n0 * a.h.pitch, a.h.pitch, a.rows - n0, a.nkb, lds, acc)) return;
   const Lane L = lane_of();
   const int wm = L.wave / C::WN, wn = L.wave % C::WN;
-  const int undo = P == 2 ? -scale_exponent(a.s->h) - scale_exponent(a.s->w) : 0;
+  int hs[C::TN];
+#pragma unroll
+  for (int x = 0; x < C::TN; ++x) {
+    const int n = n0 + (wn * C::TN + x) * 32 + L.j;
+    hs[x] = P == 2 ? a.hs[n < a.rows ? n : a.rows - 1] : 0;
+  }
   const float per = __builtin_ldexpf(1.f, DBITS - ceil_exponent(largest_gradient(a.s)));
+  const int common_w = P == 2 ? scale_exponent(a.s->w) : 0, common_h = P == 2 ? scale_exponent(a.s->h) : 0;
   unsigned* patch = (unsigned*)(lds + L.wave * PATCH);
   float* bsum = (float*)(lds + C::WAVES * PATCH);   // [WN][BM]
   float lse[C::TN], g[C::TN];
@@ -468,10 +541,14 @@ __global__ __launch_bounds__(C::THREADS, C::LDS > 81920 ? C::THREADS / 256 : C::
 #pragma unroll
   for (int y = 0; y < C::TM; ++y) {
     const int mb = m0 + (wm * C::TM + y) * 32;
-    logits_of<P>(a, acc[y], mb, L.h, undo);
-    float bs[16];
+    i32x4 ws[4];
+    logits_of<P>(a, acc[y], mb, L.h, hs, ws);
+    float bs[16], scale[16];   // scale: D's for dH
 #pragma unroll
-    for (int r = 0; r < 16; ++r) bs[r] = 0.f;
+    for (int r = 0; r < 16; ++r) {
+      bs[r] = 0.f;
+      scale[r] = P == 2 ? __builtin_ldexpf(1.f, DBITS - (apart_of(ws[r >> 2][r & 3], common_w) >> 1)) : DSCALE;
+    }
 #pragma unroll
     for (int x = 0; x < C::TN; ++x) {
       const int nb = n0 + (wn * C::TN + x) * 32;
@@ -494,11 +571,11 @@ __global__ __launch_bounds__(C::THREADS, C::LDS > 81920 ? C::THREADS / 256 : C::
       if (a.bpart)
 #pragma unroll
         for (int r = 0; r < 16; ++r) bs[r] += z[r] * g[x];
-      const float gd = g[x] * per;
+      const float gd = P == 2 ? __builtin_ldexpf(g[x] * per, -(apart_of(hs[x], common_h) >> 1)) : g[x] * per;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         v[r] = z[r] * gd;
-        z[r] *= DSCALE;
+        z[r] *= scale[r];
       }
       if (nb < a.rows && mb < a.d_cols) {
         if constexpr (N == 2) store_t_f16x2((_Float16*)a.d + (int64_t)nb * 2 * a.d_cols + mb * 2, 2 * a.d_cols, patch, L, a.rows - nb, z);
@@ -686,7 +763,7 @@ struct Layout {
   int split_h, split_w;             // parts of the sums of dH and dW
   int64_t pieces_n;
   // offsets
-  int64_t scalars, hp, wp, ht, wt, d, dt, part, picked, sums, scale, bpart, hslots, wslots, bytes;
+  int64_t scalars, scales, hp, wp, ht, wt, d, dt, part, picked, sums, scale, bpart, hslots, wslots, bytes;
 };
 // Both gradients are one launch, dH's (long) tiles first: the tiles and the parts of the sums that make it shortest.  A part costs writing
 // and reading back fp32 sums and a second launch.  The constants, us by pieces of D as above, are fitted to 70 calls (1 to 20 000 rows, 64
@@ -717,6 +794,10 @@ void plan_gradients(Layout& l, const Shape& c, int64_t vp, int p) {
       }
   }
 }
+// The parts, then the exponents of hidden's rows and of the weight's
+int64_t scales_of_hidden() { return up(sizeof(Parts), 256); }
+int64_t scales_of_weight(const Shape& c) { return scales_of_hidden() + up((c.rows + SCALES_END) * 4, 256); }
+int64_t scales_bytes(const Shape& c) { return scales_of_weight(c) + up((c.vocab + SCALES_END) * 4, 256); }
 Layout layout_of(const Shape& c, bool direct_h, bool direct_w, bool backward, bool bias) {
   Layout l = {};
   const int p = pieces(c.elem);
@@ -743,6 +824,7 @@ Layout layout_of(const Shape& c, bool direct_h, bool direct_w, bool backward, bo
   int64_t at = 0;
   auto take = [&](int64_t bytes) { const int64_t o = at; at += up(bytes, 256); return o; };
   l.scalars = take(sizeof(Scalars));
+  l.scales = take(p == 2 ? scales_bytes(c) : sizeof(Parts));
   if (l.pack_h) l.hp = take(c.rows * l.kp * per);
   if (l.pack_w) l.wp = take(l.piece * l.kp * per);
   if (!backward) {
@@ -773,6 +855,7 @@ struct Call {
   const float* bias; const int64_t* target; const float* row_weight;
   int64_t ignore; int reduction;
   float* losses; float* lse; float* total; float* count; float* largest;
+  char* scales;       // fp32: kept by the caller, or null
   const float* grad; int64_t grad_stride;
   void* gh; void* gw; float* gb;
   char* ws; size_t ws_bytes; hipStream_t stream;
@@ -801,18 +884,27 @@ View hidden_of(const Call& a) { return {a.h, a.h0, a.h1, (int)a.c.rows, (int)a.c
 
 Left left_of(const Call& a) { return {a.target, a.row_weight, a.ignore, a.bias}; }
 
+// Where the magnitudes of a call are; hs, ws: fp32
+struct Scales { Parts* parts; int *hs, *ws; };
 template <class T>
-void absmax_launch(const Call& a, Scalars* s) {
-  hipLaunchKernelGGL(k_ce_absmax<T>, dim3(HMAX + WMAX), dim3(256), 0, a.stream, hidden_of(a), weight_piece<T>(a, 0, a.c.vocab), left_of(a), s);
+Scales scales_of(const Call& a, const Layout& l) {
+  char* at = a.scales ? a.scales : a.ws + l.scales;
+  if (sizeof(T) != 4) return {(Parts*)at, nullptr, nullptr};
+  return {(Parts*)at, (int*)(at + scales_of_hidden()), (int*)(at + scales_of_weight(a.c))};
+}
+template <class T>
+void magnitudes_launch(const Call& a, const Scales& sc) {
+  hipLaunchKernelGGL(k_ce_magnitudes<T>, dim3(HMAX + WMAX), dim3(MAG_THREADS), 0, a.stream, hidden_of(a), weight_piece<T>(a, 0, a.c.vocab), left_of(a), sc.parts,
+                     sc.hs, sc.ws);
 }
 // Packs hidden (h null: not in this launch) and a weight piece, and takes the rows' gradients.
 template <class T>
-void pack_launch(const Call& a, Job h, Job w, Scale g, Scalars* s, bool known) {
+void pack_launch(const Call& a, Job h, Job w, Scale g, const Scales& sc, Scalars* s) {
   auto blocks = [](Job& j) { j.blocks = j.n || j.t ? (int)(up(j.v.cols, 64) / 64 * (up(j.v.rows, 64) / 64)) : 0; };
   blocks(h);
   blocks(w);
   const int all = h.blocks + w.blocks + g.blocks;
-  if (all > 0) hipLaunchKernelGGL(k_ce_pack<T>, dim3(all), dim3(256), 0, a.stream, h, w, g, left_of(a), s, a.largest, known);
+  if (all > 0) hipLaunchKernelGGL(k_ce_pack<T>, dim3(all), dim3(256), 0, a.stream, h, w, g, left_of(a), sc.parts, s, a.largest);
 }
 
 template <class K, class... A>
@@ -825,7 +917,7 @@ int tile_launch(K kernel, int64_t tiles, int threads, int lds, hipStream_t strea
   ((kind) == 0 ? call(Ce64) : (kind) == 1 ? call(Ce128) : call(Ce256))
 
 template <class T>
-Logits logits_call(const Call& a, const Layout& l, const View& w, int64_t v0, Scalars* s) {
+Logits logits_call(const Call& a, const Layout& l, const View& w, int64_t v0, const Scales& sc, Scalars* s) {
   constexpr int P = sizeof(T) == 4 ? 2 : 1;
   Logits g = {};
   g.h = l.pack_h ? Operand{a.ws + l.hp, l.kp * 2 * P} : Operand{(const char*)a.h, a.h0 * 2};
@@ -833,6 +925,10 @@ Logits logits_call(const Call& a, const Layout& l, const View& w, int64_t v0, Sc
   g.bias = a.bias ? a.bias + v0 : nullptr;
   g.target = a.target;
   g.s = s;
+  if (P == 2) {
+    g.hs = sc.hs;
+    g.ws = sc.ws + v0;
+  }
   g.rows = (int)a.c.rows;
   g.v0 = (int)v0;
   g.cols = w.rows;
@@ -867,16 +963,17 @@ int forward(const Call& a) {
   const Layout l = layout_of(a.c, direct(a.h, a.h0, a.h1, a.c), direct(a.w, a.w0, a.w1, a.c), false, false);
   if (!a.ws || (int64_t)a.ws_bytes < l.bytes) return set_error(GRLHIP_ERR_WORKSPACE, "linear_ce_forward: workspace too small: need " + std::to_string(l.bytes));
   Scalars* s = (Scalars*)(a.ws + l.scalars);
-  if (P == 2) absmax_launch<T>(a, s);
+  const Scales sc = scales_of<T>(a, l);
+  if (P == 2) magnitudes_launch<T>(a, sc);
   const int side = SIDE[l.kind_z];
   const int64_t tn = up(a.c.rows, side) / side;
   int tiles = 0;
   for (int64_t v0 = 0; v0 < a.c.vocab; v0 += l.piece) {
     const View w = weight_piece<T>(a, v0, a.c.vocab - v0 < l.piece ? a.c.vocab - v0 : l.piece);
-    Job jh{hidden_of(a), v0 == 0 && l.pack_h ? a.ws + l.hp : nullptr, l.kp, nullptr, 0, false, nullptr, 0};
-    Job jw{w, l.pack_w ? a.ws + l.wp : nullptr, l.kp, nullptr, 0, false, a.bias ? a.bias + v0 : nullptr, 0};
-    pack_launch<T>(a, jh, jw, Scale{}, s, false);
-    Logits g = logits_call<T>(a, l, w, v0, s);
+    Job jh{hidden_of(a), v0 == 0 && l.pack_h ? a.ws + l.hp : nullptr, l.kp, nullptr, 0, false, nullptr, sc.hs, 0};
+    Job jw{w, l.pack_w ? a.ws + l.wp : nullptr, l.kp, nullptr, 0, false, a.bias ? a.bias + v0 : nullptr, P == 2 ? sc.ws + v0 : nullptr, 0};
+    pack_launch<T>(a, jh, jw, Scale{}, sc, s);
+    Logits g = logits_call<T>(a, l, w, v0, sc, s);
     g.part = (float2*)(a.ws + l.part) + (int64_t)tiles * a.c.rows;
     g.picked = (float*)(a.ws + l.picked);
     const int tm = (int)(up(w.rows, side) / side);
@@ -894,8 +991,8 @@ int backward(const Call& a) {
   const Layout l = layout_of(a.c, direct(a.h, a.h0, a.h1, a.c), direct(a.w, a.w0, a.w1, a.c), true, a.gb != nullptr);
   if (!a.ws || (int64_t)a.ws_bytes < l.bytes) return set_error(GRLHIP_ERR_WORKSPACE, "linear_ce_backward: workspace too small: need " + std::to_string(l.bytes));
   Scalars* s = (Scalars*)(a.ws + l.scalars);
-  const bool known = P == 2 && a.largest;   // an fp32 forward call has them
-  if (!__is_same(T, _Float16) && !known) absmax_launch<T>(a, s);
+  const Scales sc = scales_of<T>(a, l);
+  if (!__is_same(T, _Float16) && !a.scales) magnitudes_launch<T>(a, sc);   // the forward call's, if the caller kept them
   float* scale = (float*)(a.ws + l.scale);
   const int side = SIDE[l.kind_z];
   const int64_t tn = up(a.c.rows, side) / side;
@@ -903,14 +1000,14 @@ int backward(const Call& a) {
     const bool first = v0 == 0, last = v0 + l.piece >= a.c.vocab;
     const int64_t cols = last ? a.c.vocab - v0 : l.piece, vp = up(cols, 64);
     const View w = weight_piece<T>(a, v0, cols);
-    const Job jh{hidden_of(a), first && l.pack_h ? a.ws + l.hp : nullptr, l.kp, first && a.gw ? a.ws + l.ht : nullptr, l.np, true, nullptr, 0};
-    const Job jw{w, l.pack_w ? a.ws + l.wp : nullptr, l.kp, a.gh ? a.ws + l.wt : nullptr, vp, false, a.bias ? a.bias + v0 : nullptr, 0};
+    const Job jh{hidden_of(a), first && l.pack_h ? a.ws + l.hp : nullptr, l.kp, first && a.gw ? a.ws + l.ht : nullptr, l.np, true, nullptr, sc.hs, 0};
+    const Job jw{w, l.pack_w ? a.ws + l.wp : nullptr, l.kp, a.gh ? a.ws + l.wt : nullptr, vp, false, a.bias ? a.bias + v0 : nullptr, P == 2 ? sc.ws + v0 : nullptr, 0};
     int64_t gblocks = (a.c.rows + 255) / 256;
     if (gblocks > GMAX) gblocks = GMAX;
-    const Scale sc{a.grad, a.grad_stride, a.count, (int)a.c.rows, (int)a.c.vocab, a.reduction, first ? (int)gblocks : 0, scale};
-    pack_launch<T>(a, jh, jw, sc, s, known);
+    const Scale rows{a.grad, a.grad_stride, a.count, (int)a.c.rows, (int)a.c.vocab, a.reduction, first ? (int)gblocks : 0, scale};
+    pack_launch<T>(a, jh, jw, rows, sc, s);
 
-    Logits g = logits_call<T>(a, l, w, v0, s);
+    Logits g = logits_call<T>(a, l, w, v0, sc, s);
     g.lse = a.lse;
     g.scale = scale;
     g.d = a.ws + l.d;
@@ -979,6 +1076,16 @@ using namespace grlhip;
 
 extern "C" {
 
+size_t grlhip_linear_ce_scales_bytes(int64_t rows, int64_t vocab) {
+  return guarded_size([&]() -> size_t {
+    if (rows < 1 || vocab < 1 || rows > MAX_ROWS || vocab > MAX_VOCAB) {
+      set_error(GRLHIP_ERR_UNSUPPORTED, "linear_ce: rows and vocabulary must be 1 to 2^20 and 2^21");
+      return 0;
+    }
+    return (size_t)scales_bytes(Shape{rows, 1, vocab, GRLHIP_ELEM_F32});
+  });
+}
+
 size_t grlhip_linear_ce_workspace_bytes(const void* hidden, const int64_t* hidden_strides, const void* weight, const int64_t* weight_strides,
                                         int64_t rows, int64_t features, int64_t vocab, int elem, int backward_) {
   return guarded_size([&]() -> size_t {
@@ -1000,6 +1107,8 @@ int grlhip_linear_ce_forward(const void* hidden, const int64_t* hidden_strides, 
                              int elem, int reduction, float* losses, float* lse, float* total, float* count, float* largest, void* workspace, size_t workspace_bytes, void* stream) {
   return guarded([&]() -> int {
     Call a = {};
+    const bool kept = (elem & GRLHIP_ELEM_SCALES) && largest;
+    if (elem == (GRLHIP_ELEM_F32 | GRLHIP_ELEM_SCALES)) elem = GRLHIP_ELEM_F32;
     a.c = {rows, features, vocab, elem};
     a.h = hidden;
     a.h0 = hidden_strides ? hidden_strides[0] : features;
@@ -1016,13 +1125,15 @@ int grlhip_linear_ce_forward(const void* hidden, const int64_t* hidden_strides, 
     a.lse = lse;
     a.total = total;
     a.count = count;
-    a.largest = largest;
+    a.largest = kept ? nullptr : largest;
+    a.scales = kept ? (char*)largest : nullptr;
     a.ws = (char*)workspace;
     a.ws_bytes = workspace_bytes;
     a.stream = (hipStream_t)stream;
     if (const int rc = check("linear_ce_forward", a)) return rc;
     if (!losses) return set_error(GRLHIP_ERR_INVALID, "linear_ce_forward: null losses");
     if (!total != !count || (!total && reduction != GRLHIP_REDUCE_NONE)) return set_error(GRLHIP_ERR_INVALID, "linear_ce_forward: total and count go together, and may be NULL for GRLHIP_REDUCE_NONE only");
+    if ((size_t)a.scales & 255) return set_error(GRLHIP_ERR_INVALID, "linear_ce_forward: the scales must be aligned to 256 bytes");
     if ((size_t)workspace & 255) return set_error(GRLHIP_ERR_INVALID, "linear_ce_forward: the workspace must be aligned to 256 bytes");
     return elem == GRLHIP_ELEM_F32 ? forward<float>(a) : elem == GRLHIP_ELEM_BF16 ? forward<__bf16>(a) : forward<_Float16>(a);
   });
@@ -1034,6 +1145,8 @@ int grlhip_linear_ce_backward(const void* hidden, const int64_t* hidden_strides,
                               void* grad_hidden, void* grad_weight, float* grad_bias, void* workspace, size_t workspace_bytes, void* stream) {
   return guarded([&]() -> int {
     Call a = {};
+    const bool kept = (elem & GRLHIP_ELEM_SCALES) && largest;
+    if (elem == (GRLHIP_ELEM_F32 | GRLHIP_ELEM_SCALES)) elem = GRLHIP_ELEM_F32;
     a.c = {rows, features, vocab, elem};
     a.h = hidden;
     a.h0 = hidden_strides ? hidden_strides[0] : features;
@@ -1048,7 +1161,7 @@ int grlhip_linear_ce_backward(const void* hidden, const int64_t* hidden_strides,
     a.reduction = reduction;
     a.lse = const_cast<float*>(lse);
     a.count = const_cast<float*>(count);
-    a.largest = const_cast<float*>(largest);
+    a.scales = kept ? (char*)const_cast<float*>(largest) : nullptr;
     a.grad = grad;
     a.grad_stride = grad_stride;
     a.gh = grad_hidden;
@@ -1059,6 +1172,7 @@ int grlhip_linear_ce_backward(const void* hidden, const int64_t* hidden_strides,
     a.stream = (hipStream_t)stream;
     if (const int rc = check("linear_ce_backward", a)) return rc;
     if (!lse || !grad || (!count && reduction == GRLHIP_REDUCE_MEAN)) return set_error(GRLHIP_ERR_INVALID, "linear_ce_backward: null lse, gradient or count");
+    if ((size_t)a.scales & 255) return set_error(GRLHIP_ERR_INVALID, "linear_ce_backward: the scales must be aligned to 256 bytes");
     if ((size_t)workspace & 255) return set_error(GRLHIP_ERR_INVALID, "linear_ce_backward: the workspace must be aligned to 256 bytes");
     if (!grad_hidden && !grad_weight && !grad_bias) return 0;
     return elem == GRLHIP_ELEM_F32 ? backward<float>(a) : elem == GRLHIP_ELEM_BF16 ? backward<__bf16>(a) : backward<_Float16>(a);

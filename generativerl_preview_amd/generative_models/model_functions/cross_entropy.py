@@ -32,9 +32,9 @@ class _Head:
         self.shape = rows, features, vocab
         self.operands = hidden.data_ptr(), _strides(hidden), weight.data_ptr(), _strides(weight)
         self.sizes = rows, features, vocab, _ELEM[hidden.dtype]
-        self.arguments = (*self.operands, _address(bias), target.data_ptr(), ignore_index, _address(row_weight), *self.sizes, reduction)
+        self.arguments = (*self.operands, _address(bias), target.data_ptr(), ignore_index, _address(row_weight), rows, features, vocab)
 
-    def call(self, name, backward, *rest):
+    def call(self, name, backward, scales, *rest):
         lib = L.lib()
         need = lib.grlhip_linear_ce_workspace_bytes(*self.operands, *self.sizes, backward)
         if need == 0:
@@ -43,31 +43,34 @@ class _Head:
         with _on(self.device):
             ws = torch.empty(need, dtype=torch.uint8, device=self.device)
             stream = torch.cuda.current_stream(self.device).cuda_stream
-            L.check(getattr(lib, name)(*self.arguments, *rest, ws.data_ptr(), need, stream))
+            L.check(getattr(lib, name)(*self.arguments, self.sizes[3] if scales is None else self.sizes[3] | L.ELEM_SCALES, self.reduction, *rest,
+                                       ws.data_ptr(), need, stream))
 
     def forward(self, train=False):
-        """(losses, logsumexp, reduced loss, [number of rows that are not ignored, largest magnitudes of the operands]); the
-        backward pass needs the second and the last"""
-        rows, dev = self.shape[0], self.device
+        """(losses, reduced loss, what the backward pass needs: number of rows that are not ignored, scales of fp32 operands, logsumexp)"""
+        (rows, _, vocab), dev = self.shape, self.device
         losses = torch.empty(rows, dtype=torch.float32, device=dev)
-        lse = total = numbers = count = None
+        total = kept = scales = lse = count = None
         if train:
-            lse = torch.empty(rows, dtype=torch.float32, device=dev)
-        if train or self.reduction != L.REDUCE_NONE:
-            numbers = torch.empty(3, dtype=torch.float32, device=dev)
+            # one buffer: the count, from the 64th number on the scales (aligned to 256 bytes), the logsumexps last
+            room = L.lib().grlhip_linear_ce_scales_bytes(rows, vocab) // 4 if self.dtype == torch.float32 else 0
+            kept = torch.empty(64 + room + rows, dtype=torch.float32, device=dev)
+            scales, lse = kept.data_ptr() + 256 if room else None, kept.data_ptr() + 4 * (64 + room)
         if self.reduction != L.REDUCE_NONE:
-            total, count = torch.empty((), dtype=torch.float32, device=dev), numbers.data_ptr()
-        self.call("grlhip_linear_ce_forward", 0, losses.data_ptr(), _address(lse), _address(total), count,
-                  numbers.data_ptr() + 4 if train else None)
-        return losses, lse, total, numbers
+            total = torch.empty((), dtype=torch.float32, device=dev)
+            kept = torch.empty(1, dtype=torch.float32, device=dev) if kept is None else kept
+            count = kept.data_ptr()
+        self.call("grlhip_linear_ce_forward", 0, scales, losses.data_ptr(), lse, _address(total), count, scales)
+        return losses, total, kept
 
-    def backward(self, lse, numbers, grad, need_hidden, need_weight, need_bias):
+    def backward(self, kept, grad, need_hidden, need_weight, need_bias):
         rows, features, vocab = self.shape
-        dev = self.device
+        dev, at = self.device, kept.data_ptr()
+        scales, lse = at + 256 if self.dtype == torch.float32 else None, at + 4 * (kept.numel() - rows)
         gh = torch.empty(rows, features, dtype=self.dtype, device=dev) if need_hidden else None
         gw = torch.empty(vocab, features, dtype=self.dtype, device=dev) if need_weight else None
         gb = torch.empty(vocab, dtype=torch.float32, device=dev) if need_bias else None
-        self.call("grlhip_linear_ce_backward", 1, lse.data_ptr(), numbers.data_ptr(), numbers.data_ptr() + 4, grad.data_ptr(),
+        self.call("grlhip_linear_ce_backward", 1, scales, lse, at, scales, grad.data_ptr(),
                   0 if grad.dim() == 0 else grad.stride(0), _address(gh), _address(gw), _address(gb))
         return gh, gw, gb
 
@@ -125,17 +128,17 @@ class _LinearCrossEntropy(torch.autograd.Function):
     def forward(ctx, hidden, weight, bias, target, row_weight, ignore_index, reduction):
         _watch(ctx, hidden, weight, bias)
         head = _Head(hidden, weight, bias, target, row_weight, ignore_index, reduction)
-        losses, lse, total, numbers = head.forward(train=True)
-        ctx.save_for_backward(hidden, weight, bias, target, row_weight, lse, numbers)
+        losses, total, kept = head.forward(train=True)
+        ctx.save_for_backward(hidden, weight, bias, target, row_weight, kept)
         ctx.numbers = ignore_index, reduction
         return losses if reduction == L.REDUCE_NONE else total
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        hidden, weight, bias, target, row_weight, lse, numbers = ctx.saved_tensors
+        hidden, weight, bias, target, row_weight, kept = ctx.saved_tensors
         head = _Head(hidden, weight, bias, target, row_weight, *ctx.numbers)
-        gh, gw, gb = head.backward(lse, numbers, grad.float(), *ctx.needs_input_grad[:3])
+        gh, gw, gb = head.backward(kept, grad.float(), *ctx.needs_input_grad[:3])
         return gh, gw, None if gb is None else gb.to(bias.dtype), None, None, None, None
 
 
@@ -156,8 +159,10 @@ def linear_cross_entropy(hidden, weight, target, bias=None, row_weight=None, ign
     captured, no eager loss over the same leaves from the default stream may be alive: such a call is refused
     (graphs that other operations keep alive are not seen: PyTorch's own rule for them holds).
 
-    Types: 16-bit operands are multiplied as they are, fp32 ones at fp32's precision as long as they are above 2^-39 of their tensor's
-    largest entry (rows that do not count apart); the gradients' products hold operands down to 2^-38 of it."""
+    Precision.  Logits: 16-bit operands are multiplied as they are; fp32 ones lose 2^-23 of themselves or 2^-38 of the largest entry of
+    their own row.  Gradients: bf16 operands hold their bits down to 2^-28 of their tensor's largest entry; fp32 operands, and
+    ``softmax - onehot`` beside them, lose 2^-22 of themselves or, in a row 2^d smaller than the largest one, 2^(d/2 - 38) of the
+    row's largest entry and of 1."""
     if reduction not in _REDUCE:
         raise ValueError("reduction: expected 'none', 'mean' or 'sum', got %r" % (reduction,))
     if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1]:
@@ -197,6 +202,6 @@ def linear_cross_entropy(hidden, weight, target, bias=None, row_weight=None, ign
     if torch.is_grad_enabled() and (rows.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
         loss = _LinearCrossEntropy.apply(rows, weight, bias, flat, row_weight, int(ignore_index), _REDUCE[reduction])
     else:
-        losses, _, total, _ = _Head(rows, weight, bias, flat, row_weight, int(ignore_index), _REDUCE[reduction]).forward()
+        losses, total, _ = _Head(rows, weight, bias, flat, row_weight, int(ignore_index), _REDUCE[reduction]).forward()
         loss = losses if reduction == "none" else total
     return loss.view(target.shape) if reduction == "none" else loss

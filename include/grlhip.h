@@ -372,6 +372,7 @@ int grlhip_muon_step(float* const* params, const float* const* grads, float* con
                      int nesterov, float keep, int32_t steps, float a, float b, float c, float eps,
                      void* workspace, size_t workspace_bytes, void* stream);
 
+enum { GRLHIP_ELEM_SCALES = 0x100 };   /* beside GRLHIP_ELEM_F32, for grlhip_linear_ce_forward / _backward: see `largest` there */
 typedef enum { GRLHIP_REDUCE_NONE = 0, GRLHIP_REDUCE_MEAN = 1, GRLHIP_REDUCE_SUM = 2 } grlhip_reduction;
 
 /* No counterpart in the reference (its policies are continuous).  Softmax cross entropy of a linear head over a large
@@ -379,8 +380,10 @@ typedef enum { GRLHIP_REDUCE_NONE = 0, GRLHIP_REDUCE_MEAN = 1, GRLHIP_REDUCE_SUM
  *   losses[i] = row_weight[i] (logsumexp_v z[i][v] - z[i][target[i]]);   lse[i] = logsumexp_v z[i][v]  (may be NULL)
  *   *total = sum of the losses (GRLHIP_REDUCE_SUM, _NONE) or that over *count (_MEAN); *count = number of rows whose target is
  *   not ignore_index, at least 1.  Both may be NULL for GRLHIP_REDUCE_NONE.
- *   largest[2] = largest finite magnitudes of hidden and weight, in rows that count and are not masked, written for GRLHIP_ELEM_F32 only (the backward call may take
- *   them instead of reading the operands once more); may be NULL.
+ *   largest[2] = largest finite magnitudes of hidden and weight, in rows that count and are not masked, written for GRLHIP_ELEM_F32 only; may be NULL.
+ *   With elem = GRLHIP_ELEM_F32 | GRLHIP_ELEM_SCALES, `largest` is instead a buffer of grlhip_linear_ce_scales_bytes, 256-byte aligned, in which
+ *   the forward call leaves the scales of the operands' rows for a backward call of the same operands, bias, targets and row weights, which
+ *   then need not read the operands for them once more.
  * hidden [rows][features], weight [vocab][features]: element type `elem`, element strides {row, column} in HOST arrays (NULL:
  * dense).  bias [vocab] fp32 or NULL; -inf masks an entry, whatever its row of the weight holds.  target [rows] int64; row_weight [rows] fp32 or NULL (1).
  * A row whose target is ignore_index or whose weight is 0 has loss 0 and contributes nothing, whatever its hidden row holds.  Any other
@@ -390,13 +393,14 @@ typedef enum { GRLHIP_REDUCE_NONE = 0, GRLHIP_REDUCE_MEAN = 1, GRLHIP_REDUCE_SUM
 size_t grlhip_linear_ce_workspace_bytes(const void* hidden, const int64_t* hidden_strides, const void* weight,
                                         const int64_t* weight_strides, int64_t rows, int64_t features, int64_t vocab, int elem,
                                         int backward);
+size_t grlhip_linear_ce_scales_bytes(int64_t rows, int64_t vocab);
 int grlhip_linear_ce_forward(const void* hidden, const int64_t* hidden_strides, const void* weight,
                              const int64_t* weight_strides, const float* bias, const int64_t* target, int64_t ignore_index,
                              const float* row_weight, int64_t rows, int64_t features, int64_t vocab, int elem, int reduction,
                              float* losses, float* lse, float* total, float* count, float* largest, void* workspace,
                              size_t workspace_bytes, void* stream);
 
-/* The gradients of it: `lse`, `count` and (GRLHIP_ELEM_F32; may be NULL) `largest` as the forward call left them; `grad`: DEVICE, the gradient of each loss at stride
+/* The gradients of it: `lse` and `count` as the forward call left them; `largest`: read with GRLHIP_ELEM_SCALES only; `grad`: DEVICE, the gradient of each loss at stride
  * `grad_stride` (GRLHIP_REDUCE_NONE) or of the reduced loss (grad_stride 0).  grad_hidden [rows][features] and grad_weight
  * [vocab][features] (type `elem`, dense), grad_bias [vocab] (fp32) are overwritten; each may be NULL.  The logits are recomputed in
  * pieces of the vocabulary.  Workspace: grlhip_linear_ce_workspace_bytes (backward = 1). */

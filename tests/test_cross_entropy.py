@@ -327,6 +327,58 @@ def test_gpu_fp32_operands_of_any_magnitude(scale):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("ratio", [1e6, 1e9])
+def test_gpu_rows_of_very_different_magnitudes(ratio):
+    """One row of hidden and one of the weight that count and are `ratio` times the others: in fp32 their size is their own matter.  The logits'
+    error is the products' (2^-21 and the sums', entry by entry) and the pieces' ends, 2^-38 of the largest entry of the ROW; softmax of
+    logits that are off by at most e lies between those of z_v + e_v against z_u - e_u and the reverse.  The gradients' operands end at
+    2^-25 of their scaled values, half of the rows' exponents taken by D."""
+    h, w, t, b, rw = inputs(130, 256, 300, F32, seed=21, ignored=0.1)
+    n, k, v = 130, 256, 300
+    t[7], rw[7], b[11], b[12] = 12, 1.5, 0.25, 0.25
+    h[7] *= ratio
+    w[11] *= ratio
+    leaves = [h.requires_grad_(), w.requires_grad_()]
+    loss = linear_cross_entropy(*leaves, t, bias=b, row_weight=rw, reduction="none")
+    total = linear_cross_entropy(*leaves, t, bias=b, row_weight=rw, reduction="sum")
+    dh, dw = torch.autograd.grad(total, leaves)
+    H, W, B = h.detach().double(), w.detach().double(), b.double()
+    kept = (t != -100) & (rw != 0)
+    z = H @ W.t() + B
+    open_ = z > -math.inf
+    hm, wm = H.abs().max(1, keepdim=True).values, W.abs().max(1, keepdim=True).values
+    ez = ((k / 16 + 16) * 2.0 ** -24 + 2.0 ** -21) * (H.abs() @ W.abs().t()) + 2.0 ** -23 * torch.where(open_, z.abs(), 0.0)
+    ez = ez + 2.0 ** -38 * (hm * W.abs().sum(1) + H.abs().sum(1, keepdim=True) * wm.t())
+    lse = torch.logsumexp(z, 1)
+    e_lse = torch.maximum(torch.logsumexp(z + ez, 1) - lse, lse - torch.logsumexp(z - ez, 1))
+    at = t.clamp(min=0).unsqueeze(1)
+    picked, e_picked = z.gather(1, at).squeeze(1), ez.gather(1, at).squeeze(1)
+    g = torch.where(kept, rw.double(), 0.0)
+    near(loss.detach(), "losses", {"losses": (torch.where(kept, (lse - picked) * g, 0.0),
+                                              torch.where(kept, g * (e_lse + e_picked + 2.0 ** -21 * (1 + lse.abs() + picked.abs())), 0.0))})
+    # log of what the others' exponentials come to, without entry u: [n][v]
+    others = lambda x: torch.logsumexp(x.unsqueeze(1).expand(n, v, v).masked_fill(torch.eye(v, dtype=torch.bool, device=DEV), -math.inf), 2)  # noqa: E731
+    p = torch.softmax(z, 1)
+    hi, lo = torch.sigmoid(z + ez - others(z - ez)), torch.sigmoid(z - ez - others(z + ez))
+    ep = torch.maximum(hi - p, p - lo) + p * (torch.where(open_, (z - lse.unsqueeze(1)).abs(), 0.0) + 2) * 2.0 ** -22
+    d = p.scatter_add(1, at, torch.full_like(p[:, :1], -1.0))
+    d, ep = torch.where(kept.unsqueeze(1), d, 0.0), torch.where(kept.unsqueeze(1), ep, 0.0)
+    masked = (b == -math.inf).unsqueeze(1)
+    W, wm = W.masked_fill(masked, 0.0), wm.masked_fill(masked, 0.0)
+    H, hm = H.masked_fill(~kept.unsqueeze(1), 0.0), hm.masked_fill(~kept.unsqueeze(1), 0.0)
+    # the pieces' ends: of a row's entries 2^-38 of sqrt(its largest x the tensor's), of D 2^-39 of the square root of their ratio (2: odd exponents)
+    wend, dend = 2.0 ** -38 * 2 * (wm * wm.max()).sqrt(), 2.0 ** -39 * 2 * (wm.max() / wm.clamp(min=1e-30)).sqrt()
+    hend, gend = 2.0 ** -38 * 2 * (hm * hm.max()).sqrt(), 2.0 ** -39 * 2 * (hm.max() / hm.clamp(min=1e-30)).sqrt() * g.max()
+    want = (d @ W) * g.unsqueeze(1)
+    e = (ep + 2.0 ** -20 * d.abs() + (v / 16 + 80) * 2.0 ** -24 * d.abs() + dend.t() * kept.unsqueeze(1)) @ W.abs() + d.abs() @ wend.expand(v, k)
+    near(dh, "dh", {"dh": (want, e * g.unsqueeze(1) + 2.0 ** -21 * want.abs())})
+    gd = d * g.unsqueeze(1)
+    want = gd.t() @ H
+    e = ((ep + 2.0 ** -20 * d.abs() + (n / 16 + 80) * 2.0 ** -24 * d.abs()) * g.unsqueeze(1) + gend).t() @ H.abs() + gd.abs().t() @ hend.expand(n, k)
+    near(dw, "dw", {"dw": (want, e + 2.0 ** -21 * want.abs())})
+
+
+@pytest.mark.gpu
 def test_gpu_large_logits_of_operands_at_the_ends_of_the_range():
     """Logits of 5e4 from hidden of 1e35: what the operands were multiplied by is undone at once, not one factor after the other."""
     h, w, t, b, rw = inputs(64, 96, 150, F32, seed=9)
@@ -568,6 +620,34 @@ def test_gpu_c_calls_write_the_magnitudes_as_the_header_says(dtype):
     near(gh, "dh", out)
 
 
+@pytest.mark.gpu
+def test_gpu_c_calls_take_the_scales_that_the_forward_call_left():
+    """GRLHIP_ELEM_SCALES: the gradients are those of a backward call that reads the operands itself, bit for bit."""
+    n, k, v = 70, 100, 130
+    h, w, t, b, rw = inputs(n, k, v, F32, seed=18)
+    lib, stream = L.lib(), ctypes.c_void_p(torch.cuda.current_stream(DEV).cuda_stream)
+    f = lambda *s: torch.empty(*s, device=DEV)  # noqa: E731
+    losses, lse, count, total, one = f(n), f(n), f(1), f(1), torch.ones((), device=DEV)
+    scales = torch.empty(lib.grlhip_linear_ce_scales_bytes(n, v), dtype=torch.uint8, device=DEV)
+    ws = [torch.empty(lib.grlhip_linear_ce_workspace_bytes(h.data_ptr(), None, w.data_ptr(), None, n, k, v, L.ELEM_F32, back), dtype=torch.uint8, device=DEV)
+          for back in (0, 1)]
+    head = (h.data_ptr(), None, w.data_ptr(), None, b.data_ptr(), t.data_ptr(), -100, rw.data_ptr(), n, k, v)
+    L.check(lib.grlhip_linear_ce_forward(*head, L.ELEM_F32 | L.ELEM_SCALES, L.REDUCE_MEAN, losses.data_ptr(), lse.data_ptr(), total.data_ptr(),
+                                         count.data_ptr(), scales.data_ptr(), ws[0].data_ptr(), ws[0].numel(), stream))
+    results = []
+    for elem, given in ((L.ELEM_F32 | L.ELEM_SCALES, scales.data_ptr()), (L.ELEM_F32, None), (L.ELEM_F32 | L.ELEM_SCALES, None)):
+        grads = f(n, k), f(v, k), f(v)
+        ws[1].fill_(0x3f)
+        L.check(lib.grlhip_linear_ce_backward(*head, elem, L.REDUCE_MEAN, lse.data_ptr(), count.data_ptr(), given, one.data_ptr(), 0,
+                                              *(g.data_ptr() for g in grads), ws[1].data_ptr(), ws[1].numel(), stream))
+        results.append(grads)
+    out = oracle(h, w, t, b, rw, "mean")
+    near(total[0], "total", out)
+    for k, name in enumerate(("dh", "dw", "db")):
+        near(results[0][k], name, out)
+        assert torch.equal(results[0][k], results[1][k]) and torch.equal(results[0][k], results[2][k])
+
+
 # ------------------------------------------------------------------------------------------------- refusals, on the CPU
 def test_refusals_of_the_python_call():
     h, w, t = torch.randn(4, 8), torch.randn(10, 8), torch.zeros(4, dtype=torch.int64)
@@ -611,3 +691,19 @@ def test_c_entry_points_check_their_arguments_without_a_gpu():
         assert bwd(**{bad: None}) == -1, bad
     assert fwd(n=0) == -1 and fwd(elem=9) == -1 and fwd(red=3) == -1 and fwd(n=1 << 21) == -2 and fwd(ws=ctypes.c_void_p(p.value + 8)) == -1
     assert bwd(gh=None) == 0      # nothing is asked for
+
+
+def test_c_scales_check_their_arguments_without_a_gpu():
+    lib = L.lib()
+    size = lib.grlhip_linear_ce_scales_bytes
+    assert size(5, 7) >= 4 * 12 and size(5, 7) % 256 == 0 and size(1 << 20, 1 << 21) >= 4 * 3 * (1 << 20)
+    assert size(0, 7) == size(5, 0) == size((1 << 20) + 1, 7) == size(5, (1 << 21) + 1) == 0
+    buf = (ctypes.c_char * 512)()
+    p = ctypes.c_void_p((ctypes.addressof(buf) + 255) // 256 * 256)
+    odd = ctypes.c_void_p(p.value + 64)
+    fwd = lambda elem, scales: lib.grlhip_linear_ce_forward(p, None, p, None, None, p, -100, None, 4, 8, 10, elem, L.REDUCE_MEAN, p, p, p, p, scales, p, 1, None)  # noqa: E731
+    bwd = lambda elem, scales: lib.grlhip_linear_ce_backward(p, None, p, None, None, p, -100, None, 4, 8, 10, elem, L.REDUCE_MEAN, p, p, scales, p, 0, p, None, None, p, 1, None)  # noqa: E731
+    for call in (fwd, bwd):
+        assert call(L.ELEM_F32 | L.ELEM_SCALES, p) == -4                 # the workspace is too small; the rest is fine
+        assert call(L.ELEM_F32 | L.ELEM_SCALES, odd) == -1 and call(L.ELEM_F32, odd) == -4
+        assert call(L.ELEM_BF16 | L.ELEM_SCALES, p) == call(L.ELEM_F16 | L.ELEM_SCALES, p) == call(L.ELEM_SCALES << 1, p) == -1
