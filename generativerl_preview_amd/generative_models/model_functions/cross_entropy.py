@@ -5,6 +5,7 @@ import ctypes
 import weakref
 
 import torch
+from torch.autograd import forward_ad
 
 from ... import _lib as L
 from ...engine import _on
@@ -19,6 +20,12 @@ def _address(t):
 
 def _strides(t):
     return None if t.is_contiguous() else (ctypes.c_int64 * 2)(*t.stride())
+
+
+def _has_tangent(*tensors):
+    if getattr(forward_ad, "_current_level", 0) < 0:   # no dual level, no dual tensor: the question costs 1 us a tensor
+        return False
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 class _Head:
@@ -153,7 +160,7 @@ def linear_cross_entropy(hidden, weight, target, bias=None, row_weight=None, ign
     ``reduction``: ``"none"`` (losses of target's shape), ``"sum"``, or ``"mean"`` -- the weighted sum over the number of rows
     that are not ignored (0 when there are none).  The loss is fp32.
 
-    Differentiable (once) with respect to hidden, weight and bias; the gradients have the operands' types.  Logits are never stored:
+    Differentiable (once, in reverse mode) with respect to hidden, weight and bias; the gradients have the operands' types.  Logits are never stored:
     the forward pass keeps one logsumexp per row, the backward pass recomputes them in pieces of the vocabulary.  With
     ``reduction="none"`` and no gradient this is the negative log-probability of single tokens (serving).  While a HIP graph is
     captured, no eager loss over the same leaves from the default stream may be alive: such a call is refused
@@ -186,6 +193,8 @@ def linear_cross_entropy(hidden, weight, target, bias=None, row_weight=None, ign
             raise ValueError("row_weight: expected shape %s, got %s" % (tuple(target.shape), tuple(row_weight.shape)))
         if row_weight.requires_grad:
             raise ValueError("row_weight: no gradient is taken to the weights of rows; detach them")
+    if _has_tangent(hidden, weight, bias, row_weight):
+        raise NotImplementedError("linear_cross_entropy has no forward-mode derivative")
     dev = hidden.device
     if dev.type != "cuda":
         raise L.GrlHipError("hidden must live on a HIP device (got %s): there is no CPU fallback" % dev)

@@ -665,6 +665,19 @@ def test_refusals_of_the_python_call():
             bad()
 
 
+def test_forward_mode_derivatives_are_refused():
+    """A dual tensor requires no gradient; a result without a tangent would be a derivative of zero."""
+    import torch.autograd.forward_ad as fad
+    h, w, t, b, r = torch.randn(4, 8), torch.randn(10, 8), torch.zeros(4, dtype=torch.int64), torch.randn(10), torch.rand(4)
+    with fad.dual_level():
+        dual = lambda x: fad.make_dual(x, torch.ones_like(x))  # noqa: E731
+        for args, kw in (((dual(h), w, t), {}), ((h, dual(w), t), {}), ((h, w, t), dict(bias=dual(b))), ((h, w, t), dict(row_weight=dual(r)))):
+            with pytest.raises(NotImplementedError, match="forward"):
+                linear_cross_entropy(*args, **kw)
+        with pytest.raises(L.GrlHipError, match="HIP device"):
+            linear_cross_entropy(h, w, t, bias=b, row_weight=r)
+
+
 def test_c_entry_points_check_their_arguments_without_a_gpu():
     lib = L.lib()
     size = lambda n=4, k=8, v=10, elem=L.ELEM_F32, back=0: lib.grlhip_linear_ce_workspace_bytes(None, None, None, None, n, k, v, elem, back)  # noqa: E731
