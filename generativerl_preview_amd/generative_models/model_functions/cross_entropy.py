@@ -2,6 +2,7 @@
 discretised actions (behaviour cloning, or advantage-weighted with ``row_weight``), beside the fused losses of the continuous
 models.  ``grlhip_linear_ce_forward`` / ``grlhip_linear_ce_backward``."""
 import ctypes
+import threading
 import weakref
 
 import torch
@@ -90,7 +91,8 @@ class _Graph:
         self.roots = roots
 
 
-_ON_DEFAULT_STREAM = weakref.WeakSet()
+_ON_DEFAULT_STREAM = weakref.WeakSet()   # of all threads and devices
+_WATCH = threading.RLock()               # one thread's capture looks through it while others add to it
 
 
 def _leaves(roots):
@@ -121,13 +123,16 @@ def _watch(ctx, *tensors):
     if not roots:
         return
     if torch.cuda.is_current_stream_capturing():
-        live = [r for graph in list(_ON_DEFAULT_STREAM) for r in graph.roots]
+        with _WATCH:
+            graphs = list(_ON_DEFAULT_STREAM)
+        live = [r for graph in graphs for r in graph.roots]
         if live and _leaves(roots).keys() & _leaves(live).keys():
             raise L.GrlHipError("linear_cross_entropy under graph capture: an eager loss of the same leaves, computed on the "
                                 "default stream, is still alive; drop it (del loss) before the capture")
     elif torch.cuda.current_stream(tensors[0].device).cuda_stream == 0:
         ctx.graph = _Graph(roots)
-        _ON_DEFAULT_STREAM.add(ctx.graph)
+        with _WATCH:
+            _ON_DEFAULT_STREAM.add(ctx.graph)
 
 
 class _LinearCrossEntropy(torch.autograd.Function):

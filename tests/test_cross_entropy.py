@@ -678,6 +678,45 @@ def test_forward_mode_derivatives_are_refused():
             linear_cross_entropy(h, w, t, bias=b, row_weight=r)
 
 
+def test_watching_live_losses_from_several_threads(monkeypatch):
+    """Losses that come and go on other threads while one thread looks through the live ones, as it does under capture."""
+    import sys
+    import threading
+    import types
+    from generativerl_preview_amd.generative_models.model_functions import cross_entropy as ce
+    me = threading.get_ident()
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: threading.get_ident() == me)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: types.SimpleNamespace(cuda_stream=0))
+    leaves = [torch.zeros(1, requires_grad=True) for _ in range(4)]
+    stop, failed = threading.Event(), []
+
+    def work(leaf):
+        kept = []
+        try:
+            while not stop.is_set():
+                kept.append(types.SimpleNamespace())
+                ce._watch(kept[-1], leaf)
+                if len(kept) > 40:
+                    del kept[::2]
+        except Exception as e:  # noqa: BLE001
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(x,)) for x in leaves]
+    interval = sys.getswitchinterval()
+    try:
+        sys.setswitchinterval(1e-6)
+        for th in threads:
+            th.start()
+        for _ in range(300):
+            ce._watch(types.SimpleNamespace(), torch.zeros(1, requires_grad=True))
+    finally:
+        sys.setswitchinterval(interval)
+        stop.set()
+        for th in threads:
+            th.join()
+    assert not failed
+
+
 def test_c_entry_points_check_their_arguments_without_a_gpu():
     lib = L.lib()
     size = lambda n=4, k=8, v=10, elem=L.ELEM_F32, back=0: lib.grlhip_linear_ce_workspace_bytes(None, None, None, None, n, k, v, elem, back)  # noqa: E731
