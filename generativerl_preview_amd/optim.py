@@ -135,14 +135,55 @@ def _matrices(tensors, name, like=None):
     return [t.data_ptr() if t.numel() else 0 for t in tensors], dense
 
 
-def _written(tensors, pointers, dense, name):
-    """What is written must not overlap itself; the addresses of its matrices, without the empty ones'."""
-    if not dense and any(st == 0 and n > 1 for t in tensors for st, n in zip(t.stride(), t.shape)):
-        raise ValueError("%s: a matrix that is written to must not share memory with itself" % name)
-    seen = {p for p in pointers if p}
-    if len(seen) != sum(1 for p in pointers if p):
-        raise ValueError("%s: the matrices are written to and must not share memory" % name)
-    return seen
+def _meets_itself(t):
+    """Whether two entries of a matrix lie at one place: i s0 = j s1 for some i, j inside of it."""
+    (rows, cols), (s0, s1) = t.shape, t.stride()
+    if rows < 2 or cols < 2:
+        return max(rows, cols) > 1 and min(rows, cols) > 0 and (s0 if rows > 1 else s1) == 0
+    g = math.gcd(s0, s1)
+    return g == 0 or (s1 // g < rows and s0 // g < cols)
+
+
+def _share(a, b):
+    """Whether two matrices of 4-byte entries, none of which meets itself, have a place in common."""
+    away, part = divmod(b.data_ptr() - a.data_ptr(), 4)
+    if part:
+        return True
+    # axes of one entry have any stride: the other matrix' one; the larger stride first
+    strides = [(x if n > 1 else y, y if m > 1 else x) for x, y, n, m in zip(a.stride(), b.stride(), a.shape, b.shape)]
+    if strides[0][0] == strides[0][1] and strides[1][0] == strides[1][1]:
+        # slices of one buffer: i s + j t = away for some i, j between -(sizes of b) and the sizes of a
+        (s, n, m), (t, p, q) = sorted(((x, n, m) for (x, _), n, m in zip(strides, a.shape, b.shape)), reverse=True)
+        return any((away - j * t) % s == 0 and -m < (away - j * t) // s < n for j in range(1 - q, p)) if s else away == 0
+    if a.numel() + b.numel() > 1 << 24:
+        return True
+    places = lambda x, at: (at + torch.arange(x.shape[0])[:, None] * x.stride(0) + torch.arange(x.shape[1]) * x.stride(1)).view(-1)  # noqa: E731
+    return bool(torch.isin(places(a, 0), places(b, away)).any())
+
+
+def _check_memory(lists, pointers, dense):
+    """``lists``: parameters, gradients, momentum buffers.  What is written, all but the gradients, shares no memory with itself or with
+    anything else.  Ranges of addresses first; the matrices behind them are looked at where these meet."""
+    if not all(dense) and any(_meets_itself(t) for k in (0, 2) for t in lists[k]):
+        raise ValueError("muon_step: a matrix that is written to must not share memory with itself")
+    spans = sorted((at, at + 4 * (t.numel() if d else 1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))), k, i)
+                   for k, (ts, ats, d) in enumerate(zip(lists, pointers, dense)) for i, (t, at) in enumerate(zip(ts, ats)) if at)
+    written = read = 0      # where those so far end
+    meet = False
+    for at, end, k, _ in spans:
+        meet = meet or at < written or (k != 1 and at < read)
+        if k == 1:
+            read = max(read, end)
+        else:
+            written = max(written, end)
+    if not meet:
+        return
+    for n, (at, end, k, i) in enumerate(spans):
+        for at2, end2, k2, i2 in spans[n + 1:]:
+            if at2 >= end:
+                break
+            if not k == k2 == 1 and _share(lists[k][i], lists[k2][i2]):
+                raise ValueError("muon_step: parameters, gradients and momentum buffers must not share memory")
 
 
 def _pointers(addresses):
@@ -225,9 +266,7 @@ def muon_step(params, grads, momentum_buffers, lr, momentum=0.95, nesterov=True,
     for name, ts in (("params", params), ("grads", grads), ("momentum_buffers", bufs)):
         if ts[0].dtype != torch.float32:
             raise TypeError("%s: expected float32, got %s" % (name, ts[0].dtype))
-    ps, bs = _written(params, pp, pd, "params"), _written(bufs, bp, bd, "momentum_buffers")
-    if not bs.isdisjoint(ps) or not bs.isdisjoint(gp) or not ps.isdisjoint(gp):
-        raise ValueError("muon_step: parameters, gradients and momentum buffers must not share memory")
+    _check_memory((params, grads, bufs), (pp, gp, bp), (pd, gd, bd))
     sides = [t.shape for t in params]
     rates = (ctypes.c_float * len(params))(*(
         [lr * math.sqrt(max(1.0, r / max(c, 1))) for r, c in sides] if adjust_lr == "original" else

@@ -350,6 +350,60 @@ def test_gpu_refusals_that_need_device_tensors():
         optim.orthogonalize(m, steps=-1)
 
 
+def test_shared_memory_is_found_exactly():
+    """Against the sets of places, for slices, transposes and strange strides of one buffer."""
+    buf = torch.zeros(400)
+    views = [buf.as_strided(size, stride, at) for size in ((3, 4), (1, 5), (4, 1), (2, 2), (5, 6), (1, 1), (0, 3)) for stride in ((10, 1), (1, 10), (6, 2), (2, 3), (5, 5), (0, 1))
+             for at in (0, 1, 4, 7, 13)]
+    places = lambda t: [t.storage_offset() + i * t.stride(0) + j * t.stride(1) for i in range(t.shape[0]) for j in range(t.shape[1])]  # noqa: E731
+    sets = [set(places(t)) for t in views]
+    plain = []
+    for t, s in zip(views, sets):
+        assert optim._meets_itself(t) == (len(s) < t.numel()), (t.shape, t.stride())
+        if len(s) == t.numel() > 0:
+            plain.append((t, s))
+    for t, s in plain:
+        for u, r in plain:
+            assert optim._share(t, u) == bool(s & r), (t.shape, t.stride(), t.storage_offset(), u.shape, u.stride(), u.storage_offset())
+
+
+def test_matrices_that_share_memory_are_refused():
+    def check(p, g, b):
+        lists = tuple([x] if torch.is_tensor(x) else x for x in (p, g, b))
+        optim._check_memory(lists, [[t.data_ptr() if t.numel() else 0 for t in ts] for ts in lists], [all(t.is_contiguous() for t in ts) for ts in lists])
+
+    big, other, third = torch.zeros(12, 10), torch.zeros(12, 10), torch.zeros(24, 10)
+    for bad in (([big[:6], big[5:11]], [other[:6], other[6:]], [third[:6], third[6:12]]),       # parameters that overlap
+                (big[:6], big[3:9], third[:6]),                                                 # a gradient inside of a parameter
+                (big[:6], other[:6], other[4:10]),                                              # a buffer over a gradient
+                (big[:, :6], other[:, :6], big[:, 5:]),                                         # one column in common
+                (big[::2], other[::2], big[2:8]),                                                    # rows 2, 4 and 6 of both
+                (big.as_strided((3, 3), (2, 2)), other[:3, :3], third[:3, :3])):                # a parameter that meets itself
+        with pytest.raises(ValueError, match="share memory"):
+            check(*bad)
+    # one buffer, no place in common: halves of its columns, every other row, rows beside each other; gradients may share
+    check([big[:, :5], big[:, 5:]], [other[:, :5], other[:, :5]], [third[:12, :5], third[12:, 5:]])
+    check(big[::2], big[1::2], other[::2])
+    check([big[:6], big[6:]], [other[:6], other[2:8]], [third[:6], third[6:12]])
+    check([big[:, :1].t(), big[:0]], [other[:, :1].t(), other[:0]], [big[:, 1:2].t(), other[:0]])
+
+
+@pytest.mark.gpu
+def test_gpu_muon_step_refuses_matrices_that_overlap_and_takes_those_that_do_not():
+    big, g = torch.randn(20, 30, device=DEV), [grad_like(10, 30), grad_like(10, 30, seed=1)]
+    with pytest.raises(ValueError, match="share memory"):
+        optim.muon_step([big[:10], big[9:19]], g, [torch.zeros(10, 30, device=DEV) for _ in range(2)], lr=0.1)
+    # interleaved rows and buffers in one tensor: the same step as of copies
+    store = torch.zeros(20, 60, device=DEV)
+    want_p, want_b = [big[::2].clone(), big[1::2].clone()], [torch.zeros(10, 30, device=DEV) for _ in range(2)]
+    optim.muon_step(want_p, g, want_b, lr=0.1)
+    bufs = [store[:10, :30], store[:10, 30:]]
+    optim.muon_step([big[::2], big[1::2]], g, bufs, lr=0.1)
+    for got, want in zip((big[::2], big[1::2], *bufs), (*want_p, *want_b)):
+        assert torch.equal(got, want)
+    assert not store[10:].any()
+
+
 def test_c_entry_points_check_their_arguments_without_a_gpu():
     lib = L.lib()
     shapes = (ctypes.c_int64 * 2)(8, 8)
