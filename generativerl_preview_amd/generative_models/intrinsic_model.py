@@ -10,7 +10,7 @@ import torch.nn as nn
 
 from .. import _lib as L
 from ..config import as_config
-from ..engine import NetPlan, differentiable_forward
+from ..engine import NetPlan, differentiable_forward, packed_image
 from ..neural_network import ConcatenateMLP, TemporalSpatialResidualNet, get_module
 from ..neural_network.encoders import GaussianFourierProjectionTimeEncoder, get_encoder
 
@@ -35,7 +35,8 @@ class IntrinsicModel(nn.Module):
 
     # derived HIP state (plan handle, packed images, gradient staging) is never copied or pickled: a deep copy
     # (target networks) or a checkpoint rebuilds it lazily from the parameters
-    _DERIVED = ("_plan", "_packed", "_flat_grads", "_grad_stage", "_stage_token")
+    _DERIVED = ("_plan", "_packed", "_flat_grads", "_grad_stage", "_stage_token", "_in_graph")
+    _in_graph = False   # see packed_image (engine.py)
 
     def __getstate__(self):
         st = dict(self.__dict__)
@@ -95,10 +96,8 @@ class IntrinsicModel(nn.Module):
     def packed(self, dtype=None):
         dtype = self.compute_dtype if dtype is None else dtype
         named = self._named()
-        key = tuple((p.data_ptr(), p._version) for p in named.values())
-        hit = self._packed.get(dtype)
-        if hit is None or hit[0] != key:
-            hit = (key, self.plan.pack(named, dtype))
+        hit = packed_image(self, self._packed.get(dtype), named, dtype)
+        if hit[0] is not None:
             self._packed[dtype] = hit
         return hit[1]
 

@@ -105,6 +105,8 @@ class FlatAdam:
         # packed-image cache (IntrinsicModel.packed) is keyed on them -- drop it explicitly
         if hasattr(self.owner, "_packed"):
             self.owner._packed = {} if isinstance(self.owner._packed, dict) else None
+            if torch.cuda.is_current_stream_capturing():   # every replay writes them
+                self.owner._in_graph = True
 
     def state_dict(self):
         return {"step": self.step_count, "exp_avg": self.exp_avg.clone(), "exp_avg_sq": self.exp_avg_sq.clone(),
@@ -252,7 +254,8 @@ def muon_step(params, grads, momentum_buffers, lr, momentum=0.95, nesterov=True,
     with lr' = lr sqrt(max(1, rows / cols)) for ``adjust_lr="original"`` and 0.2 lr sqrt(max(rows, cols)) for
     ``"match_rms_adamw"`` (updates of the size of Adam's).  Any strides; the three lists must not share memory.  ``lr`` and the
     other numbers are read on the host: a captured graph keeps the ones it was captured with.  The call counts as an in-place
-    operation on the parameters and buffers (their version counters move; a replay of a captured graph moves none)."""
+    operation on the parameters and buffers (their version counters move; a replay of a captured graph moves none, and a
+    network of this framework that was not captured with the step does not see it)."""
     params, grads, bufs = list(params), list(grads), list(momentum_buffers)
     if not len(params) == len(grads) == len(bufs):
         raise ValueError("muon_step: %d parameters, %d gradients, %d momentum buffers" % (len(params), len(grads), len(bufs)))

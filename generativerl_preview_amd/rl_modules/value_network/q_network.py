@@ -10,7 +10,7 @@ import torch.nn as nn
 
 from ... import _lib as L
 from ...config import as_config
-from ...engine import NetPlan, differentiable_forward
+from ...engine import NetPlan, differentiable_forward, packed_image
 from ...neural_network import ConcatenateMLP, get_module
 
 
@@ -29,6 +29,8 @@ class QNetwork(nn.Module):
         self._plan = None
         self._io_dims = None
         self._packed = None
+
+    _in_graph = False   # see packed_image (engine.py)
 
     def __deepcopy__(self, memo):
         twin = QNetwork(self.config)
@@ -66,10 +68,10 @@ class QNetwork(nn.Module):
 
     def packed(self, dtype=L.F32):
         named = self._named()
-        key = tuple((p.data_ptr(), p._version) for p in named.values())
-        if self._packed is None or self._packed[0] != key or self.always_repack:
-            self._packed = (key, self.plan.pack(named, L.F32))
-        return self._packed[1]
+        hit = packed_image(self, None if self.always_repack else self._packed, named, L.F32)
+        if hit[0] is not None:
+            self._packed = hit
+        return hit[1]
 
     # ------------------------------------------------------------------ reference API
     def forward(self, action, state):

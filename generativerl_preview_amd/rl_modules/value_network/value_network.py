@@ -6,7 +6,7 @@ import torch.nn as nn
 
 from ... import _lib as L
 from ...config import as_config
-from ...engine import NetPlan, differentiable_forward
+from ...engine import NetPlan, differentiable_forward, packed_image
 from ...neural_network import MultiLayerPerceptron, get_module
 
 
@@ -24,10 +24,12 @@ class VNetwork(nn.Module):
         self._plan = None
         self._packed = None
 
+    _in_graph = False   # see packed_image (engine.py)
+
     def __getstate__(self):   # the plan handle and packed image are derived state: never copied or pickled
         st = dict(self.__dict__)
         st["_plan"], st["_packed"] = None, None
-        st.pop("_flat_grads", None); st.pop("_grad_stage", None); st.pop("_stage_token", None)
+        st.pop("_flat_grads", None); st.pop("_grad_stage", None); st.pop("_stage_token", None); st.pop("_in_graph", None)
         return st
 
     @property
@@ -48,10 +50,10 @@ class VNetwork(nn.Module):
 
     def packed(self, dtype=L.F32):
         named = self._named()
-        key = tuple((p.data_ptr(), p._version) for p in named.values())
-        if self._packed is None or self._packed[0] != key:
-            self._packed = (key, self.plan.pack(named, L.F32))
-        return self._packed[1]
+        hit = packed_image(self, self._packed, named, L.F32)
+        if hit[0] is not None:
+            self._packed = hit
+        return hit[1]
 
     def forward(self, state, condition=None):
         """:48-70"""

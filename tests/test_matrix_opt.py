@@ -308,6 +308,81 @@ def test_gpu_a_weight_stepped_between_forward_and_backward_is_noticed():
         loss.backward()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("make", [optim.FlatMuon, optim.FlatAdam])
+@pytest.mark.parametrize("before,between", [(True, False), (False, True), (True, True)])
+def test_gpu_captured_steps_and_eager_passes_see_each_others_weights(make, before, between):
+    """Forward passes before the capture, and between the replays: the captured loss follows the weights, and so do the passes."""
+    kind, cfg, a = um.build("small_icfm", DEV)
+    kind, cfg, b = um.build("small_icfm", DEV)
+    b.load_state_dict(copy.deepcopy(a.state_dict()))
+    oa, ob = (make(m.model, lr=0.01, capturable=True) for m in (a, b))
+    gen = torch.Generator().manual_seed(9)
+    B = 300
+    x0, x1 = torch.randn(B, 6, generator=gen).to(DEV), torch.rand(B, 6, generator=gen).to(DEV)
+    cond, t, eps = torch.randn(B, 17, generator=gen).to(DEV), torch.rand(B, generator=gen).to(DEV), torch.randn(B, 6, generator=gen).to(DEV)
+
+    def step(m, o):
+        o.zero_grad()
+        loss = m.flow_matching_loss(x0, x1, cond, t=t, noise=eps)
+        loss.backward()
+        o.step()
+        return loss.detach()
+
+    def look(m):
+        with torch.no_grad():
+            return m.model(t, x0, cond).clone()
+
+    side = torch.cuda.Stream(device=DEV)
+    side.wait_stream(torch.cuda.current_stream(DEV))
+    with torch.cuda.stream(side):
+        step(b, ob)
+    torch.cuda.current_stream(DEV).wait_stream(side)
+    step(a, oa)
+    if before:
+        assert torch.equal(look(a), look(b))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step(b, ob)
+    for k in range(4):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(held, step(a, oa)), k
+        if between:
+            assert torch.equal(look(a), look(b)), k
+    assert torch.equal(look(a), look(b))
+
+
+def _q_net():
+    from generativerl_preview_amd.rl_modules.value_network.q_network import QNetwork
+    net = QNetwork(dict(backbone=dict(type="ConcatenateMLP", args=dict(hidden_sizes=[17, 64, 64], output_size=1, activation="relu")))).to(DEV)
+    net.set_io_dims(6, 11)
+    return net
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("make,inputs", [(_residual_net, ((50,), (50, 11))), (_value_net, ((50, 17),)), (_q_net, ((50, 6), (50, 11)))])
+def test_gpu_a_captured_forward_pass_follows_the_weights(make, inputs):
+    torch.manual_seed(12)
+    net, fresh = make(), make()
+    x = [torch.rand(s, device=DEV) for s in inputs]
+    with torch.no_grad():
+        net(*x)                                  # what is packed already must not be what the graph reads
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held = net(*x)
+        for k in range(3):
+            for p in net.parameters():
+                p.mul_(0.5 + k)
+            fresh.load_state_dict(net.state_dict())
+            want = fresh(*x)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(held, want) and torch.equal(net(*x), want)
+    twin = copy.deepcopy(net)
+    assert not twin._in_graph and torch.equal(twin(*x), want)
+
+
 # ------------------------------------------------------------------------------------------------- refusals, on the CPU
 def test_refusals_of_the_python_calls():
     m = torch.randn(4, 5)
