@@ -303,7 +303,7 @@ def packed_image(owner, kept, named, dtype):
     written in place, else anew.  Replays of a captured graph write parameters without moving their version counters, and meet
     parameters that were written since: what is captured packs for itself (key None: memory of the graph, not to be kept), and
     a network that was captured once trusts nothing that it kept."""
-    if torch.cuda.is_current_stream_capturing():
+    if next(iter(named.values())).is_cuda and torch.cuda.is_current_stream_capturing():
         owner._in_graph = True
         return None, owner.plan.pack(named, dtype)
     key = tuple((p.data_ptr(), p._version) for p in named.values())
