@@ -300,12 +300,10 @@ struct Logits {
   Operand w, h;             // rows of the weight piece, rows of hidden
   const float* bias;        // of the piece, or null
   const int64_t* target;
-  const float* row_weight;
   const float* lse;         // backward
   const float* scale;       // backward: gradient of each row's loss (0: the row does not count)
   const Scalars* s;
   const int *hs, *ws;       // fp32: the exponents of the rows' scales, of hidden and of the piece
-  int64_t ignore;
   int rows, v0, cols;       // rows; first vocabulary entry and entries of the piece
   int nkb;                  // K blocks
   // forward
