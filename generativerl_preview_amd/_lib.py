@@ -83,6 +83,8 @@ PROTOTYPES = {
                                         _vp, _sz, _vp]),
     "grlhip_linear_ce_workspace_bytes": (_sz, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, ctypes.c_int, ctypes.c_int]),
     "grlhip_linear_ce_scales_bytes": (_sz, [_i64, _i64]),
+    "grlhip_linear_ce_tiles": (ctypes.c_int, [_i64, _i64, _i64, ctypes.c_int, _vp]),
+    "grlhip_orthogonalize_tiles": (ctypes.c_int, [_vp, _i32, _vp]),
     "grlhip_linear_ce_forward": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _i64, _i64, ctypes.c_int,
                                                 ctypes.c_int, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "grlhip_linear_ce_backward": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _i64, _i64, ctypes.c_int,

@@ -1100,6 +1100,22 @@ size_t grlhip_linear_ce_workspace_bytes(const void* hidden, const int64_t* hidde
   });
 }
 
+int grlhip_linear_ce_tiles(int64_t rows, int64_t features, int64_t vocab, int elem, int32_t* kinds) {
+  return guarded([&]() -> int {
+    Call a = {};
+    a.c = {rows, features, vocab, elem};
+    a.h = a.w = kinds;
+    a.target = (const int64_t*)kinds;
+    if (const int rc = check("linear_ce_tiles", a)) return rc;
+    const bool in_place = direct(nullptr, features, 1, a.c);
+    const Layout forward = layout_of(a.c, in_place, in_place, false, false), backward = layout_of(a.c, in_place, in_place, true, true);
+    kinds[0] = forward.kind_z;
+    kinds[1] = backward.kind_z;
+    kinds[2] = backward.kind_g;
+    return 0;
+  });
+}
+
 int grlhip_linear_ce_forward(const void* hidden, const int64_t* hidden_strides, const void* weight, const int64_t* weight_strides, const float* bias,
                              const int64_t* target, int64_t ignore_index, const float* row_weight, int64_t rows, int64_t features, int64_t vocab,
                              int elem, int reduction, float* losses, float* lse, float* total, float* count, float* largest, void* workspace, size_t workspace_bytes, void* stream) {

@@ -613,6 +613,14 @@ Plan plan_of(const int64_t* shapes, int count) {
   return plan;
 }
 
+bool all_small(const int64_t* shapes, int count) {
+  for (int i = 0; i < count; ++i) {
+    const Parts p = parts_of(shapes + 2 * i);
+    if (p.mp > 0 && p.np > 0 && (p.mp > SMALL_M || p.np > SMALL_N)) return false;
+  }
+  return true;
+}
+
 template <class C, int STAGE, class T, bool MUON>
 int launch(const Table& t, const Numbers& num, int k, int64_t tiles, hipStream_t stream) {
   const auto kernel = k_orth_product<C, STAGE, T, MUON>;
@@ -671,12 +679,7 @@ int run(const char* who, const Call& c, char* ws, size_t ws_bytes, hipStream_t s
   const int present = (int)order.size();
   if (present == 0) return 0;
   const Numbers num{c.ca, c.cb, c.cc, c.eps, (float)c.momentum, (float)(1.0 - c.momentum), c.keep, c.nesterov};
-  bool small = true;
-  for (const int i : order) {
-    const Parts p = parts_of(c.shapes + 2 * i);
-    small = small && p.mp <= SMALL_M && p.np <= SMALL_N;
-  }
-  if (small) {
+  if (all_small(c.shapes, c.count)) {
     const auto kernel = k_orth_small<T, MUON>;
     LAUNCH_TRY(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, SMALL_LDS));
     for (int done = 0; done < present;) {
@@ -757,6 +760,17 @@ extern "C" {
 
 size_t grlhip_orthogonalize_workspace_bytes(const int64_t* shapes, int32_t count) {
   return guarded_size([&]() -> size_t { return check_shapes("orthogonalize", shapes, count) ? 0 : (size_t)workspace_bytes(shapes, count); });
+}
+
+int grlhip_orthogonalize_tiles(const int64_t* shapes, int32_t count, int32_t* kinds) {
+  return guarded([&]() -> int {
+    if (const int rc = check_shapes("orthogonalize", shapes, count)) return rc;
+    if (!kinds) return set_error(GRLHIP_ERR_INVALID, "orthogonalize_tiles: null kinds");
+    const bool small = all_small(shapes, count);
+    const Plan plan = plan_of(shapes, count);
+    for (int s = 0; s < 3; ++s) kinds[s] = small ? -1 : plan.kind[s];
+    return 0;
+  });
 }
 
 int grlhip_orthogonalize(const void* const* src, void* const* dst, const int64_t* shapes, const int64_t* strides, int32_t count, int elem,

@@ -358,6 +358,9 @@ typedef enum { GRLHIP_ELEM_F32 = 0, GRLHIP_ELEM_BF16 = 1, GRLHIP_ELEM_F16 = 2 } 
  * Coefficients that let a singular value pass 1.9 (or b s^2 + c s^4 pass 3.8) from 1 on: GRLHIP_ERR_UNSUPPORTED.
  * The results do not depend on the other matrices of the call.  Workspace: grlhip_orthogonalize_workspace_bytes, 256-byte aligned. */
 size_t grlhip_orthogonalize_workspace_bytes(const int64_t* shapes, int32_t count);
+/* For the tests: the kinds of tiles (in the order of their sizes) that a call of these matrices takes in its three products, -1 where all
+ * of them stay in one workgroup each. */
+int grlhip_orthogonalize_tiles(const int64_t* shapes, int32_t count, int32_t* kinds);
 int grlhip_orthogonalize(const void* const* src, void* const* dst, const int64_t* shapes, const int64_t* strides,
                          int32_t count, int elem, int32_t steps, float a, float b, float c, float eps,
                          void* workspace, size_t workspace_bytes, void* stream);
@@ -394,6 +397,9 @@ size_t grlhip_linear_ce_workspace_bytes(const void* hidden, const int64_t* hidde
                                         const int64_t* weight_strides, int64_t rows, int64_t features, int64_t vocab, int elem,
                                         int backward);
 size_t grlhip_linear_ce_scales_bytes(int64_t rows, int64_t vocab);
+/* For the tests: the kinds of tiles that calls of dense operands take for the logits of the forward pass, of the backward pass and for the
+ * gradients. */
+int grlhip_linear_ce_tiles(int64_t rows, int64_t features, int64_t vocab, int elem, int32_t* kinds);
 int grlhip_linear_ce_forward(const void* hidden, const int64_t* hidden_strides, const void* weight,
                              const int64_t* weight_strides, const float* bias, const int64_t* target, int64_t ignore_index,
                              const float* row_weight, int64_t rows, int64_t features, int64_t vocab, int elem, int reduction,

@@ -144,6 +144,21 @@ def test_gpu_forward_without_a_gradient_is_the_same_loss(dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES)
+def test_gpu_each_gradient_alone(dtype):
+    """What is not asked for is not computed; the rest is the same, bit for bit."""
+    for size in ((150, 72, 333), (40, 128, 5000)):
+        h, w, t, b, rw = inputs(*size, dtype, seed=41)
+        leaves = [h.requires_grad_(), w.requires_grad_(), b.requires_grad_()]
+        want = torch.autograd.grad(linear_cross_entropy(*leaves[:2], t, bias=b, row_weight=rw), leaves)
+        for chosen in ((0,), (1,), (2,), (0, 1), (0, 2), (1, 2)):
+            some = [x.detach().requires_grad_(k in chosen) for k, x in enumerate(leaves)]
+            loss = linear_cross_entropy(*some[:2], t, bias=some[2], row_weight=rw)
+            for g, k in zip(torch.autograd.grad(loss, [some[k] for k in chosen]), chosen):
+                assert torch.equal(g, want[k]), (size, chosen, k)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
 def test_gpu_pieces_of_the_vocabulary(dtype):
     """More rows than one piece of the vocabulary holds entries for: the gradients are added up over the pieces."""
     n, k, v = 50000, 64, 5000
@@ -646,6 +661,41 @@ def test_gpu_c_calls_take_the_scales_that_the_forward_call_left():
     for k, name in enumerate(("dh", "dw", "db")):
         near(results[0][k], name, out)
         assert torch.equal(results[0][k], results[1][k]) and torch.equal(results[0][k], results[2][k])
+
+
+# sizes that between them take every kind of tile for the logits, forward and backward, and for the gradients, with rests and more K blocks
+# than a tile's ring has stages
+KINDS = [(53, 213, 51), (66, 237, 17081), (131, 201, 41215), (133, 205, 51755), (2421, 691, 67), (7323, 685, 131), (8275, 663, 391)]
+
+
+def test_the_sizes_below_take_every_kind_of_tile():
+    lib, kinds = L.lib(), (ctypes.c_int32 * 3)()
+    for elem in (L.ELEM_F32, L.ELEM_BF16, L.ELEM_F16):
+        seen = [set(), set(), set()]
+        for n, k, v in KINDS:
+            assert lib.grlhip_linear_ce_tiles(n, k, v, elem, kinds) == 0
+            assert (kinds[0] == 0) == (kinds[1] == 0)      # the same sums of the logits in both passes
+            for s in range(3):
+                seen[s].add(kinds[s])
+        assert seen == [{0, 1, 2}] * 3, (elem, seen)
+    for n, k, v in ((1, 1, 1), (300, 200, 9000), (174, 70, 34497), (1000, 100, 2600), (1 << 20, 64, 5000), (7, 65536, 100000)):
+        for elem in (L.ELEM_F32, L.ELEM_BF16, L.ELEM_F16):
+            assert lib.grlhip_linear_ce_tiles(n, k, v, elem, kinds) == 0 and (kinds[0] == 0) == (kinds[1] == 0)
+    assert lib.grlhip_linear_ce_tiles(4, 8, 0, L.ELEM_F32, kinds) == -1 and lib.grlhip_linear_ce_tiles(4, 8, 9, 7, kinds) == -1
+    assert lib.grlhip_linear_ce_tiles(4, 8, 9, L.ELEM_F32, None) == -1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("size", KINDS)
+def test_gpu_every_kind_of_tile(size, dtype):
+    h, w, t, b, rw = inputs(*size, dtype, seed=61)
+    leaves = [h.requires_grad_(), w.requires_grad_(), b.requires_grad_()]
+    loss = linear_cross_entropy(h, w, t, bias=b, row_weight=rw)
+    out = oracle(h, w, t, b, rw, "mean")
+    near(loss.detach(), "total", out)
+    for g, name in zip(torch.autograd.grad(loss, leaves), ("dh", "dw", "db")):
+        near(g, name, out)
 
 
 # ------------------------------------------------------------------------------------------------- refusals, on the CPU

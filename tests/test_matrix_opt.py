@@ -383,6 +383,61 @@ def test_gpu_a_captured_forward_pass_follows_the_weights(make, inputs):
     assert not twin._in_graph and torch.equal(twin(*x), want)
 
 
+# groups that between them take every kind of tile in every product, with rests in all of them
+GROUPS = [(1, (65, 65)), (4, (646, 514)), (1, (193, 2)), (1, (2, 225)), (1, (226, 225)), (24, (195, 198)), (24, (225, 266)), (24, (292, 308)),
+          (12, (460, 455)), (24, (454, 464)), (24, (587, 594)), (12, (356, 370)), (24, (169, 161)), (24, (676, 33)), (8, (98, 3085)), (24, (1696, 97)),
+          (24, (193, 1411)), (8, (1432, 1411))]
+
+
+def test_the_groups_below_take_every_kind_of_tile():
+    lib, kinds, seen = L.lib(), (ctypes.c_int32 * 3)(), [set(), set(), set()]
+    for count, shape in GROUPS:
+        assert lib.grlhip_orthogonalize_tiles((ctypes.c_int64 * (2 * count))(*(shape * count)), count, kinds) == 0
+        for s in range(3):
+            seen[s].add(kinds[s])
+    assert seen == [set(range(9))] * 3, seen
+    assert lib.grlhip_orthogonalize_tiles((ctypes.c_int64 * 2)(64, 192), 1, kinds) == 0 and list(kinds) == [-1] * 3
+    assert lib.grlhip_orthogonalize_tiles((ctypes.c_int64 * 2)(64, 192), 1, None) == -1
+    assert lib.grlhip_orthogonalize_tiles((ctypes.c_int64 * 2)(-1, 192), 1, kinds) == -2
+
+
+def polar_on_the_gpu(g):
+    x = g.double()
+    tall = x.shape[0] > x.shape[1]
+    x = x.t().contiguous() if tall else x
+    x = x / float(torch.linalg.vector_norm(x))
+    for _ in range(5):
+        s = x @ x.t().contiguous()
+        x = ABC[0] * x + ABC[1] * (s @ x) + ABC[2] * (s @ (s @ x))
+    return x.t() if tall else x
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("group", range(len(GROUPS)))
+def test_gpu_every_kind_of_tile(group):
+    """Each type, and the optimiser step, of the first, a middle and the last matrix of each group."""
+    count, shape = GROUPS[group]
+    some = sorted({0, count // 2, count - 1})
+    gs = [grad_like(*shape, seed=100 * group + k) if k in some else 1e-3 * torch.randn(shape, device=DEV) for k in range(count)]
+    want = {k: polar_on_the_gpu(gs[k]) for k in some}
+    got = optim.orthogonalize(gs)
+    for k in some:
+        assert off(got[k], want[k]) <= TOL, k
+    for dtype in (torch.bfloat16, torch.float16):
+        half = [g.to(dtype) for g in gs]
+        got = optim.orthogonalize(half)
+        for k in some:
+            assert off(got[k], polar_on_the_gpu(half[k])) <= tol(dtype), (dtype, k)
+    ps, bufs = [torch.randn(shape, device=DEV) for _ in gs], [torch.zeros_like(g) for g in gs]
+    old = [p.double() for p in ps]
+    optim.muon_step(ps, gs, bufs, lr=0.05, momentum=0.9, nesterov=False, weight_decay=0.1)
+    rate = 0.05 * math.sqrt(max(1.0, shape[0] / shape[1]))
+    for k in some:      # the momentum is 0.1 of the gradient: the same direction
+        slip = float(torch.linalg.vector_norm(ps[k].double() - ((1 - 0.005) * old[k] - rate * want[k])))
+        change = float(torch.linalg.vector_norm(rate * want[k] + 0.005 * old[k]))
+        assert slip <= TOL * change + 2.0 ** -23 * float(torch.linalg.vector_norm(old[k])), k
+
+
 # ------------------------------------------------------------------------------------------------- refusals, on the CPU
 def test_refusals_of_the_python_calls():
     m = torch.randn(4, 5)
