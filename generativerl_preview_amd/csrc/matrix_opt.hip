@@ -568,11 +568,11 @@ constexpr int KINDS = 9, SIDE[KINDS] = {32, 32, 32, 64, 64, 96, 128, 128, 256}, 
 // A launch, in us: ALONE is a K block of 32 (two pieces, 3 MFMAs) of a tile with its CU to itself, FULL the CU's time for one of a full chip,
 // FIXED what a tile costs whatever its length, shared by the workgroups beside each other, EPILOGUE an entry's stores and loads.
 // Fitted to the times of 28 groups of matrices (one of 128 x 128 to 24 of 1024 x 4096) with each kind in each of the three products in turn:
-// in all of them but two the kind that the rule takes is within 1.5 % of the best call, in those within 3 %; 18 other groups: 2 %, and 5 % in
-// one.  Cards differ, launches of 64-wide tiles most (3 x 1000 x 777 with them 303 to 343 us, with 128-wide ones 311 to 325): their FULL is
-// 5 % above the fit, so that the wider tile has the ties.
+// in all of them but one the kind that the rule takes is within 1.5 % of the best call, and in that one within 3 %; 18 other groups: 2 %, and 5 % in one.
+// Near its ties it errs by more: of 135 random groups whose choice changes when FULL of the two-a-CU 64-wide tile is 5 % higher, the other
+// choice was 1.5 % slower on average, but 12 % faster in the best one (3 x 1000 x 777: 345 us by the fit, 329 by the other).
 constexpr double ALONE[KINDS] = {0.096, 0.131, 0.26, 0.224, 0.333, 0.48, 0.584, 0.646, 1.58};
-constexpr double FULL[KINDS] = {0.104, 0.09, 0.093, 0.222, 0.222, 0.474, 0.641, 0.563, 2.24};
+constexpr double FULL[KINDS] = {0.104, 0.09, 0.093, 0.222, 0.212, 0.474, 0.641, 0.563, 2.24};
 constexpr double FIXED[KINDS] = {1.74, 1.46, 1.19, 1.79, 1.16, 0.88, 2.72, 3.17, 2.64}, EPILOGUE = 1.2e-3;
 
 int64_t tiles_of(const Parts& p, int stage, int side) {

@@ -384,8 +384,8 @@ def test_gpu_a_captured_forward_pass_follows_the_weights(make, inputs):
 
 
 # groups that between them take every kind of tile in every product, with rests in all of them
-GROUPS = [(1, (65, 65)), (4, (646, 514)), (1, (193, 2)), (1, (2, 225)), (1, (226, 225)), (24, (195, 198)), (24, (225, 266)), (24, (292, 308)),
-          (12, (460, 455)), (24, (454, 464)), (24, (587, 594)), (12, (356, 370)), (24, (169, 161)), (24, (676, 33)), (8, (98, 3085)), (24, (1696, 97)),
+GROUPS = [(1, (65, 65)), (6, (660, 540)), (1, (193, 2)), (1, (2, 225)), (1, (226, 225)), (24, (195, 198)), (24, (225, 266)), (24, (292, 308)),
+          (12, (518, 523)), (24, (454, 464)), (24, (587, 594)), (12, (356, 370)), (24, (169, 161)), (24, (676, 33)), (8, (98, 3085)), (24, (1696, 97)),
           (24, (193, 1411)), (8, (1432, 1411))]
 
 
