@@ -5,8 +5,9 @@
 // target's logit; one pass over these partials gives logsumexp and the loss.  2 N V H flops.
 // Backward, one piece of the vocabulary at a time: z again (the same products in the same order), D = softmax - onehot written
 // in fp16 both ways round, D as [row][v] for dH += D W and D scaled by the row's gradient as [v][row] for dW = D^T H.  6 N V H
-// flops; the workspace holds D of one piece.  Recomputing z costs a third more products than keeping it would, and N V
-// floats less memory.
+// flops; the workspace holds D of one piece.  Recomputing z costs a third more products than keeping it would.  For that nothing of N V
+// entries outlives the forward pass.  At the peak, in the backward pass, it saves memory only where there are several pieces: one of up to
+// 2^27 entries holds D in 4 bytes an entry (bf16) or 8, as much as fp32 logits or twice that.
 //
 // Precision.  z: 16-bit operands are used as they are, fp32 ones as two fp16 pieces a value (gemm_core.hip.inc), each row of hidden and of the
 // weight scaled by a power of two of its own that brings its largest entry to 2^13..2^14: what is lost of a value is at most 2^-23 of it or 2^-38

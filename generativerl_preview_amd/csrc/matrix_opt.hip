@@ -51,7 +51,7 @@ struct Numbers {
 };
 // What the launches after the first know of the matrices lies in the workspace: `first` of all matrices, [4][count], and the
 // descriptions themselves.
-// A lone matrix comes with the kernel arguments instead: two trips to memory less in each launch.
+// To the products a lone matrix comes with the kernel arguments instead: two trips to memory less in each of these launches.
 struct Table { const int* first; const Mat* mat; int count; double* part; Mat one; };
 struct Group {
   Mat mat[GROUP];

@@ -168,8 +168,9 @@ def linear_cross_entropy(hidden, weight, target, bias=None, row_weight=None, ign
     Differentiable (once, in reverse mode) with respect to hidden, weight and bias; the gradients have the operands' types.  Logits are never stored:
     the forward pass keeps one logsumexp per row, the backward pass recomputes them in pieces of the vocabulary.  With
     ``reduction="none"`` and no gradient this is the negative log-probability of single tokens (serving).  While a HIP graph is
-    captured, no eager loss over the same leaves from the default stream may be alive: such a call is refused
-    (graphs that other operations keep alive are not seen: PyTorch's own rule for them holds).
+    captured, no eager loss over the same leaves from the default stream may be alive: such a call is refused, also where no gradient of it
+    would be taken (under ``torch.no_grad()`` it is not), and graphs that other operations keep alive are not seen: PyTorch's own
+    rule for them holds.
 
     Precision.  Logits: 16-bit operands are multiplied as they are; fp32 ones lose 2^-23 of themselves or 2^-38 of the largest entry of
     their own row.  Gradients: bf16 operands hold their bits down to 2^-28 of their tensor's largest entry; fp32 operands, and

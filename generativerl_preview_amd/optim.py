@@ -215,7 +215,8 @@ def orthogonalize(matrices, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7):
     """Newton-Schulz orthogonalisation: ``steps`` times ``X <- a X + (b A + c A A) X`` with ``A = X X^T``, from
     ``X = G / max(|G|_F, eps)`` (grlhip_orthogonalize).  ``matrices``: a tensor ``(..., rows, cols)`` -- every matrix of it on
     its own -- or a list of such tensors, fp32, bf16 or fp16, any strides; all of them go through one chain of launches.
-    Returns new tensors of the same shapes and type.  Products are fp32 (two fp16 pieces per value), rounded to the type once at the end.
+    Returns new tensors of the same shapes and type.  Products are fp32 (two fp16 pieces per value), rounded to the type once at the end;
+    the order of their sums depends on all matrices of the call, so that beside others a matrix' result may differ by roundings.
     No gradient is recorded.  A matrix that holds an infinity or NaN comes back as NaN, a zero matrix as zeros."""
     single = torch.is_tensor(matrices)
     tensors = [matrices] if single else list(matrices)

@@ -356,7 +356,8 @@ typedef enum { GRLHIP_ELEM_F32 = 0, GRLHIP_ELEM_BF16 = 1, GRLHIP_ELEM_F16 = 2 } 
  * `strides`: HOST [count][6] element strides (row, column) of src, dst and a third pair that is ignored here, or NULL for
  * dense rows.  Host arrays are read before the call returns.  src_i == dst_i with the same strides is allowed.
  * Coefficients that let a singular value pass 1.9 (or b s^2 + c s^4 pass 3.8) from 1 on: GRLHIP_ERR_UNSUPPORTED.
- * The results do not depend on the other matrices of the call.  Workspace: grlhip_orthogonalize_workspace_bytes, 256-byte aligned. */
+ * Tiles are chosen for the matrices of a call together, and with them the order of the sums: beside other matrices a matrix' result may differ by
+ * roundings.  The same call repeats its bits.  Workspace: grlhip_orthogonalize_workspace_bytes, 256-byte aligned. */
 size_t grlhip_orthogonalize_workspace_bytes(const int64_t* shapes, int32_t count);
 /* For the tests: the kinds of tiles (in the order of their sizes) that a call of these matrices takes in its three products, -1 where all
  * of them stay in one workgroup each. */
