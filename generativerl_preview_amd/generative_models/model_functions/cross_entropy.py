@@ -173,9 +173,10 @@ def linear_cross_entropy(hidden, weight, target, bias=None, row_weight=None, ign
     rule for them holds.
 
     Precision.  Logits: 16-bit operands are multiplied as they are; fp32 ones lose 2^-23 of themselves or 2^-38 of the largest entry of
-    their own row.  Gradients: bf16 operands hold their bits down to 2^-28 of their tensor's largest entry; fp32 operands, and
-    ``softmax - onehot`` beside them, lose 2^-22 of themselves or, in a row 2^d smaller than the largest one, 2^(d/2 - 38) of the
-    row's largest entry and of 1."""
+    their own row.  Gradients: bf16 operands hold their bits down to 2^-28 of their tensor's largest entry, and ``softmax - onehot``
+    beside them loses 2^-11 of itself or 2^-39; beside fp16 operands 2^-22 of itself or 2^-39; fp32 operands, and it beside them, lose
+    2^-22 of themselves or, in a row 2^d smaller than the largest one, 2^(d/2 - 38) of the row's largest entry and of 1.  In the weight's
+    gradient that is: of the largest row gradient."""
     if reduction not in _REDUCE:
         raise ValueError("reduction: expected 'none', 'mean' or 'sum', got %r" % (reduction,))
     if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1]:

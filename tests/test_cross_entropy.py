@@ -535,6 +535,37 @@ def test_gpu_captured_step_replays():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, F16])
+def test_gpu_captured_step_of_other_types_replays(dtype):
+    """What the forward call leaves for the backward call (fp32: the scales of the rows) follows the inputs of each replay."""
+    h, w, t, b, rw = inputs(190, 130, 700, dtype, seed=13)
+    h.requires_grad_(), w.requires_grad_()
+
+    def both():
+        loss = linear_cross_entropy(h, w, t, bias=b, row_weight=rw)
+        return [loss.detach(), *torch.autograd.grad(loss, [h, w])]
+
+    side = torch.cuda.Stream(device=DEV)
+    side.wait_stream(torch.cuda.current_stream(DEV))
+    with torch.cuda.stream(side):
+        both()
+    torch.cuda.current_stream(DEV).wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = both()
+    gen = torch.Generator().manual_seed(3)
+    for k in range(3):
+        with torch.no_grad():
+            h.copy_(torch.randn(h.shape, generator=gen) * 4.0 ** k)
+            w.mul_(0.25)
+            rw.copy_(torch.rand(rw.shape, generator=gen))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [x.clone() for x in held]
+        assert all(torch.equal(x, y) for x, y in zip(got, both()))
+
+
+@pytest.mark.gpu
 def test_gpu_capture_beside_a_live_eager_loss_is_refused(monkeypatch):
     """autograd would add up the leaves' gradients on the default stream, which cannot be captured."""
     h, w, t, _, _ = inputs(20, 64, 50, F32)
