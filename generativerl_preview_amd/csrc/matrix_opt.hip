@@ -663,11 +663,31 @@ Mat describe(const Call& c, int i) {
   return a;
 }
 
+// Whether a dense matrix that is written (parameter, momentum) lies over another one.
+bool dense_overlap(const Call& c) {
+  struct Span { const char *at, *end; bool written; };
+  std::vector<Span> spans;
+  for (int i = 0; i < c.count; ++i) {
+    const int64_t bytes = c.shapes[2 * i] * c.shapes[2 * i + 1] * 4;
+    if (bytes == 0) continue;
+    const void* const all[3] = {c.src[i], c.dst[i], c.buf[i]};
+    for (int k = 0; k < 3; ++k) spans.push_back({(const char*)all[k], (const char*)all[k] + bytes, k > 0});
+  }
+  std::sort(spans.begin(), spans.end(), [](const Span& x, const Span& y) { return x.at < y.at; });
+  const char *written = nullptr, *read = nullptr;   // where those so far end
+  for (const Span& s : spans) {
+    if (s.at < written || (s.written && s.at < read)) return true;
+    (s.written ? written : read) = std::max(s.written ? written : read, s.end);
+  }
+  return false;
+}
+
 template <class T, bool MUON>
 int run(const char* who, const Call& c, char* ws, size_t ws_bytes, hipStream_t stream) {
   const int64_t need = workspace_bytes(c.shapes, c.count);
   if (need > (int64_t)ws_bytes || (!ws && c.count > 0)) return set_error(GRLHIP_ERR_WORKSPACE, std::string(who) + ": workspace too small: need " + std::to_string(need));
   if ((size_t)ws & 255) return set_error(GRLHIP_ERR_INVALID, std::string(who) + ": the workspace must be aligned to 256 bytes");
+  if (MUON && !c.strides && dense_overlap(c)) return set_error(GRLHIP_ERR_INVALID, std::string(who) + ": parameters, gradients and momentum buffers must not share memory");
   // the matrices with the longest sums first, so that a launch does not end with them
   std::vector<int> order;
   for (int i = 0; i < c.count; ++i)

@@ -370,7 +370,7 @@ int grlhip_orthogonalize(const void* const* src, void* const* dst, const int64_t
  *   buf = momentum buf + (1 - momentum) grad;   u = nesterov ? (1 - momentum) grad + momentum buf : buf;
  *   param = keep param - rates_i orthogonalize(u)          (keep = 1 - lr * weight_decay; rates: HOST [count])
  * with the arguments of grlhip_orthogonalize; `strides`: HOST [count][6] of grad, param, buf, or NULL for dense rows.
- * Parameters, gradients and buffers must not overlap.  Workspace: grlhip_orthogonalize_workspace_bytes. */
+ * Parameters and buffers must not overlap themselves, each other or gradients (dense ones that do: GRLHIP_ERR_INVALID).  Workspace: grlhip_orthogonalize_workspace_bytes. */
 int grlhip_muon_step(float* const* params, const float* const* grads, float* const* momentum_buffers,
                      const int64_t* shapes, const int64_t* strides, const float* rates, int32_t count, double momentum,
                      int nesterov, float keep, int32_t steps, float a, float b, float c, float eps,

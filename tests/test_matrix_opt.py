@@ -560,3 +560,19 @@ def test_c_entry_points_check_their_arguments_without_a_gpu():
     for bad in (dict(p=null), dict(g=null), dict(b=null), dict(r=None), dict(mom=1.0), dict(mom=math.nan)):
         assert muon(**bad) == -1, bad
     assert lib.grlhip_orthogonalize_workspace_bytes((ctypes.c_int64 * 2)(-1, 2), 1) == 0
+
+
+def test_c_entry_point_refuses_dense_matrices_that_overlap():
+    """Each of these calls is refused before anything is launched: the memory is the host's."""
+    lib = L.lib()
+    shapes = (ctypes.c_int64 * 4)(8, 8, 4, 4)
+    need = lib.grlhip_orthogonalize_workspace_bytes(shapes, 2)
+    buf = (ctypes.c_char * (need + 8192))()
+    base = (ctypes.addressof(buf) + 255) // 256 * 256
+    at = base + (need + 255) // 256 * 256
+    rates = (ctypes.c_float * 2)(0.1, 0.1)
+    ptrs = lambda *offsets: (ctypes.c_void_p * 2)(*(at + o for o in offsets))  # noqa: E731
+    step = lambda p, g, b: lib.grlhip_muon_step(ptrs(*p), ptrs(*g), ptrs(*b), shapes, None, rates, 2, 0.9, 1, 1.0, 5, *ABC, 1e-7, base, need, None)  # noqa: E731
+    ok = ((0, 256), (512, 1024), (2048, 2304))         # 256 and 64 bytes each
+    for bad in (((0, 252), *ok[1:]), ((0, 0), *ok[1:]), (ok[0], (0, 1024), ok[2]), (ok[0], (512, 316), ok[2]), (ok[0], ok[1], (764, 2304)), (ok[0], ok[1], (2048, 2048))):
+        assert step(*bad) == -1 and b"share memory" in lib.grlhip_last_error(), bad
