@@ -77,6 +77,7 @@ PROTOTYPES = {
                                         ctypes.c_float, ctypes.c_float, _i64, _vp]),
     "grlhip_adam_step_counted": (ctypes.c_int, [_vp, _vp, _vp, _vp, _i64, ctypes.c_float, ctypes.c_float, ctypes.c_float,
                                                 ctypes.c_float, ctypes.c_float, _vp, ctypes.c_int, _vp]),
+    "grlhip_capture_id": (ctypes.c_uint64, [_vp]),
     "grlhip_orthogonalize_workspace_bytes": (_sz, [_vp, _i32]),
     "grlhip_orthogonalize": (ctypes.c_int, [_vp, _vp, _vp, _vp, _i32, ctypes.c_int, _i32, _f, _f, _f, _f, _vp, _sz, _vp]),
     "grlhip_muon_step": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i32, ctypes.c_double, ctypes.c_int, _f, _i32, _f, _f, _f, _f,

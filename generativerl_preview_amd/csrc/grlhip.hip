@@ -132,6 +132,12 @@ int grlhip_device_available(void) {
   return (hipGetDeviceCount(&n) == hipSuccess && n > 0) ? 1 : 0;
 }
 
+uint64_t grlhip_capture_id(void* stream) {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  return hipStreamGetCaptureInfo((hipStream_t)stream, &status, &id) == hipSuccess && status == hipStreamCaptureStatusActive ? (uint64_t)id : 0;
+}
+
 int grlhip_plan_create(const grlhip_net_desc* net, grlhip_plan** out_plan) {
   if (!net || !out_plan) return fail(GRLHIP_ERR_INVALID, "null argument");
   std::string err;

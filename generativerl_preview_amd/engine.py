@@ -301,13 +301,15 @@ class NetPlan:
 def packed_image(owner, kept, named, dtype):
     """(key, packed weights) of a network for its present parameters: ``kept``, an earlier result, while no parameter was replaced or
     written in place, else anew.  Replays of a captured graph write parameters without moving their version counters, and meet
-    parameters that were written since: what is captured packs for itself (key None: memory of the graph, not to be kept), and
-    a network that was captured once trusts nothing that it kept."""
-    if next(iter(named.values())).is_cuda and torch.cuda.is_current_stream_capturing():
+    parameters that were written since: each capture packs for itself, and outside of one a network that was captured trusts
+    nothing that it kept."""
+    capture, dev = 0, next(iter(named.values())).device
+    if dev.type == "cuda" and torch.cuda.is_current_stream_capturing():
         owner._in_graph = True
-        return None, owner.plan.pack(named, dtype)
-    key = tuple((p.data_ptr(), p._version) for p in named.values())
-    return kept if kept is not None and kept[0] == key and not owner._in_graph else (key, owner.plan.pack(named, dtype))
+        capture = L.lib().grlhip_capture_id(_stream(dev))
+    key = (capture, *((p.data_ptr(), p._version) for p in named.values()))
+    usable = kept is not None and kept[0] == key and (capture or not owner._in_graph)
+    return kept if usable else (key, owner.plan.pack(named, dtype))
 
 
 class _DifferentiableForward(torch.autograd.Function):

@@ -96,9 +96,7 @@ class IntrinsicModel(nn.Module):
     def packed(self, dtype=None):
         dtype = self.compute_dtype if dtype is None else dtype
         named = self._named()
-        hit = packed_image(self, self._packed.get(dtype), named, dtype)
-        if hit[0] is not None:
-            self._packed[dtype] = hit
+        hit = self._packed[dtype] = packed_image(self, self._packed.get(dtype), named, dtype)
         return hit[1]
 
     # ------------------------------------------------------------------ reference API

@@ -68,10 +68,8 @@ class QNetwork(nn.Module):
 
     def packed(self, dtype=L.F32):
         named = self._named()
-        hit = packed_image(self, None if self.always_repack else self._packed, named, L.F32)
-        if hit[0] is not None:
-            self._packed = hit
-        return hit[1]
+        self._packed = packed_image(self, None if self.always_repack else self._packed, named, L.F32)
+        return self._packed[1]
 
     # ------------------------------------------------------------------ reference API
     def forward(self, action, state):

@@ -50,10 +50,8 @@ class VNetwork(nn.Module):
 
     def packed(self, dtype=L.F32):
         named = self._named()
-        hit = packed_image(self, self._packed, named, L.F32)
-        if hit[0] is not None:
-            self._packed = hit
-        return hit[1]
+        self._packed = packed_image(self, self._packed, named, L.F32)
+        return self._packed[1]
 
     def forward(self, state, condition=None):
         """:48-70"""

@@ -70,6 +70,9 @@ typedef struct grlhip_plan grlhip_plan; /* opaque; immutable after creation */
 const char* grlhip_last_error(void);
 /* 1 when a HIP device is usable by this process, else 0 (never fails). */
 int grlhip_device_available(void);
+/* What tells a capture of `stream` into a graph from every other capture; 0 while it is not captured.  Memory that a captured call
+ * fills is good for that capture only. */
+uint64_t grlhip_capture_id(void* stream);
 
 /* Replaces: module construction through get_module()/get_encoder(),
  * grl/generative_models/intrinsic_model.py:19-52.  Builds the op program, the activation-slab

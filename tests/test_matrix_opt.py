@@ -383,6 +383,36 @@ def test_gpu_a_captured_forward_pass_follows_the_weights(make, inputs):
     assert not twin._in_graph and torch.equal(twin(*x), want)
 
 
+@pytest.mark.gpu
+def test_gpu_a_capture_packs_once_and_for_itself(monkeypatch):
+    """The calls of one capture share a packed image; another capture does not read it, and eager calls do not either."""
+    torch.manual_seed(13)
+    net, x = _value_net(), torch.rand(50, 17, device=DEV)
+    packs, pack = [], type(net.plan).pack
+    monkeypatch.setattr(type(net.plan), "pack", lambda *a: packs.append(1) or pack(*a))
+    with torch.no_grad():
+        net(x), net(x)
+        assert len(packs) == 1
+        graphs, held = [], []
+        for k in range(2):
+            graphs.append(torch.cuda.CUDAGraph())
+            with torch.cuda.graph(graphs[-1]):
+                held.append((net(x), net(x)))
+            assert len(packs) == 2 + k
+        graphs[1].replay()             # the second graph alone: nothing of the first one's
+        torch.cuda.synchronize()
+        want = net(x)
+        assert len(packs) == 4 and all(torch.equal(y, want) for y in held[1])
+        for p in net.parameters():
+            p.mul_(1.5)
+        want = net(x)
+        for g, ys in zip(graphs, held):
+            g.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(y, want) for y in ys)
+    assert L.lib().grlhip_capture_id(ctypes.c_void_p(torch.cuda.current_stream(DEV).cuda_stream)) == 0
+
+
 # groups that between them take every kind of tile in every product, with rests in all of them
 GROUPS = [(1, (65, 65)), (6, (660, 540)), (1, (193, 2)), (1, (2, 225)), (1, (226, 225)), (24, (195, 198)), (24, (225, 266)), (24, (292, 308)),
           (12, (518, 523)), (24, (454, 464)), (24, (587, 594)), (12, (356, 370)), (24, (169, 161)), (24, (676, 33)), (8, (98, 3085)), (24, (1696, 97)),
